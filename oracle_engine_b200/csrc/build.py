@@ -57,6 +57,7 @@ LIBRARIES = {
     "attention_tc5": ("attention_tcgen05.cu", []),
     "attention_split_tc": ("attention_split_mma.cu", []),
     "head_matmul_tc": ("head_matmul_mma.cu", []),
+    "attention_kv8": ("attention_kv8.cu", []),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}
@@ -199,7 +200,7 @@ def build_all(names=None, verbose: bool = True) -> list[Path]:
     for n in names:
         if n == "attention_tc":
             jobs.extend((n, {"OE_HD": hd}) for hd in DEFAULT_HEAD_DIMS)
-        elif n == "attention_tc5":
+        elif n in ("attention_tc5", "attention_kv8"):
             jobs.extend((n, {"OE_HD": hd}) for hd in (64, 128))
         elif n == "attention_split_tc":
             jobs.extend((n, {"OE_DK": dk, "OE_DV": dv}) for dk, dv in ((64, 128), (128, 128)))

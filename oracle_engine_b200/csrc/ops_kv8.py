@@ -1,0 +1,211 @@
+"""The 8-bit paged cache and the attention that reads it, and the attention of sequences that begin with the same pages
+(csrc/attention_kv8.cu, one library per head size).
+
+A `cache` argument is one cache entry: a pair (codes [pages, 2, KVH, PAGE, hd] int8 or float8_e4m3fn, scales float32 [pages, 2, KVH,
+PAGE]), or, where a function says so, the 16-bit entry [pages, 2, KVH, PAGE, hd] bfloat16.  A row (one token's key or value of one KV
+head) reads as code * scale: with a the row's largest magnitude and c = 127 or 448, code = row * c / a to the nearest code (ties to
+even) and scale = a / c.  Keys are turned by their position and rounded to bfloat16 before that.  A row with an infinite or
+undefined value reads as undefined.
+
+`ahead`: the caller knows that another kernel lies between whatever wrote the cache's earlier rows and this call, as in a model's
+step, where the projections do; the kernel then asks for those rows while the kernel before it still runs.
+"""
+from __future__ import annotations
+
+from ctypes import c_float, c_int, c_longlong, c_void_p
+
+import torch
+
+from . import build as _build
+from . import ops
+from .ops import PAGE, KernelError
+
+HEAD_DIMS = (64, 128)
+CODE_TYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+_KINDS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
+_libs: dict = {}
+
+
+def _lib(head_dim: int):
+    lib = _libs.get(head_dim)
+    if lib is None:
+        if head_dim not in HEAD_DIMS:
+            raise KernelError(f"the 8-bit cache's kernels take heads of {HEAD_DIMS}, not {head_dim}")
+        lib = _build.load("attention_kv8", {"OE_HD": head_dim})
+        P, I, F, L = c_void_p, c_int, c_float, c_longlong
+        lib.oe_kv8_write.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, I, P]
+        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, P, I, P, I, P]
+        lib.oe_attn_kv8_prefix.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, F, P, P, P, I, I, I, P, I, P]
+        for f in (lib.oe_kv8_write, lib.oe_attn_kv8, lib.oe_attn_kv8_prefix):
+            f.restype = c_int
+        _libs[head_dim] = lib
+    return lib
+
+
+def supported(head_dim: int, n_heads: int, n_kv_heads: int) -> bool:
+    return head_dim in HEAD_DIMS and n_kv_heads >= 1 and n_heads % n_kv_heads == 0 and n_heads >= n_kv_heads
+
+
+def _cache_args(what: str, cache, n_kv_heads: int, head_dim: int, allow_16: bool) -> tuple:
+    """(kind, rows, scales or None) of a cache entry."""
+    rows, scales = (cache, None) if isinstance(cache, torch.Tensor) else cache
+    if rows.dtype not in _KINDS or (scales is None) != (rows.dtype == torch.bfloat16):
+        raise KernelError(f"{what}: a cache entry is (codes, scales) with int8 or float8_e4m3fn codes, or a bfloat16 tensor")
+    if scales is None and not allow_16:
+        raise KernelError(f"{what}: codes and scales expected")
+    if tuple(rows.shape[1:]) != (2, n_kv_heads, PAGE, head_dim) or not rows.is_contiguous():
+        raise KernelError(f"{what}: cache entry must be contiguous [pages, 2, KVH, PAGE, head_dim]")
+    if scales is not None and (scales.dtype != torch.float32 or not scales.is_contiguous() or scales.shape != rows.shape[:-1]):
+        raise KernelError(f"{what}: scales must be contiguous float32 [pages, 2, KVH, PAGE]")
+    return _KINDS[rows.dtype], rows, scales
+
+
+def _check_heads(what: str, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+    if not supported(head_dim, n_heads, n_kv_heads):
+        raise KernelError(f"{what}: {n_heads} heads over {n_kv_heads} KV heads of {head_dim} are outside what the kernels take "
+                          f"(head sizes {HEAD_DIMS}, heads a multiple of the KV heads)")
+
+
+def _check_rows(what: str, qkv, cos, sin, width: int, head_dim: int) -> None:
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or qkv.stride(0) % 8 or \
+            qkv.data_ptr() % 16:
+        raise KernelError(f"{what}: qkv must be bfloat16 [T, {width}] with rows of multiples of 16 bytes")
+    if (cos is None) != (sin is None) or cos is not None and (
+            cos.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != head_dim // 2 or not cos.is_contiguous()
+            or sin.dtype != torch.float32 or sin.shape != cos.shape or not sin.is_contiguous()):
+        raise KernelError(f"{what}: cos/sin must be contiguous float32 [max_pos, head_dim/2]")
+
+
+def _here(what: str, *tensors) -> None:
+    """Every tensor is on the current device, whose stream the kernel is launched on."""
+    ops._dev(*tensors)
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != dev:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+def _check_step(what: str, out, qkv, cos, tables, ctx, n_heads: int, head_dim: int) -> None:
+    for t, n in ((tables, "tables"), (ctx.cu_q, "cu_q"), (ctx.seq_start, "seq_start"), (ctx.seq_qlen, "seq_qlen")):
+        ops._i32(t, f"{what}: {n}")
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != (qkv.shape[0], n_heads * head_dim) or not out.is_contiguous():
+        raise KernelError(f"{what}: out must be contiguous bfloat16 [T, {n_heads * head_dim}]")
+    if tables.dim() != 2 or tables.shape[0] < ctx.n_seqs or ctx.cu_q.numel() < ctx.n_seqs + 1 or \
+            ctx.seq_start.numel() < ctx.n_seqs or ctx.seq_qlen.numel() < ctx.n_seqs:
+        raise KernelError(f"{what}: the step's tables are shorter than its {ctx.n_seqs} sequences")
+    longest = getattr(ctx, "max_kvlen", 0)
+    if longest > tables.shape[1] * PAGE or cos is not None and longest > cos.shape[0]:
+        raise KernelError(f"{what}: a sequence of {longest} tokens is longer than its page table or the position tables")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+    """Keys (turned at each token's position; cos/sin float32 [max_pos, hd/2] or None) and values of the step's tokens into the
+    8-bit cache.  qkv [T, (H + 2 KVH) hd] is left as it is; tok_seq < 0: a padding row; a page outside the cache: nothing is
+    written."""
+    what = "kv8_write"
+    _check_heads(what, n_heads, n_kv_heads, head_dim)
+    kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
+    _here(what, qkv, cos, sin, codes, scales, tables, tok_seq, tok_pos)
+    _check_rows(what, qkv, cos, sin, (n_heads + 2 * n_kv_heads) * head_dim, head_dim)
+    for t, n in ((tables, "tables"), (tok_seq, "tok_seq"), (tok_pos, "tok_pos")):
+        ops._i32(t, f"{what}: {n}")
+    T = qkv.shape[0]
+    if tables.dim() != 2 or tok_seq.numel() < T or tok_pos.numel() < T:
+        raise KernelError(f"{what}: fewer places than the {T} tokens")
+    if T == 0:
+        return
+    ops._check(_lib(head_dim).oe_kv8_write(
+        kind, qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+        tables.data_ptr(), tables.shape[1], tok_seq.data_ptr(), tok_pos.data_ptr(), T, n_heads, n_kv_heads, ops._stream()), what)
+
+
+def decode_cluster(n_seqs: int, n_kv_heads: int, context_class: int, sm_count: int | None = None) -> int:
+    """How many CTAs (a thread-block cluster) share the keys of one (sequence, KV head) of a step of single tokens."""
+    if context_class < 1:
+        return 1
+    budget = sm_count or ops.sm_count()
+    for cr in (8, 4, 2):
+        if n_seqs * n_kv_heads * cr <= budget:
+            return cr
+    return 1
+
+
+def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float,
+                  has_kv: bool = True, ahead: bool = False, cluster: int | None = None) -> None:
+    """Rotation, cache write (has_kv) and attention of the step's tokens over the 8-bit cache: out[t] is the attention of token t's
+    query heads over its sequence's keys up to its own position (window 0: all of them, n > 0: the last n, -n: those of the
+    chunk of n positions it lies in), as the cache keeps them, the step's own among them.
+
+    qkv bfloat16 [T, (H + 2 KVH) hd] (or [T, H hd] when has_kv is false: the rows are in the cache) before rotation, left as it
+    is; out bfloat16 [T, H hd]; ctx: the step (StepContext: cu_q, seq_start, seq_qlen, tok_seq, tok_pos, n_seqs, max_qlen,
+    all_decode).  A step of one token a sequence is one launch, any other a write and an attention."""
+    what = "attention_kv8"
+    _check_heads(what, n_heads, n_kv_heads, head_dim)
+    kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
+    _here(what, out, qkv, cos, sin, codes, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen)
+    _check_rows(what, qkv, cos, sin, (n_heads + (2 * n_kv_heads if has_kv else 0)) * head_dim, head_dim)
+    _check_step(what, out, qkv, cos, tables, ctx, n_heads, head_dim)
+    T = qkv.shape[0]
+    if T == 0 or ctx.n_seqs == 0:
+        return
+    single = bool(ctx.all_decode) and T == ctx.n_seqs
+    if has_kv and not single:
+        kv8_write(qkv, cos, sin, cache, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
+    if cluster is None:
+        cluster = decode_cluster(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0)) if single else 1
+    ops._check(_lib(head_dim).oe_attn_kv8(
+        kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(),
+        int(has_kv and single), codes.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
+        ctx.seq_qlen.data_ptr(), ctx.n_seqs, 1 if single else max(1, ctx.max_qlen), n_heads, n_kv_heads, int(window), float(scale),
+        int(cluster), None, 0, None, int(ahead), ops._stream()), what, {"cluster": int(cluster)})
+
+
+def prefix_splits(n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, sm_count: int | None = None) -> int:
+    """Into how many parts the pages of a prefix are cut."""
+    tiles = max(1, (n_members * group + 15) // 16) * n_kv_heads
+    return max(1, min(max_pages, 2 * (sm_count or ops.sm_count()) // tiles, 32))
+
+
+def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
+                     has_kv: bool = True, ahead: bool = False) -> None:
+    """A step of one token a sequence in which groups of sequences begin with the same pages: rotation, cache write (has_kv) and
+    attention over all keys, as attention_kv8 with window 0, but a group's common pages are read once for all of its members.
+    cache: the 8-bit pair or the 16-bit entry.
+
+    prefix: n_groups and n_members (host numbers, or bounds for them: what first and members hold beyond the real ones are
+    groups without members), max_pages (the most pages a group has in common), and int32 tensors members (sequences in the order of
+    their groups), first [n_groups + 1] (where each group's members begin), pages [n_groups] (full pages that the group's
+    tables begin with), seq_pages [n_seqs] (those of the sequence's group, 0 for a sequence in none)."""
+    what = "attention_shared"
+    _check_heads(what, n_heads, n_kv_heads, head_dim)
+    kind, rows, scales = _cache_args(what, cache, n_kv_heads, head_dim, True)
+    lists = (prefix.members, prefix.first, prefix.pages, prefix.seq_pages)
+    _here(what, out, qkv, cos, sin, rows, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen, *lists)
+    _check_rows(what, qkv, cos, sin, (n_heads + (2 * n_kv_heads if has_kv else 0)) * head_dim, head_dim)
+    _check_step(what, out, qkv, cos, tables, ctx, n_heads, head_dim)
+    B = ctx.n_seqs
+    if not ctx.all_decode or qkv.shape[0] != B:
+        raise KernelError(f"{what}: one token a sequence expected")
+    for t, n, least in zip(lists, ("members", "first", "pages", "seq_pages"), (prefix.n_members, prefix.n_groups + 1, prefix.n_groups, B)):
+        ops._i32(t, f"{what}: {n}")
+        if t.numel() < least:
+            raise KernelError(f"{what}: {n} holds {t.numel()} numbers, {least} are needed")
+    if B == 0:
+        return
+    lib, group = _lib(head_dim), n_heads // n_kv_heads
+    splits = prefix_splits(prefix.n_members, prefix.n_groups, group, n_kv_heads, max(1, prefix.max_pages))
+    partial = torch.empty(B * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device)
+    step = (rows.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr())
+    if prefix.n_groups > 0 and prefix.n_members > 0:
+        ops._check(lib.oe_attn_kv8_prefix(
+            kind, qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), *step, n_heads, n_kv_heads,
+            float(scale), prefix.members.data_ptr(), prefix.first.data_ptr(), prefix.pages.data_ptr(), prefix.n_groups,
+            prefix.n_members, splits, partial.data_ptr(), int(ahead), ops._stream()), "attention_shared_prefix", {"splits": splits})
+    ops._check(lib.oe_attn_kv8(
+        kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), int(has_kv),
+        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 1, prefix.seq_pages.data_ptr(), splits,
+        partial.data_ptr(), int(ahead), ops._stream()), what)

@@ -12,6 +12,10 @@ group as soon as they lie in chunks the next query has left, so their pools can 
 handed out again; nothing is cleared, since a position is readable only after it has
 been written (each sequence's length bounds every read).
 
+A sequence may begin with another one's pages (`fork`): both slots' tables then name the same pages, which nobody writes any more,
+and a page returns to its pool when the last of its holders has given it back.  Slots forked from one another at the same
+length carry the same mark (`prefix`), by which an attention can read the common pages once for all of them.
+
 The reference's cache is one sequence's [layers][ctx][kv_heads*head_dim] float32 arrays
 with the context fixed at 512 (core/model.hpp:29-54, core/model.cpp:64).
 """
@@ -37,8 +41,13 @@ class CacheView:
 
     @property
     def kv(self):
-        """Attention's tensor [pages, 2, kv_heads, PAGE, head_dim]."""
-        return None if self.tensors is None else self.tensors["kv"]
+        """Attention's tensor [pages, 2, kv_heads, PAGE, head_dim], or an 8-bit cache's pair (codes of that shape, scales float32
+        [pages, 2, kv_heads, PAGE])."""
+        if self.tensors is None:
+            return None
+        if "codes" in self.tensors:
+            return self.tensors["codes"], self.tensors["scales"][..., 0]
+        return self.tensors["kv"]
 
 
 def page_shape(per_token_shape) -> tuple:
@@ -62,12 +71,13 @@ class CacheGroup:
         self.storage: dict | None = None        # tensor name -> [entries, pages, *outer, PAGE, inner]
 
     def allocate(self, dtype, device) -> None:
-        self.storage = {name: torch.zeros((len(self.entries), self.pool.n) + page_shape(shape), dtype=dtype,
+        own = dict(self.need.dtypes)
+        self.storage = {name: torch.zeros((len(self.entries), self.pool.n) + page_shape(shape), dtype=own.get(name, dtype),
                                           device=device)
                         for name, shape in self.need.tensors}
 
     def bytes_per_page(self, itemsize: int) -> int:
-        return len(self.entries) * PAGE * self.need.elements_per_token() * itemsize
+        return len(self.entries) * PAGE * self.need.bytes_per_token(itemsize)
 
 
 def pages_for(n_tokens: int) -> int:
@@ -90,6 +100,9 @@ class KVCache:
         self.slots = SlotAllocator(self.n_slots)
         self.lengths = np.zeros(self.n_slots, dtype=np.int64)
         self.version = 0                       # grows whenever any page table changes
+        # per slot: (a mark that slots with the same first pages share, how many pages), or None
+        self.prefix: list = [None] * self.n_slots
+        self._prefix_marks = 0
         self.groups: list[CacheGroup] = []
         self.entry_group: dict[int, tuple[int, int]] = {}      # entry -> (group, index in group)
         by_need: dict = {}
@@ -135,7 +148,32 @@ class KVCache:
             g.lo[slot] = g.hi[slot] = 0
         self.version += 1
         self.lengths[slot] = 0
+        self.prefix[slot] = None
         self.slots.free(slot)
+
+    def fork(self, slot: int) -> int:
+        """A new slot that begins with everything `slot` holds: the same pages, which neither writes from now on.  The length has
+        to be a whole number of pages, since a page that is still being filled cannot have two writers."""
+        if not self.slots.is_held(slot):
+            raise ValueError(f"slot {slot} is not held")
+        length = int(self.lengths[slot])
+        if length == 0 or length % PAGE:
+            raise ValueError(f"slot {slot} holds {length} tokens: only whole pages of {PAGE} tokens can be shared")
+        n = length // PAGE
+        new = self.alloc_slot()
+        for g in self.groups:
+            row = g.tables[slot, :n]
+            g.pool.share(row[row >= 0].tolist())
+            g.tables[new, :n] = row
+            g.lo[new], g.hi[new] = min(int(g.lo[slot]), n), n
+        self.lengths[new] = length
+        mark = self.prefix[slot]
+        if mark is None or mark[1] != n:
+            self._prefix_marks += 1
+            mark = self.prefix[slot] = (self._prefix_marks, n)
+        self.prefix[new] = mark
+        self.version += 1
+        return new
 
     def length(self, slot: int) -> int:
         return int(self.lengths[slot])
@@ -219,9 +257,10 @@ class KVCache:
         self.slots.check()
         for g in self.groups:
             g.pool.check()
-            held = g.tables[g.tables >= 0]
-            assert len(held) == len(set(held.tolist())), "a page is mapped twice"
-            assert set(held.tolist()) == g.pool._used, "page tables and pool disagree"
+            pages, counts = np.unique(g.tables[g.tables >= 0], return_counts=True)
+            assert all(c == g.pool.holders(p) for p, c in zip(pages.tolist(), counts.tolist())), \
+                "a page is mapped twice, or not as often as it has holders"
+            assert set(pages.tolist()) == g.pool._used, "page tables and pool disagree"
             for s in range(self.n_slots):
                 if not self.slots.is_held(s):
                     assert (g.tables[s] < 0).all(), f"free slot {s} still maps pages"

@@ -49,12 +49,14 @@ class SlotAllocator:
 
 
 class PagePool:
-    """Pages 0..n-1 of one cache group."""
+    """Pages 0..n-1 of one cache group.  A page in use has one holder, or more after `share`; it is free again when the last
+    of them has released it."""
 
     def __init__(self, n_pages: int):
         self.n = n_pages
         self._free = list(range(n_pages - 1, -1, -1))
         self._used = set()
+        self._more = {}                  # page -> holders beyond the first
 
     def alloc(self) -> int:
         if not self._free:
@@ -79,12 +81,37 @@ class PagePool:
         if len(set(pages)) != len(pages) or not self._used.issuperset(pages):
             bad = next((p for p in pages if p not in self._used), None)
             raise ValueError(f"page {bad} is not in use (released twice?)" if bad is not None else "a page is released twice")
+        if self._more:
+            pages = [p for p in pages if not self._drop(p)]
         self._used.difference_update(pages)
         self._free.extend(pages)
+
+    def share(self, pages: list) -> None:
+        """One more holder for every page; nothing changes if one of them is not in use."""
+        if len(set(pages)) != len(pages) or not self._used.issuperset(pages):
+            raise ValueError("only pages in use can be shared, each once")
+        for p in pages:
+            self._more[p] = self._more.get(p, 0) + 1
+
+    def holders(self, page: int) -> int:
+        return (1 + self._more.get(page, 0)) if page in self._used else 0
+
+    def _drop(self, page: int) -> bool:
+        """True if the page keeps a holder."""
+        more = self._more.get(page, 0)
+        if more == 0:
+            return False
+        if more == 1:
+            del self._more[page]
+        else:
+            self._more[page] = more - 1
+        return True
 
     def release(self, page: int) -> None:
         if page not in self._used:
             raise ValueError(f"page {page} is not in use (released twice?)")
+        if self._drop(page):
+            return
         self._used.remove(page)
         self._free.append(page)
 
@@ -96,3 +123,4 @@ class PagePool:
         assert len(self._free) == len(set(self._free)), "a page is on the free list twice"
         assert not (set(self._free) & self._used), "a page is both free and used"
         assert len(self._free) + len(self._used) == self.n, "a page was lost"
+        assert self._used.issuperset(self._more) and all(n > 0 for n in self._more.values()), "a free page has holders"

@@ -57,5 +57,13 @@ class StateStore:
         self._rows = ops.row_table(tensors)
         ops.zero_rows(*self._rows, slot)
 
+    def copy(self, src: int, dst: int) -> None:
+        """Row `dst` of every tensor becomes a copy of row `src`."""
+        for slot in (src, dst):
+            if not 0 <= slot < self.n_slots:
+                raise IndexError(f"slot {slot} of {self.n_slots}")
+        for t in self._tensors.values():
+            t[dst].copy_(t[src])
+
     def total_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self._tensors.values())

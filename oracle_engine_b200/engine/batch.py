@@ -109,6 +109,51 @@ def context_class(n_tokens: int) -> int:
 
 
 @dataclass
+class SharedPrefixes:
+    """Which sequences of a step of single tokens begin with the same pages, as the attention takes it (csrc/ops_kv8.py:
+    attention_shared): host numbers, and the integers on the host (`arrays`) or as tensors."""
+    n_groups: int                   # a bound: groups beyond the real ones have no members
+    n_members: int                  # a bound
+    max_pages: int                  # a bound
+    arrays: tuple = ()              # numpy int32: members, first, pages, seq_pages
+    members: torch.Tensor | None = None
+    first: torch.Tensor | None = None
+    pages: torch.Tensor | None = None
+    seq_pages: torch.Tensor | None = None
+
+    @property
+    def shape(self):
+        """What a captured step's launches depend on."""
+        return self.n_groups, self.n_members, self.max_pages
+
+
+def shared_prefixes(marks: list, pad_seqs: int) -> SharedPrefixes | None:
+    """marks: per sequence the cache's (mark, pages) or None (cache/kv_cache.py: fork).  Groups are sequences with the same mark,
+    two at least; None if there is no group.  The host numbers are rounded up to few different ones, so that a captured step
+    serves many."""
+    groups: dict = {}
+    for b, m in enumerate(marks):
+        if m is not None:
+            groups.setdefault(m, []).append(b)
+    groups = {m: bs for m, bs in groups.items() if len(bs) > 1}
+    if not groups:
+        return None
+    up = lambda n: 1 << max(0, n - 1).bit_length()                       # noqa: E731
+    n_groups = up(len(groups))
+    members = np.zeros(pad_seqs, dtype=np.int32)
+    first, pages = np.zeros(n_groups + 1, dtype=np.int32), np.zeros(n_groups, dtype=np.int32)
+    seq_pages = np.zeros(pad_seqs, dtype=np.int32)
+    at = 0
+    for g, ((_, n), bs) in enumerate(groups.items()):
+        members[at:at + len(bs)] = bs
+        seq_pages[bs] = pages[g] = n
+        at += len(bs)
+        first[g + 1] = at
+    first[len(groups) + 1:] = at
+    return SharedPrefixes(n_groups, min(up(at), pad_seqs), up(int(pages.max())), (members, first, pages, seq_pages))
+
+
+@dataclass
 class StepContext:
     """Device-side view of a step, handed to every part."""
     n_tokens: int
@@ -130,16 +175,17 @@ class StepContext:
     n_real_tokens: int = 0          # without padding, and the two below of the sequences as they are (see StepPlan)
     longest: int = 0
     scan_chunks: int = 0
+    prefix: SharedPrefixes | None = None     # a step of single tokens whose sequences begin with the same pages
 
 
 class StepBuffers:
     """Pinned host staging and its device mirror for a step of fixed (padded) sizes."""
 
-    def __init__(self, n_tokens: int, n_seqs: int, n_want: int, table_shapes: list, device):
+    def __init__(self, n_tokens: int, n_seqs: int, n_want: int, table_shapes: list, device, prefix: SharedPrefixes | None = None):
         self.n_tokens, self.n_seqs, self.n_want = n_tokens, n_seqs, n_want
         self.table_shapes = list(table_shapes)
         sizes = [n_tokens, n_tokens, n_tokens, n_seqs, n_seqs, n_seqs, n_seqs + 1, n_want] + \
-                [a * b for a, b in table_shapes]
+                [a * b for a, b in table_shapes] + ([a.size for a in prefix.arrays] if prefix is not None else [])
         # 16-byte aligned sections so that vector loads of any section are legal
         self.offsets = []
         off = 0
@@ -163,7 +209,7 @@ class StepBuffers:
     def _dev_view(self, i):
         return self._dev_views[i]
 
-    def upload(self, plan: StepPlan, tables: list) -> StepContext:
+    def upload(self, plan: StepPlan, tables: list, prefix: SharedPrefixes | None = None) -> StepContext:
         """Fills the staging buffer from the plan and copies it to the device (one
         asynchronous copy on the current stream)."""
         if self._pending:                     # the previous copy must have read the staging buffer
@@ -177,11 +223,14 @@ class StepBuffers:
                 self._host_view(i)[:] = arr
         for j, tb in enumerate(tables):
             self._host_view(8 + j)[:] = tb.reshape(-1)
+        if prefix is not None:
+            for j, arr in enumerate(prefix.arrays):
+                self._host_view(8 + len(self.table_shapes) + j)[:] = arr
         self.dev.copy_(self.host, non_blocking=True)
         if self._copied is not None:
             self._copied.record(torch.cuda.current_stream())
             self._pending = True
-        return self.context(plan)
+        return self.context(plan, prefix)
 
     def update_decode(self, tokens, starts, n: int) -> None:
         """For a step of the same sequences as the last upload, each one token further: only
@@ -200,12 +249,14 @@ class StepBuffers:
     def bytes(self) -> int:
         return self.total * 4
 
-    def context(self, plan: StepPlan) -> StepContext:
+    def context(self, plan: StepPlan, prefix: SharedPrefixes | None = None) -> StepContext:
         v = self._dev_views
+        if prefix is not None:
+            prefix = SharedPrefixes(*prefix.shape, (), *v[8 + len(self.table_shapes):])
         tabs = list(self._dev_tables)
         return StepContext(
             n_tokens=self.n_tokens, n_seqs=self.n_seqs, n_want=self.n_want, token_ids=v[0], tok_seq=v[1],
             tok_pos=v[2], seq_slot=v[3], seq_start=v[4], seq_qlen=v[5], cu_q=v[6], want_rows=v[7], tables=tabs,
             max_qlen=plan.max_qlen, max_kvlen=plan.max_kvlen, all_decode=plan.all_decode,
             context_class=context_class(plan.max_kvlen), n_real_tokens=plan.n_real_tokens, longest=plan.longest,
-            scan_chunks=plan.scan_chunks)
+            scan_chunks=plan.scan_chunks, prefix=prefix)

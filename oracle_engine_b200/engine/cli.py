@@ -19,6 +19,8 @@ This library's own:
     --dtype bfloat16|float32 (default bfloat16)   --max-tokens <N> cache size in tokens
     --batch <N>     requests per batch (default: all at once)
     --step-tokens <N>  most prompt tokens per step (longer prompts go through in portions)
+    --cache-dtype int8|fp8  keep keys and values in 8 bits (default: the compute type)
+    --share-prefix  what prompts of a batch begin with alike is computed, kept and read once
     --profile       device time per kind of kernel, on standard error (runs without CUDA graphs)
     --random-weights <seed> --config <config.json>   run a configuration with seeded random weights
 Unknown option or missing -m / prompt: usage, exit 2.  Model cannot be loaded: exit 1.
@@ -38,6 +40,7 @@ USAGE = """Usage: {exe} -m <model_dir> (-p <prompt> | --tokens <ids>) [options]
   --tokens a,b,c  prompt as token ids (repeatable)
   --seed <N>  --repeat-penalty <f>  --repeat-last-n <N>  --stop-id <N>  --ignore-eos
   --dtype bfloat16|float32  --max-tokens <N>  --batch <N>  --step-tokens <N>  --profile
+  --cache-dtype int8|fp8  --share-prefix
   --random-weights <seed> --config <config.json>
   --no-stream     print the answer in one block
 """
@@ -49,7 +52,7 @@ def main(argv=None) -> int:
     from ..sampling.params import GenParams
     params = GenParams()
     opt = {"model": "", "prompt": "", "tokens": [], "stream": True, "dtype": "bfloat16", "max_tokens": 0,
-           "batch": None, "stop": [], "random": None, "config": "", "step_tokens": None, "profile": False}
+           "batch": None, "stop": [], "random": None, "config": "", "step_tokens": None, "profile": False, "cache_dtype": None, "share": False}
     i = 0
 
     def val(name):
@@ -95,6 +98,10 @@ def main(argv=None) -> int:
                 opt["batch"] = int(val(k))
             elif k == "--step-tokens":
                 opt["step_tokens"] = int(val(k))
+            elif k == "--cache-dtype":
+                opt["cache_dtype"] = val(k)
+            elif k == "--share-prefix":
+                opt["share"] = True
             elif k == "--profile":
                 opt["profile"] = True
             elif k == "--random-weights":
@@ -129,11 +136,11 @@ def main(argv=None) -> int:
             raw = json.loads(open(opt["config"]).read())
             config = get_architecture(architecture_name(raw)).config_cls.from_dict(raw)
             engine = Engine.from_config(config, seed=opt["random"], dtype=opt["dtype"], max_tokens=max_tokens,
-                                        use_graphs=not opt["profile"])
+                                        use_graphs=not opt["profile"], cache_dtype=opt["cache_dtype"])
             tok = None
         else:
             engine = Engine.from_pretrained(opt["model"], dtype=opt["dtype"], max_tokens=max_tokens,
-                                            use_graphs=not opt["profile"])
+                                            use_graphs=not opt["profile"], cache_dtype=opt["cache_dtype"])
             tok = Tokenizer.from_folder(opt["model"], engine.spec.bos_id)
     except Exception as e:                                   # noqa: BLE001 - reported, exit code 1 as the reference
         sys.stderr.write(f"error: failed to load model '{opt['model'] or opt['config']}': {e}\n")
@@ -172,11 +179,11 @@ def main(argv=None) -> int:
             from .profile import KernelProfile
             with KernelProfile() as prof:
                 outs = engine.generate(prompts, params, batch_size=opt["batch"], on_token=on_token,
-                                       max_step_tokens=opt["step_tokens"])
+                                       max_step_tokens=opt["step_tokens"], share_prefix=opt["share"])
             prof.report(sys.stderr)
         else:
             outs = engine.generate(prompts, params, batch_size=opt["batch"], on_token=on_token,
-                                   max_step_tokens=opt["step_tokens"])
+                                   max_step_tokens=opt["step_tokens"], share_prefix=opt["share"])
     except Exception as e:                                   # noqa: BLE001 - a kernel's error flag included
         sys.stderr.write(f"error: {e}\n")
         return 1

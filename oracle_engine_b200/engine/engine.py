@@ -28,25 +28,41 @@ from ..weights.random_init import RandomSource
 from ..weights.safetensors_io import ModelFiles
 from .batch import SequenceStep
 from .generate import GenerationResult, run_generation
-from .runtime import Runtime, parse_dtype
+from .runtime import Runtime, parse_cache_dtype, parse_dtype
 from .step import Stepper
+
+
+def check_cache_form(model, rt) -> None:
+    """Refuses an 8-bit cache for a model one of whose mixers keeps something per token and has no such form."""
+    if rt.cache_codes is None:
+        return
+    for i, e in enumerate(model.schedule):
+        mixer = model.layers[e.layer].mixer
+        if mixer.cache_need() is not None and not mixer.quantised_cache:
+            raise ValueError(f"layer {i}: a {mixer.kind!r} mixer has no 8-bit cache")
 
 
 class Engine:
     def __init__(self, config, arch, source, dtype="bfloat16", max_tokens: int = 8192,
                  max_seq_len: int | None = None, device="cuda:0", use_graphs: bool = True,
-                 tensor_cores: bool = True, n_slots: int | None = None):
+                 tensor_cores: bool = True, n_slots: int | None = None, cache_dtype=None):
+        """cache_dtype: None, a cache of the compute type; "int8" or "fp8", keys and values kept as 8-bit codes with a float32
+        scale per token and KV head (about half the bytes; csrc/ops_kv8.py says how they are rounded).  For bfloat16 models whose
+        caches are all those of `gqa_attention` with heads of 64 or 128; others are refused."""
         ops.require_cuda()
         self.config = config
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
-        self.rt = Runtime(parse_dtype(dtype), self.device, tensor_cores)
+        self.rt = Runtime(parse_dtype(dtype), self.device, tensor_cores, parse_cache_dtype(cache_dtype))
+        if self.rt.cache_codes is not None and not (self.rt.dtype == torch.bfloat16 and tensor_cores):
+            raise ValueError("an 8-bit cache goes with bfloat16 on the tensor cores")
         page = ops.PAGE
         max_tokens = max(page, (int(max_tokens) + page - 1) // page * page)
         limit = arch.build_spec(config, None).max_positions        # the architecture's own limit
         self.max_seq_len = min(int(max_seq_len or limit), limit, max_tokens)
         self.spec = arch.build_spec(config, self.max_seq_len)
         self.model = DecoderModel(self.spec, self.rt)
+        check_cache_form(self.model, self.rt)
         load_weights(self.model, source(self.model) if callable(source) else source)
         self.cache = KVCache(self.model.cache_needs(), max_tokens, self.max_seq_len, self.rt.dtype, self.device,
                              n_slots=n_slots)
@@ -88,6 +104,14 @@ class Engine:
         self.state.reset(slot)
         return slot
 
+    def fork(self, slot: int) -> int:
+        """A new slot that goes on from where `slot` is: it has the same cached pages (shared, not copied) and a copy of the
+        recurrent layers' and the sampler's state.  `slot` has to hold a whole number of pages of 64 tokens.  Steps of single
+        tokens of slots forked from one another at the same length read the common pages once for all of them."""
+        new = self.cache.fork(slot)
+        self.state.copy(slot, new)
+        return new
+
     def free(self, slot: int) -> None:
         self.cache.free_slot(slot)
 
@@ -109,19 +133,21 @@ class Engine:
     # ------------------------------------------------------------------ generation
     def generate(self, prompts, params: GenParams | None = None, batch_size: int | None = None,
                  on_token=None, return_results: bool = False, lookahead: bool = True,
-                 max_step_tokens: int | None = None):
+                 max_step_tokens: int | None = None, share_prefix: bool = False):
         """prompts: lists of token ids.  Returns the new tokens of each request (or
         GenerationResult objects with the finish reason).  lookahead: the next step is queued
         before the host has read the last tokens (same tokens either way; `on_token` then hears
         of a token while the step after it is already running).  max_step_tokens: the most
         prompt tokens a step takes; longer prompts go through in portions (bounds the memory
-        of a step's activations; None: every prompt whole).  Raises RuntimeError if a kernel
+        of a step's activations; None: every prompt whole).  share_prefix: whole pages of 64 tokens with which prompts of a batch
+        begin alike go through the model once, are kept once, and are read once a step for all of these requests (the results
+        may round differently).  Raises RuntimeError if a kernel
         reported an error during a batch (the tokens of that batch are then not returned)."""
         params = params or GenParams()
         backend = _Backend(self)
         backend.supports_lookahead = bool(lookahead)
         results = run_generation(backend, prompts, params, batch_size, self.spec.stop_ids, on_token,
-                                 max_step_tokens)
+                                 max_step_tokens, share_prefix)
         return results if return_results else [r.tokens for r in results]
 
 
@@ -143,6 +169,14 @@ class _Backend:
 
     def free(self, slot):
         self.e.free(slot)
+
+    def alloc_prefix(self):
+        return self.e.alloc()
+
+    def alloc_behind(self, prefix_slot, request_index, prompt, params):
+        slot = self.e.fork(prefix_slot)
+        self.e.sampler.start_sequence(slot, params.seed + request_index, prompt, params)
+        return slot
 
     def check(self):
         self.e.check_device_errors()

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass, field
 
+from ..csrc.ops import PAGE
 from .batch import SequenceStep
 
 
@@ -43,6 +44,10 @@ class GenerationBackend:
     # Optional: check() raises if the device reported an error since the last call (a bounded wait
     # that ran out, a token id outside the vocabulary); the loop calls it once per batch.
 
+    # A backend whose sequences can begin with another's cache has, for `share_prefix`:
+    #   alloc_prefix() -> slot                                          an empty slot for the common tokens
+    #   alloc_behind(prefix_slot, request_index, prompt, params) -> slot    as alloc, with the prefix slot's tokens in it
+
     # A backend that can run one step ahead of the host sets `supports_lookahead` and has:
     #   sample_async(logits, slots, params) -> handle     sampling started, tokens not yet read
     #   read(handle) -> list                               the tokens of that sampling, on the host
@@ -51,13 +56,42 @@ class GenerationBackend:
     supports_lookahead = False
 
 
+def common_prefixes(prompts: list, requests: list) -> list:
+    """[(requests, tokens)] of the requests whose prompts begin alike: those with the same first page, two at least, and how many
+    tokens all of them have in common, in whole pages, at least one token of every prompt left."""
+    groups: dict = {}
+    for i in requests:
+        if len(prompts[i]) > PAGE:
+            groups.setdefault(tuple(prompts[i][:PAGE]), []).append(i)
+    found = []
+    for members in groups.values():
+        if len(members) < 2:
+            continue
+        base = prompts[members[0]]
+        n = min(len(prompts[i]) for i in members) - 1
+        for i in members[1:]:
+            p, lo, hi = prompts[i], 0, n
+            while lo < hi:                               # the largest k <= n with equal first k tokens
+                mid = (lo + hi + 1) // 2
+                if p[lo:mid] == base[lo:mid]:
+                    lo = mid
+                else:
+                    hi = mid - 1
+            n = lo
+        found.append((members, n // PAGE * PAGE))
+    return found
+
+
 def run_generation(backend: GenerationBackend, prompts, params, batch_size: int | None = None,
-                   stop_ids=(), on_token=None, max_step_tokens: int | None = None) -> list[GenerationResult]:
+                   stop_ids=(), on_token=None, max_step_tokens: int | None = None,
+                   share_prefix: bool = False) -> list[GenerationResult]:
     """max_step_tokens: the most prompt tokens one step takes (None: every prompt whole, in the
     batch's first step).  With a limit, prompts are cut into portions, in request order: a
     portion that does not end its prompt wants no logits; a request whose prompt is complete
     decodes one token per step in the same steps in which later requests still bring portions;
-    a request that got no room in a step is left out of it.  The tokens are the same either way."""
+    a request that got no room in a step is left out of it.  The tokens are the same either way.
+    share_prefix: what prompts of a batch have in common (`common_prefixes`) goes through the model once, in steps of its own
+    before the batch's first one, and the requests begin behind it."""
     params.validate()
     prompts = [list(p) for p in prompts]
     for i, p in enumerate(prompts):
@@ -78,14 +112,28 @@ def run_generation(backend: GenerationBackend, prompts, params, batch_size: int 
         batch = list(range(b0, min(len(prompts), b0 + batch_size)))
         slots: dict[int, int] = {}
         try:
+            fed = {i: 0 for i in batch}            # prompt tokens given to the step function so far
+            if share_prefix and params.n_predict > 0:
+                for members, n in common_prefixes(prompts, batch):
+                    base = backend.alloc_prefix()
+                    try:
+                        common = prompts[members[0]][:n]
+                        portion = max_step_tokens or n
+                        for at in range(0, n, portion):
+                            backend.step([SequenceStep(base, common[at:at + portion], [])])
+                        for i in members:
+                            slots[i] = backend.alloc_behind(base, i, prompts[i], params)
+                            fed[i] = n
+                    finally:
+                        backend.free(base)
             for i in batch:
-                slots[i] = backend.alloc(i, prompts[i], params)
+                if i not in slots:
+                    slots[i] = backend.alloc(i, prompts[i], params)
             if params.n_predict == 0:
                 for i in batch:
                     results[i].finish_reason = "length"
                 continue
             length = {i: len(prompts[i]) for i in batch}
-            fed = {i: 0 for i in batch}            # prompt tokens given to the step function so far
             last = {}                              # request -> its newest token, to be fed next
             active = list(batch)
 

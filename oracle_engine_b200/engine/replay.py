@@ -91,6 +91,7 @@ def main(argv=None) -> int:
     ap.add_argument("--out", required=True, help="folder for <step>.f32 files")
     ap.add_argument("--max-tokens", type=int, required=True,
                     help="most tokens live requests hold at any time (each rounded up to 64); sizes the cache")
+    ap.add_argument("--cache-dtype", choices=["int8", "fp8"], default=None, help="keep keys and values in 8 bits")
     ap.add_argument("--no-graphs", action="store_true", help="do not capture CUDA graphs for one-token steps")
     args = ap.parse_args(argv)
 
@@ -102,7 +103,7 @@ def main(argv=None) -> int:
     tokens = int(args.max_tokens) + SLACK_REQUESTS * PAGE
     slots = min(MAX_SLOTS, max(1, tokens // PAGE), max(8, STATE_BUDGET_BYTES // max(1, state_bytes_per_slot(args.model))))
     engine = Engine.from_pretrained(args.model, dtype=args.dtype, max_tokens=tokens, max_seq_len=tokens,
-                                    n_slots=slots, use_graphs=not args.no_graphs)
+                                    n_slots=slots, use_graphs=not args.no_graphs, cache_dtype=args.cache_dtype)
     replay(engine, sys.stdin, Path(args.out))
     return 0
 

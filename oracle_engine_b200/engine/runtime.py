@@ -26,11 +26,25 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"dtype must be bfloat16 or float32, got {name!r}") from None
 
 
+def parse_cache_dtype(name) -> torch.dtype | None:
+    """The type of the cache's codes: None for a cache of the compute type, else "int8" or "fp8" (e4m3)."""
+    if name is None or str(name) in ("", "same"):
+        return None
+    from ..csrc.ops_kv8 import CODE_TYPES
+    if isinstance(name, torch.dtype) and name in CODE_TYPES.values():
+        return name
+    try:
+        return CODE_TYPES[str(name).lower()]
+    except KeyError:
+        raise ValueError(f"cache_dtype must be int8 or fp8 (or None: the compute type), got {name!r}") from None
+
+
 @dataclass
 class Runtime:
     dtype: torch.dtype
     device: torch.device
     tensor_cores: bool = True          # bf16 only: use the tcgen05 / mma kernels where they take the shape
+    cache_codes: torch.dtype | None = None     # the type of an 8-bit cache's codes (csrc/ops_kv8.py); None: a cache of the compute type
     # A hint for the part that runs now: the weight matrix that the part after it streams first (or
     # None).  The model and the block set it before they call a part; a part's last product may ask
     # the first megabytes of it into the L2 while its own epilogue runs (csrc/ops_tc.py: gemm(then=)).

@@ -24,7 +24,7 @@ import torch
 from ..cache.kv_cache import CacheView
 from ..csrc import build as _build
 from ..csrc import ops
-from .batch import SequenceStep, StepBuffers, build_plan, context_class
+from .batch import SequenceStep, StepBuffers, build_plan, context_class, shared_prefixes
 
 _BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
 # A step of up to this many tokens that is no decode step (a short prompt, a piece of one, prompts and single
@@ -172,18 +172,24 @@ class Stepper:
             self.cache.commit(s.slot, st + len(s.tokens))
         return logits
 
+    def _prefixes(self, seqs, pad_seqs: int):
+        """Which sequences of a step of single tokens begin with the same pages, or None."""
+        marks = [self.cache.prefix[s.slot] for s in seqs]
+        return shared_prefixes(marks, pad_seqs) if any(m is not None for m in marks) else None
+
     def _step_eager(self, seqs, starts, device_tokens=None, token_arrays=None):
         plan = build_plan(seqs, starts, token_arrays=token_arrays)
-        key = (plan.n_tokens, plan.n_seqs, plan.want_rows.size)
+        prefix = self._prefixes(seqs, len(seqs)) if plan.all_decode else None
+        key = (plan.n_tokens, plan.n_seqs, plan.want_rows.size, None if prefix is None else prefix.n_groups)
         buf = self._eager_buffers.get(key)
         if buf is None:
             if len(self._eager_buffers) > 64:
                 self._eager_buffers.clear()
             buf = StepBuffers(plan.n_tokens, plan.n_seqs, plan.want_rows.size, self._table_shapes(plan.n_seqs),
-                              self.rt.device)
+                              self.rt.device, prefix)
             self._eager_buffers[key] = buf
         tables = [self.cache.tables_for(g.index, plan.seq_slot) for g in self.cache.groups]
-        ctx = buf.upload(plan, tables)
+        ctx = buf.upload(plan, tables, prefix)
         if device_tokens is not None:
             ctx.token_ids[:len(seqs)].copy_(device_tokens[:len(seqs)])
         self.last_h2d_bytes = buf.bytes()
@@ -280,11 +286,13 @@ class Stepper:
     def _step_graph(self, seqs, starts, tables_changed=True, device_tokens=None):
         B = len(seqs)
         bucket = _bucket(B)
-        # one graph per padded batch size and context class: kernels chosen by the class stay right
-        gkey = (bucket, context_class(max(starts) + 1))
+        # one graph per padded batch size and context class: kernels chosen by the class stay right; and per shape of the
+        # sequences' common pages, where there are any
+        prefix = self._prefixes(seqs, bucket)
+        gkey = (bucket, context_class(max(starts) + 1)) + (() if prefix is None else prefix.shape)
         g = self._graphs.get(gkey)
         if g is None:
-            g = _DecodeGraph(bucket, StepBuffers(bucket, bucket, bucket, self._table_shapes(bucket), self.rt.device))
+            g = _DecodeGraph(bucket, StepBuffers(bucket, bucket, bucket, self._table_shapes(bucket), self.rt.device, prefix))
             self._graphs[gkey] = g
         key = tuple(s.slot for s in seqs)
         if key == g.key and g.version == self.cache.version:
@@ -294,7 +302,7 @@ class Stepper:
         else:
             plan = build_plan(seqs, starts, pad_seqs=bucket, pad_tokens=bucket, want_all_rows=True)
             tables = [self.cache.tables_for(gr.index, plan.seq_slot) for gr in self.cache.groups]
-            ctx = g.buffers.upload(plan, tables)
+            ctx = g.buffers.upload(plan, tables, prefix)
             g.key, g.ctx, g.version = key, ctx, self.cache.version
         if device_tokens is not None:         # after the copy of the step's tables, before the kernels
             ctx.token_ids[:B].copy_(device_tokens[:B])

@@ -16,7 +16,7 @@ import math
 
 import torch
 
-from ..csrc import ops
+from ..csrc import ops, ops_kv8
 from .linear import chain_flags, matmul_nt
 from .registry import MIXERS, Part
 from .spec import TensorDecl, attention_cache_need, mask_span, visible_keys, visible_pairs
@@ -71,13 +71,16 @@ class GQAAttention(Part):
         self.w_o = to(get(self.names["o"]))
 
     def cache_need(self):
-        return attention_cache_need(self.KVH, self.hd, self.span)
+        codes = self.rt.cache_codes
+        if codes is not None and not ops_kv8.supported(self.hd, self.H, self.KVH):
+            raise ValueError(f"gqa_attention: an 8-bit cache takes heads of {ops_kv8.HEAD_DIMS}, not {self.hd}")
+        return attention_cache_need(self.KVH, self.hd, self.span, codes)
 
     def weight_bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.w_qkv, self.w_o) if t is not None)
 
     def cache_bytes_per_query(self, context):
-        return visible_keys(self.span, context) * 2 * self.KVH * self.hd * (2 if self.rt.dtype == torch.bfloat16 else 4)
+        return visible_keys(self.span, context) * self.cache_need().bytes_per_token(self.rt.dtype.itemsize)
 
     def flops(self, start, count):
         rows = 2 * self.H + (0 if self.reads_cache else 2 * self.KVH)            # q, k, v and o projections
@@ -89,6 +92,7 @@ class GQAAttention(Part):
 
     joint_weight = "w_qkv"         # parts/block.py: JoinedInput
     takes_scaled = True            # its input goes to one product (Runtime.leave_normed)
+    quantised_cache = True
 
     def forward(self, h, residual, ctx, cache, state, owns_cache=True, projected=None):
         """projected: Wqkv h (Wq h first), computed by the caller; the rotation works in it."""

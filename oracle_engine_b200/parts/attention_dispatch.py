@@ -4,17 +4,27 @@ take it: 0 every key, n > 0 the last n, -n the query's own chunk of n (parts/spe
 
 float32, and head sizes the tensor-core kernels do not take, use the one-path kernel of
 csrc/attention.cu; bfloat16 uses the tensor-core prefill kernel and the split-KV decode
-kernel of csrc/attention_mma.cu.
+kernel of csrc/attention_mma.cu.  An 8-bit cache, and single tokens of sequences that begin with the same pages, go to the kernels
+of csrc/ops_kv8.py.
 """
 from __future__ import annotations
 
 import torch
 
-from ..csrc import ops
+from ..csrc import ops, ops_kv8
 
 
 def mixer_core(rt, out, qkv, cos, sin, cache, ctx, H, KVH, hd, window, scale, owns_cache) -> None:
-    """Rotation, cache write and attention of one attention mixer for the step's tokens."""
+    """Rotation, cache write and attention of one attention mixer for the step's tokens.  (`ahead`: in a model's step the
+    projections lie between whatever wrote the cache and its attention.)"""
+    if getattr(ctx, "prefix", None) is not None and not window and rt.dtype == torch.bfloat16 and rt.tensor_cores and \
+            ops_kv8.supported(hd, H, KVH):
+        # single tokens of sequences that begin with the same pages: those are read once for all of them
+        ops_kv8.attention_shared(out, qkv, cos, sin, cache.kv, cache.tables, ctx, ctx.prefix, H, KVH, hd, scale, owns_cache, ahead=True)
+        return
+    if rt.cache_codes is not None:
+        ops_kv8.attention_kv8(out, qkv, cos, sin, cache.kv, cache.tables, ctx, H, KVH, hd, window, scale, owns_cache, ahead=True)
+        return
     if rt.dtype == torch.bfloat16 and rt.tensor_cores and ctx.all_decode and ctx.n_tokens == ctx.n_seqs:
         from ..csrc import ops_tc
         # One CTA (or, for few long sequences, one cluster of CTAs) per (sequence, KV head) whose warps

@@ -98,6 +98,10 @@ class ParallelMixers(Part):
         matmul_nt(self.rt, y, h, self.w_joined, early=chain_flags("mixer_in", h.shape[0]))
         return [{"projected": y[:, lo:hi]} for lo, hi in self.columns]
 
+    @property
+    def quantised_cache(self):
+        return all(m.quantised_cache for _, m, _ in self.branches if m.cache_need() is not None)
+
     def cache_need(self):
         for _, m, _ in self.branches:
             if m.cache_need() is not None:

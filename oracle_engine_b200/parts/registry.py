@@ -37,6 +37,9 @@ Mixer  (MIXERS; e.g. attention)
     optional: a mixer or feed-forward whose forward chooses by the real lengths of a step's sequences says so in
     step_choice(step) (Part.step_choice); one that is a mixture of experts has `mixture = True`
 
+    optional: a mixer whose forward also takes an 8-bit cache (cache.kv is then a pair, CacheView.kv) has `quantised_cache = True`
+    and declares that form where runtime.cache_codes asks for it
+
     optional: a mixer made of mixers with output norms may hand those outputs over unnormed, with the norms' weights
     (`normed_outputs`, `eps`); an arrangement that norms the sum then does all of it in one kernel
 
@@ -119,6 +122,7 @@ class Part:
     runs_beside = False
 
     mixture = False                # a mixture of experts
+    quantised_cache = False        # a mixer that can keep its cache in 8 bits (Runtime.cache_codes)
 
     def __init__(self, params: dict, prefix: str, runtime):
         self.params = dict(params)

@@ -21,6 +21,8 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import Any, Optional
 
+import torch
+
 
 @dataclass(frozen=True)
 class TensorDecl:
@@ -71,11 +73,14 @@ class CacheNeed:
     given back) or "chunk" (those of the query's own chunk of `window` positions, counted from
     position 0; the pages of finished chunks are given back).  `also`: (kind, window) pairs of
     further readers of the same rows: what any of them still sees is kept.
-    Entries with equal needs share one group of storage and page tables."""
+    Entries with equal needs share one group of storage and page tables.
+    `dtypes`: ((name, torch dtype), ...) of tensors that are not of the compute type, e.g. the codes and scales of an 8-bit
+    cache."""
     kind: str
     tensors: tuple
     window: int = 0
     also: tuple = ()
+    dtypes: tuple = ()
 
     def first_position(self, pos: int) -> int:
         """The oldest position that a query at `pos`, or at any later one, still reads."""
@@ -92,29 +97,39 @@ class CacheNeed:
         if set(theirs) <= set(mine):
             return self
         if any(kind == "full" for kind, _ in mine + theirs):
-            return CacheNeed("full", self.tensors)
+            return CacheNeed("full", self.tensors, dtypes=self.dtypes)
         rest = sorted(set(mine + theirs) - {(self.kind, self.window)})
-        return CacheNeed(self.kind, self.tensors, self.window, tuple(rest))
+        return CacheNeed(self.kind, self.tensors, self.window, tuple(rest), self.dtypes)
 
     def elements_per_token(self) -> int:
+        return self.bytes_per_token(1, {})
+
+    def bytes_per_token(self, itemsize: int, sizes: dict | None = None) -> int:
+        """itemsize: a value's bytes in the tensors of the compute type (sizes: those of the others, by name)."""
+        if sizes is None:
+            sizes = {name: dtype.itemsize for name, dtype in self.dtypes}
         n = 0
-        for _, shape in self.tensors:
-            e = 1
+        for name, shape in self.tensors:
+            e = sizes.get(name, itemsize)
             for d in shape:
                 e *= int(d)
             n += e
         return n
 
 
-def span_need(tensors: tuple, span: int) -> CacheNeed:
+def span_need(tensors: tuple, span: int, dtypes: tuple = ()) -> CacheNeed:
     """The need of an attention whose mask is `span` as the kernels take it (csrc/common.cuh: oe_first_key): 0 every
     key, n > 0 the last n keys, -n the keys of the query's own chunk of n."""
-    return CacheNeed("window" if span > 0 else "chunk" if span < 0 else "full", tensors, abs(int(span)))
+    return CacheNeed("window" if span > 0 else "chunk" if span < 0 else "full", tensors, abs(int(span)), dtypes=dtypes)
 
 
-def attention_cache_need(kv_heads: int, head_dim: int, span: int = 0) -> CacheNeed:
-    """Keys and values of grouped-query attention: one tensor "kv", per page [2, kv_heads, PAGE, head_dim]."""
-    return span_need((("kv", (2, int(kv_heads), int(head_dim))),), span)
+def attention_cache_need(kv_heads: int, head_dim: int, span: int = 0, codes=None) -> CacheNeed:
+    """Keys and values of grouped-query attention: one tensor "kv", per page [2, kv_heads, PAGE, head_dim].  codes: the type of
+    an 8-bit cache's codes; then two tensors, "codes" of that shape and type and "scales", per page [2, kv_heads, PAGE, 1] float32."""
+    if codes is None:
+        return span_need((("kv", (2, int(kv_heads), int(head_dim))),), span)
+    return span_need((("codes", (2, int(kv_heads), int(head_dim))), ("scales", (2, int(kv_heads), 1))), span,
+                     (("codes", codes), ("scales", torch.float32)))
 
 
 def mask_span(window, chunk) -> int:

@@ -1,5 +1,5 @@
-// Attention of a few rows at a time over the paged cache in its 8-bit forms (kv8.cuh) or in bfloat16, the write of the
-// 8-bit forms, and the attention of shared prefixes; compiled for one head size: -DOE_HD=64 or 128.
+// Attention of a few rows at a time over the paged cache in its 8-bit forms (kv8.cuh) or in bfloat16, and the write of the
+// 8-bit forms; compiled for one head size: -DOE_HD=64 or 128.
 //
 // A row is a (token, query head of the group) pair.  A CTA (or a cluster of CTAs) has 16 rows of one KV head and a range of
 // keys; its warps split the keys in tiles of 32, each with a ring of tiles of its own that cp.async fills and a running
@@ -127,13 +127,11 @@ struct Args {
     float scale_log2;
     int cluster;               // CTAs that share a tile of rows
     int ahead;                 // rows of earlier tokens may be read before the wait
-    // sequences that begin with the same pages
-    const int* members;        // sequences in the order of their groups
-    const int* first;          // [n_groups + 1] where each group's members begin
-    const int* pages;          // [n_groups] pages of its prefix
+    // sequences that begin with the same pages: what attention_rows.cu has left of those pages
     const int* seq_pages;      // [B] pages of the sequence's prefix (0: none); null: no prefixes
-    int n_groups, splits;
-    float* partial;            // [B, H, splits, HD + 2]: o, m, l of the prefixes' parts
+    int splits;
+    const float* part_o;       // [B * H, splits, HD]
+    const float* part_ml;      // [B * H, splits, 2]
 };
 
 __device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
@@ -260,10 +258,9 @@ struct NewToken {
     }
 };
 
-// PREFIX false: the rows are those of one sequence's new tokens (blockIdx.z), the keys its own, from behind its prefix on; the
-// result is stored, joined with its prefix's parts if it has one.  PREFIX true: the rows are those of all members of a group
-// (blockIdx.z), the keys a split of the group's prefix; the result is a part.
-template <int KIND, bool PREFIX, int NW, int ST>
+// The rows are those of one sequence's new tokens (blockIdx.z), the keys its own, from behind its prefix on if it has one, whose
+// parts are joined with the result.
+template <int KIND, int NW, int ST>
 __global__ void __launch_bounds__(NW * 32)
 attn_kv8_kernel(const Args a) {
     using L = Tile<KIND>;
@@ -275,41 +272,26 @@ attn_kv8_kernel(const Args a) {
     const int G = a.H / a.KVH, kvh = blockIdx.y;
     const int CR = a.cluster, rank = CR > 1 ? (int)cluster_ctarank() : 0;
     const int bx = blockIdx.x / CR;
-    int n_rows, row0, split = 0, b = 0, start = 0, key_lo, key_hi;
-    long long packed0 = 0;
-    if (PREFIX) {
-        split = bx % a.splits;
-        row0 = bx / a.splits * 16;
-        const int g = blockIdx.z;
-        n_rows = (a.first[g + 1] - a.first[g]) * G;
-        b = n_rows > 0 ? a.members[a.first[g]] : 0;                  // the prefix's pages are every member's first ones
-        const int n = a.pages[g] * PARTS;                             // in tiles
-        key_lo = (int)((long long)n * split / a.splits) * TB;
-        key_hi = (int)((long long)n * (split + 1) / a.splits) * TB - 1;
-    } else {
-        b = blockIdx.z;
-        row0 = bx * 16;
-        const int qlen = a.seq_qlen[b];
-        n_rows = qlen > 0 ? qlen * G : 0;
-        start = a.seq_start[b];
-        packed0 = a.cu_q[b];
-        key_lo = oe_first_key(start + row0 / G, a.window);
-        key_hi = start + min(row0 + 15, n_rows - 1) / G;
-        if (a.seq_pages != nullptr) key_lo = max(key_lo, a.seq_pages[b] * OE_PAGE);
-    }
+    const int b = blockIdx.z, row0 = bx * 16, qlen = a.seq_qlen[b], n_rows = qlen > 0 ? qlen * G : 0;
     if (row0 >= n_rows) {                                            // the whole cluster
         pdl_wait();
         return;
     }
+    const int start = a.seq_start[b];
+    const long long packed0 = a.cu_q[b];
+    int key_lo = oe_first_key(start + row0 / G, a.window);
+    const int key_hi = start + min(row0 + 15, n_rows - 1) / G;
+    const int common = a.seq_pages != nullptr ? a.seq_pages[b] : 0;
+    key_lo = max(key_lo, common * OE_PAGE);
     const int* trow = a.tables + (size_t)b * a.max_pages;
     uint8_t* mine = smem + (size_t)warp * WARP_BYTES;
     const int gw = rank * NW + warp, stride = NW * CR;
     const int t_lo = key_lo / TB, t_hi = key_hi >= key_lo ? key_hi / TB : t_lo - 1;
     const int n_my = t_lo + gw <= t_hi ? (t_hi - t_lo - gw) / stride + 1 : 0;
-    const bool own_kv = !PREFIX && a.cache_w != nullptr;
+    const bool own_kv = a.cache_w != nullptr;
     // where the caller says so, keys and values of earlier steps are asked for before the wait: only the new token's q, k and v
     // come from the kernel before this one
-    const bool ahead = a.ahead && (own_kv || PREFIX);
+    const bool ahead = a.ahead && own_kv;
     if (!ahead) pdl_wait();
 #pragma unroll
     for (int pre = 0; pre < ST; pre++) {
@@ -324,25 +306,16 @@ attn_kv8_kernel(const Args a) {
     // this thread's two rows
     bool valid[2];
     int head[2], pos[2], low[2];
-    long long tok[2], part_row[2];
+    long long tok[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const int r = row0 + gid + i * 8;
         valid[i] = r < n_rows;
         const int rr = valid[i] ? r : row0;
         head[i] = kvh * G + rr % G;
-        if (PREFIX) {
-            const int sq = a.members[a.first[blockIdx.z] + rr / G];
-            tok[i] = a.cu_q[sq];
-            pos[i] = a.seq_start[sq];
-            low[i] = 0;
-            part_row[i] = (long long)sq * a.H + head[i];
-        } else {
-            tok[i] = packed0 + rr / G;
-            pos[i] = start + rr / G;
-            low[i] = oe_first_key(pos[i], a.window);
-            part_row[i] = (long long)b * a.H + head[i];
-        }
+        tok[i] = packed0 + rr / G;
+        pos[i] = start + rr / G;
+        low[i] = oe_first_key(pos[i], a.window);
     }
     // Q fragments, turned: qf, and for a 16-bit cache what its rounding leaves
     constexpr int KL = KIND == OE_KV_BF16 ? KS : 1;
@@ -462,7 +435,7 @@ attn_kv8_kernel(const Args a) {
             const int k0 = tile * TB;
             // (key_lo: the first key of this CTA's range, beside each row's own)
             const bool whole = k0 >= key_lo && k0 + TB - 1 <= key_hi &&
-                               (PREFIX || (k0 + TB - 1 <= min(pos[0], pos[1]) && k0 >= max(low[0], low[1])));
+                               k0 + TB - 1 <= min(pos[0], pos[1]) && k0 >= max(low[0], low[1]);
             const bool mask = !__all_sync(0xffffffffu, whole);
             float rmax[2] = {-INFINITY, -INFINITY}, sv_most = 0.f;
 #pragma unroll
@@ -482,7 +455,7 @@ attn_kv8_kernel(const Args a) {
                     const int i = e >> 1, ke = key + (e & 1);
                     float v = s[n][e] * (KIND == OE_KV_BF16 ? row_scale[i] : (e & 1 ? ksc.y : ksc.x) * row_scale[i]);
                     if (mask) {
-                        const bool seen = ke >= key_lo && ke <= key_hi && (PREFIX || (ke <= pos[i] && ke >= low[i]));
+                        const bool seen = ke >= key_lo && ke <= pos[i] && ke >= low[i];
                         v = seen ? v : -INFINITY;
                     }
                     s[n][e] = v;
@@ -628,14 +601,15 @@ attn_kv8_kernel(const Args a) {
     }
     if (CR > 1) cluster_sync_all();
     else __syncthreads();
-    const int n_pre = !PREFIX && a.seq_pages != nullptr && a.seq_pages[b] > 0 ? a.splits : 0;
+    const int n_pre = common > 0 ? a.splits : 0;
     for (int idx = threadIdx.x + rank * NW * 32; idx < rows * HD; idx += NW * 32 * CR) {
         const int r = idx / HD, d = idx % HD;
         float m = -INFINITY, l = 0.f, o = 0.f;
         for (int q = 0; q < CR; q++) m = fmaxf(m, CR > 1 ? ld_peer_f32(cpart + r * (HD + 2) + HD, q) : cpart[r * (HD + 2) + HD]);
         const int h = kvh * G + (row0 + r) % G;
-        const float* pre = a.partial + ((long long)b * a.H + h) * a.splits * (HD + 2);
-        for (int q = 0; q < n_pre; q++) m = fmaxf(m, pre[q * (HD + 2) + HD]);
+        const float* pre_o = a.part_o + ((long long)b * a.H + h) * a.splits * HD;
+        const float2* pre_ml = (const float2*)a.part_ml + ((long long)b * a.H + h) * a.splits;
+        for (int q = 0; q < n_pre; q++) m = fmaxf(m, pre_ml[q].x);
         const float mu = m == -INFINITY ? 0.f : m;
         for (int q = 0; q < CR; q++) {
             const float pm = CR > 1 ? ld_peer_f32(cpart + r * (HD + 2) + HD, q) : cpart[r * (HD + 2) + HD];
@@ -646,44 +620,28 @@ attn_kv8_kernel(const Args a) {
             o += (CR > 1 ? ld_peer_f32(cpart + r * (HD + 2) + d, q) : cpart[r * (HD + 2) + d]) * e;
         }
         for (int q = 0; q < n_pre; q++) {
-            const float pm = pre[q * (HD + 2) + HD], pl = pre[q * (HD + 2) + HD + 1];
-            if (pm == -INFINITY && pl == 0.f) continue;
-            const float e = exp2f(pm - mu);
-            l += pl * e;
-            o += pre[q * (HD + 2) + d] * e;
+            const float2 ml = pre_ml[q];
+            if (ml.x == -INFINITY && ml.y == 0.f) continue;
+            const float e = exp2f(ml.x - mu);
+            l += ml.y * e;
+            o += pre_o[q * HD + d] * e;
         }
-        if (PREFIX) {
-            const int sq = a.members[a.first[blockIdx.z] + (row0 + r) / G];
-            float* p = a.partial + (((long long)sq * a.H + h) * a.splits + split) * (HD + 2);
-            p[d] = o;
-            if (d == 0) { p[HD] = m; p[HD + 1] = l; }
-        } else {
-            a.out[(packed0 + (row0 + r) / G) * (long long)(a.H * HD) + (long long)h * HD + d] =
-                __float2bfloat16_rn(l > 0.f ? o / l : l == 0.f ? 0.f : l);
-        }
+        a.out[(packed0 + (row0 + r) / G) * (long long)(a.H * HD) + (long long)h * HD + d] = __float2bfloat16_rn(l > 0.f ? o / l : l == 0.f ? 0.f : l);
     }
     if (CR > 1) cluster_sync_all();                         // nobody leaves while its shared memory is read
 }
 
-template <int KIND, bool PREFIX>
-int launch(const Args& a, int row_tiles, int groups, cudaStream_t st) {
+template <int KIND>
+int launch(const Args& a, int row_tiles, int n_seqs, cudaStream_t st) {
     constexpr int NW = KIND == OE_KV_BF16 ? 3 : 4, ST = KIND == OE_KV_BF16 ? 2 : 3;
     constexpr size_t smem = (size_t)NW * ST * Tile<KIND>::BYTES;
     const long long x = (long long)row_tiles * a.cluster;
-    if (x > 0x7fffffffLL || a.KVH > 65535 || groups > 65535) return OE_ERR_UNSUPPORTED;
-    cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<KIND, PREFIX, NW, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (x > 0x7fffffffLL || a.KVH > 65535 || n_seqs > 65535) return OE_ERR_UNSUPPORTED;
+    cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<KIND, NW, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    const dim3 grid((unsigned)x, a.KVH, groups);
-    if (a.cluster > 1)
-        return oe_launch_cluster(attn_kv8_kernel<KIND, PREFIX, NW, ST>, (unsigned)a.cluster, grid, dim3(NW * 32), smem, st, a);
-    return oe_launch(attn_kv8_kernel<KIND, PREFIX, NW, ST>, grid, dim3(NW * 32), smem, st, a);
-}
-template <bool PREFIX>
-int launch_kind(int kind, const Args& a, int row_tiles, int groups, cudaStream_t st) {
-    if (kind == OE_KV_BF16) return launch<OE_KV_BF16, PREFIX>(a, row_tiles, groups, st);
-    if (kind == OE_KV_INT8) return launch<OE_KV_INT8, PREFIX>(a, row_tiles, groups, st);
-    if (kind == OE_KV_E4M3) return launch<OE_KV_E4M3, PREFIX>(a, row_tiles, groups, st);
-    return OE_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)x, a.KVH, n_seqs);
+    if (a.cluster > 1) return oe_launch_cluster(attn_kv8_kernel<KIND, NW, ST>, (unsigned)a.cluster, grid, dim3(NW * 32), smem, st, a);
+    return oe_launch(attn_kv8_kernel<KIND, NW, ST>, grid, dim3(NW * 32), smem, st, a);
 }
 
 }  // namespace
@@ -709,42 +667,28 @@ int oe_kv8_write(int kind, const bf16* qkv, long long stride, const float* cos_t
 
 // Attention of the step's tokens over their sequences' caches (kind: OE_KV_*).  write != 0: every sequence brings one token, whose
 // key and value this kernel writes.  With seq_pages the pages before a sequence's own are left out and the parts that
-// oe_attn_kv8_prefix left in `partial` are added.
+// oe_attn_rows_prefix left are added.
 int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, void* cache,
                 float* scales, int write, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
                 const int* seq_qlen, int n_seqs, int max_qlen, int H, int KVH, int window, float scale, int cluster,
-                const int* seq_pages, int splits, float* partial, int ahead, cudaStream_t st) {
+                const int* seq_pages, int splits, const float* part_o, const float* part_ml, int ahead, cudaStream_t st) {
     if (n_seqs <= 0 || max_qlen <= 0) return 0;
     if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15)) return OE_ERR_UNSUPPORTED;
     if (cluster < 1 || cluster > 8 || (write && max_qlen != 1)) return OE_ERR_UNSUPPORTED;
-    if (seq_pages != nullptr && (window != 0 || max_qlen != 1 || splits < 1 || partial == nullptr)) return OE_ERR_UNSUPPORTED;
+    if (seq_pages != nullptr && (window != 0 || max_qlen != 1 || splits < 1 || part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
     Args a = {};
     a.out = out; a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab;
     a.cache = cache; a.scales = scales;
     if (write) { a.cache_w = cache; a.scales_w = scales; }
     a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start; a.seq_qlen = seq_qlen;
     a.H = H; a.KVH = KVH; a.window = window; a.scale_log2 = scale * LOG2E; a.cluster = cluster;
-    a.seq_pages = seq_pages; a.splits = splits; a.partial = partial; a.ahead = ahead;
-    const long long rows = (long long)max_qlen * (H / KVH);
-    return launch_kind<false>(kind, a, (int)((rows + 15) / 16), n_seqs, st);
-}
-
-// The parts of the groups' prefixes: every member's queries against the pages that its group has in common, in `splits` parts.
-int oe_attn_kv8_prefix(int kind, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, const void* cache,
-                       const float* scales, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
-                       int H, int KVH, float scale, const int* members, const int* first, const int* pages, int n_groups, int n_members,
-                       int splits, float* partial, int ahead, cudaStream_t st) {
-    if (n_groups <= 0 || n_members <= 0) return 0;
-    if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15)) return OE_ERR_UNSUPPORTED;
-    if (splits < 1) return OE_ERR_UNSUPPORTED;
-    Args a = {};
-    a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.cache = cache; a.scales = scales;
-    a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start;
-    a.H = H; a.KVH = KVH; a.scale_log2 = scale * LOG2E; a.cluster = 1;
-    a.members = members; a.first = first; a.pages = pages; a.n_groups = n_groups; a.splits = splits; a.partial = partial; a.ahead = ahead;
-    const long long tiles = ((long long)n_members * (H / KVH) + 15) / 16 * splits;
+    a.seq_pages = seq_pages; a.splits = splits; a.part_o = part_o; a.part_ml = part_ml; a.ahead = ahead;
+    const long long rows = (long long)max_qlen * (H / KVH), tiles = (rows + 15) / 16;
     if (tiles > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
-    return launch_kind<true>(kind, a, (int)tiles, n_groups, st);
+    if (kind == OE_KV_BF16) return launch<OE_KV_BF16>(a, (int)tiles, n_seqs, st);
+    if (kind == OE_KV_INT8) return launch<OE_KV_INT8>(a, (int)tiles, n_seqs, st);
+    if (kind == OE_KV_E4M3) return launch<OE_KV_E4M3>(a, (int)tiles, n_seqs, st);
+    return OE_ERR_UNSUPPORTED;
 }
 
 }  // extern "C"

@@ -1,0 +1,910 @@
+// Attention of many rows at a time over the paged cache in its 8-bit forms (kv8.cuh), and of the rows of all sequences that begin
+// with the same pages over those pages (8-bit or bfloat16), on the 5th-generation tensor cores; compiled for one head size: -DOE_HD=64
+// or 128.
+//
+// A row is a (token, query head of the group) pair.  A CTA has MT tiles of 128 rows of one KV head and a run of cache pages (64 keys
+// each); the tiles share every page's K and V.  Per page and tile:
+//   S = Q K^T      tcgen05.mma M=128 N=64 K=HD, float32 in tensor memory (two buffers);
+//   softmax        128 threads, one row each: the row's 64 scores from tensor memory, times the keys' scales, mask, maximum and sum in
+//                  float32, P back into the buffer's columns;
+//   O += P V       tcgen05.mma M=128 N=HD K=64, P from tensor memory, O float32 in tensor memory for the whole run.
+// A row's reference maximum moves only when its maximum has grown by more than 2^7 since it was set; O and the sum are rescaled
+// then, before the page's P V is issued, and the factor cancels in O / l.
+// 8-bit forms: a code is a float16 exactly.  The pages' codes come by bulk copies; a warpgroup turns them into the swizzled float16 tiles
+// that the products read, once for all MT tiles.  The keys' scales multiply the float32 scores, the values' scales the weights.
+// Queries and weights are rounded to float16 (2^-12 of themselves): a query row is scaled by a power of two into [1, 2) first,
+// weights are relative to R, the power of two above the largest value scale so far, and times 2^8 (what float16 cannot hold is
+// then below 2^-33 of a row's largest weight).  R grows for the whole CTA at once, with the rescaling of O.
+// bfloat16: K and V as they are (TMA); queries and weights are sums of two bfloat16, a second product each.
+// Roles (warps): 0 asks for the pages, 1 issues the products, 2 prepares the scales, 4-7 turn codes into float16 (8-bit forms),
+// the last 4 MT load and turn the queries, then do the softmax and store.
+// Few tiles: the pages are cut into `splits` runs, whose parts (O, m, l) are joined by the kernel that runs next.
+// Every wait on an mbarrier is bounded in time; one that runs out raises an error flag, every role leaves its loop, copies in
+// flight get a fixed time, and tensor memory is freed.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include "kv8.cuh"
+#include <mutex>
+
+#ifndef OE_HD
+#define OE_HD 128
+#endif
+
+namespace {
+
+constexpr int HD = OE_HD;
+static_assert(HD == 64 || HD == 128, "built for head_dim 64 or 128");
+constexpr int BM = 128, BN = OE_PAGE, SUB = HD / 64;
+constexpr int Q_BYTES = BM * HD * 2;             // SUB sub-tiles of [128][64] 16-bit values
+constexpr int T_BYTES = BN * HD * 2;             // K or V of a page, SUB sub-tiles of [64][64] 16-bit values
+constexpr int RAW = BN * HD;                     // codes of a page's K or V
+constexpr int STAGES = 2, SC_SLOTS = 4;
+constexpr float RESCALE_STEP = 7.f, LOG2E = 1.4426950408889634f;
+constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
+
+__device__ int g_error = 0;
+
+struct Scales {
+    float k[BN], v[BN];                          // as copied; v then relative to R (0 where no key is)
+    float grown, ref;                            // R before / R, and R
+    int mapped, pad;
+};
+struct Ctl {
+    Scales sc[SC_SLOTS];
+    uint64_t q_full, raw_full[STAGES], raw_empty[STAGES], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
+    uint64_t sc_full[SC_SLOTS], sc_ready[SC_SLOTS], sc_empty[SC_SLOTS];
+    uint64_t s_full[2][2], p_ready[2][2], pv_done[2], o_done[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <int KIND, int MT>
+struct Shape {
+    static constexpr bool EIGHT = KIND != OE_KV_BF16;
+    static constexpr int Q_ALL = MT * Q_BYTES * (EIGHT ? 1 : 2);
+    static constexpr int K_AT = Q_ALL, V_AT = K_AT + STAGES * T_BYTES, RAW_AT = V_AT + STAGES * T_BYTES;
+    static constexpr int CTL_AT = RAW_AT + (EIGHT ? STAGES * 2 * RAW : 0);
+    static constexpr int BYTES = CTL_AT + (int)sizeof(Ctl);
+    static constexpr int CONVERT = EIGHT ? 4 : 0;                      // warps
+    static constexpr int FIRST = 4 + CONVERT;                          // the first softmax warp
+    static constexpr int THREADS = (FIRST + 4 * MT) * 32;
+    static constexpr uint32_t S_COLS = MT * 2 * BN, O_COLS = MT * HD;
+    static constexpr uint32_t COLS = S_COLS + O_COLS <= 128 ? 128 : S_COLS + O_COLS <= 256 ? 256 : 512;
+    static constexpr float HEADROOM = EIGHT ? 8.f : 0.f;
+};
+
+struct Args {
+    bf16* out;                 // [T, H*HD]
+    const bf16* q;             // rows of q_stride elements: the projections, queries first, not yet turned
+    long long q_stride;
+    const float* cos_tab;      // [max_pos, HD/2] or null
+    const float* sin_tab;
+    const uint8_t* codes;      // 8-bit forms
+    const float* scales;
+    long long n_pages;
+    const int* tables;
+    int max_pages;
+    const int* cu_q;
+    const int* seq_start;
+    const int* seq_qlen;
+    int H, KVH, window;
+    float scale_log2;
+    int ahead;
+    const int* members;        // prefixes, as in attention_kv8.cu
+    const int* first;
+    const int* pages;
+    int splits;
+    float* part_o;             // [rows, splits, HD]: row = (sequence or packed token) * H + head
+    float* part_ml;            // [rows, splits, 2]
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ unsigned long long global_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, Ctl* ctl, int code) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    for (uint32_t spin = 0;; spin++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((spin & 255u) == 255u) {
+            if (*(volatile int*)&ctl->abort_flag) return false;
+            if (global_ns() - t0 > WAIT_LIMIT_NS) {
+                atomicExch(&ctl->abort_flag, 1);
+                atomicCAS(&g_error, 0, code);
+                return false;
+            }
+        }
+    }
+}
+// All lanes of the warp wait and take the same decision.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Ctl* ctl, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctl, code));
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(c0), "r"(c1) : "memory");
+}
+// Shared-memory operand descriptor, 128-byte swizzle, version 1 (sm_100).  K-major: rows of 128 bytes along K, stride 1024 between
+// groups of 8 rows.  MN-major: rows of 128 bytes along N, one row per k, stride 1024 between groups of 8 k, leading offset between
+// column groups of 64.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lead_bytes, uint32_t stride_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)((lead_bytes >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)((stride_bytes >> 4) & 0x3FFFu) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// kind::f16 instruction descriptor: D float32, A and B both float16 or both bfloat16, A K-major, B K-major or MN-major.
+__device__ __forceinline__ uint32_t umma_idesc(int m, int n, bool b_mn_major, bool bf) {
+    return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, float* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool EIGHT>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    if (EIGHT) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *(const uint32_t*)&h;
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *(const uint32_t*)&h;
+}
+__device__ __forceinline__ uint32_t rest_bf16(float lo, float hi, uint32_t h) {
+    return pack16<false>(lo - __uint_as_float(h << 16), hi - __uint_as_float(h & 0xffff0000u));
+}
+
+// Eight consecutive dimensions d..d+7 of a row of queries and the eight they are turned with, d + HD/2 ..., as float32.
+__device__ __forceinline__ void turned8(const bf16* row, const float* cs, const float* sn, int d, float (&lo)[8], float (&hi)[8]) {
+    const uint4 a = *(const uint4*)(row + d), b = *(const uint4*)(row + d + HD / 2);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        lo[2 * j] = kv8_from_bits(aw[j] & 0xffffu); lo[2 * j + 1] = kv8_from_bits(aw[j] >> 16);
+        hi[2 * j] = kv8_from_bits(bw[j] & 0xffffu); hi[2 * j + 1] = kv8_from_bits(bw[j] >> 16);
+    }
+    if (cs != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            const float4 c = *(const float4*)(cs + d + j), s = *(const float4*)(sn + d + j);
+            const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float x = lo[j + e], y = hi[j + e];
+                lo[j + e] = x * cc[e] - y * ss[e];
+                hi[j + e] = x * ss[e] + y * cc[e];
+            }
+        }
+    }
+}
+
+// Warps 4-7: a page's codes to the swizzled 16-bit tile.  A lane takes 16 codes at a time; the lanes of the second sub-tile store their
+// two pieces in the other order, so that 8 lanes fill 8 different bank groups.
+template <int KIND>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* tile, int t) {
+    constexpr int PER_ROW = HD / 16;
+#pragma unroll
+    for (int u = t; u < BN * PER_ROW; u += 128) {
+        const int key = u / PER_ROW, g = u % PER_ROW;
+        const uint4 w = *(const uint4*)(raw + u * 16);
+        const uint32_t in[4] = {kv8_word<KIND>(w.x), kv8_word<KIND>(w.y), kv8_word<KIND>(w.z), kv8_word<KIND>(w.w)};
+        uint4 o[2];
+        o[0] = make_uint4(kv8_pair<KIND>(in[0], 0), kv8_pair<KIND>(in[0], 2), kv8_pair<KIND>(in[1], 0), kv8_pair<KIND>(in[1], 2));
+        o[1] = make_uint4(kv8_pair<KIND>(in[2], 0), kv8_pair<KIND>(in[2], 2), kv8_pair<KIND>(in[3], 0), kv8_pair<KIND>(in[3], 2));
+        uint8_t* row = tile + (g / 4) * (BN * 128) + key * 128;
+        const int c = (g % 4) * 2, x = key & 7, odd = g / 4;
+        *(uint4*)(row + (((c + odd) ^ x) << 4)) = odd ? o[1] : o[0];
+        *(uint4*)(row + (((c + 1 - odd) ^ x) << 4)) = odd ? o[0] : o[1];
+    }
+}
+
+// PREFIX false: the tiles are those of one sequence's tokens, keys up to each row's position.  PREFIX true: the rows are those of all
+// members of a group, the keys the group's common pages.
+template <int KIND, bool PREFIX, int MT>
+__global__ void __launch_bounds__(Shape<KIND, MT>::THREADS, 1)
+attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
+    using Z = Shape<KIND, MT>;
+    constexpr bool EIGHT = Z::EIGHT;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    {   // the swizzled tiles need a 1024-byte boundary; the launch leaves less than 1024 bytes of slack
+        uint32_t dyn;
+        asm volatile("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn));
+        if ((uint32_t)(smem - smem_raw) + (uint32_t)Z::BYTES > dyn) {
+            if (threadIdx.x == 0) atomicCAS(&g_error, 0, 9);
+            return;
+        }
+    }
+    uint8_t* q_s = smem;
+    uint8_t* k_s = smem + Z::K_AT;
+    uint8_t* v_s = smem + Z::V_AT;
+    uint8_t* raw_s = smem + Z::RAW_AT;
+    Ctl* ctl = (Ctl*)(smem + Z::CTL_AT);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = a.H / a.KVH, tpt = BM / G;               // tokens, or members, of a tile
+    const int kvh = blockIdx.x % a.KVH, split = blockIdx.x / a.KVH;
+    // the tiles' rows and the CTA's pages (the step's integers were written before its first kernel)
+    int b, count, t0, start = 0, key_lo = 0, j_lo, n_blocks[MT];
+    if (PREFIX) {
+        const int g = blockIdx.y;
+        count = a.first[g + 1] - a.first[g];
+        t0 = blockIdx.z * MT * tpt;
+        b = t0 < count ? a.members[a.first[g]] : 0;
+    } else {
+        b = blockIdx.y;
+        count = a.seq_qlen[b];
+        t0 = ((int)gridDim.z - 1 - (int)blockIdx.z) * MT * tpt;     // the heaviest tiles first
+    }
+    if (t0 >= count) {
+        pdl_launch_dependents();
+        pdl_wait();
+        return;
+    }
+    int any = 0;                                           // the most pages a tile has
+    {
+        int hi = 0;
+        if (PREFIX) {
+            const int n = a.pages[blockIdx.y];
+            j_lo = (int)((long long)n * split / a.splits);
+            hi = (int)((long long)n * (split + 1) / a.splits);
+        } else {
+            start = a.seq_start[b];
+            key_lo = oe_first_key(start + t0, a.window);
+            j_lo = key_lo / BN;
+            const int n = (start + min(t0 + MT * tpt, count) - 1) / BN - j_lo + 1;
+            hi = j_lo + (int)((long long)n * (split + 1) / a.splits);
+            j_lo += (int)((long long)n * split / a.splits);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            int last = hi;
+            if (!PREFIX) last = min(hi, (start + min(t0 + (t + 1) * tpt, count) - 1) / BN + 1);
+            n_blocks[t] = t0 + t * tpt < count ? max(0, last - j_lo) : 0;
+            any = max(any, n_blocks[t]);
+        }
+    }
+    const int* trow = a.tables + (size_t)b * a.max_pages;
+    if (threadIdx.x == 0) {
+        mbar_init(&ctl->q_full, MT * 4);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&ctl->raw_full[s], 1); mbar_init(&ctl->raw_empty[s], 4);
+            mbar_init(&ctl->k_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->k_empty[s], 1);
+            mbar_init(&ctl->v_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->v_empty[s], 1);
+        }
+        for (int s = 0; s < SC_SLOTS; s++) {
+            mbar_init(&ctl->sc_full[s], 1); mbar_init(&ctl->sc_ready[s], 1); mbar_init(&ctl->sc_empty[s], MT * 4);
+        }
+        for (int t = 0; t < MT; t++) {
+            mbar_init(&ctl->s_full[t][0], 1); mbar_init(&ctl->s_full[t][1], 1);
+            mbar_init(&ctl->p_ready[t][0], 4); mbar_init(&ctl->p_ready[t][1], 4);
+            mbar_init(&ctl->pv_done[t], 1); mbar_init(&ctl->o_done[t], 1);
+        }
+        ctl->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(Z::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem_base = *(volatile uint32_t*)&ctl->tmem_base;
+    pdl_launch_dependents();
+    // prefixes: where the caller says so, the pages are asked for before the wait; the queries come from the kernel before
+    const bool ahead = PREFIX && a.ahead;
+    if (!ahead || warp >= Z::FIRST) pdl_wait();
+
+    if (warp == 0) {
+        // ---------------- the pages ----------------
+        if (lane == 0) {
+            bool ok = true;
+            auto row_of = [&](int i, int which) -> long long {      // the first row of page i's K or V, -1: not mapped
+                const int j = j_lo + i, page = j < a.max_pages ? trow[j] : -1;
+                return (unsigned)page < (unsigned long long)a.n_pages ? (((long long)page * 2 + which) * a.KVH + kvh) * BN : -1;
+            };
+            if (EIGHT) {
+                for (int i = 0; i < any && ok; i++) {
+                    const int s = i % STAGES, c = i % SC_SLOTS;
+                    ok = mbar_wait(&ctl->raw_empty[s], ((uint32_t)(i / STAGES) & 1u) ^ 1u, ctl, 1);
+                    if (ok) ok = mbar_wait(&ctl->sc_empty[c], ((uint32_t)(i / SC_SLOTS) & 1u) ^ 1u, ctl, 2);
+                    if (!ok) break;
+                    fence_async();                         // the slot's scales were written by threads before
+                    long long kr = row_of(i, 0), vr = row_of(i, 1);
+                    ctl->sc[c].mapped = kr >= 0;
+                    if (kr < 0) { kr = (long long)kvh * BN; vr = kr + (long long)a.KVH * BN; }      // any codes are numbers
+                    mbar_expect_tx(&ctl->raw_full[s], 2 * RAW);
+                    bulk_load(raw_s + s * 2 * RAW, a.codes + kr * HD, RAW, &ctl->raw_full[s]);
+                    bulk_load(raw_s + s * 2 * RAW + RAW, a.codes + vr * HD, RAW, &ctl->raw_full[s]);
+                    mbar_expect_tx(&ctl->sc_full[c], 2 * BN * 4);
+                    bulk_load(ctl->sc[c].k, a.scales + kr, BN * 4, &ctl->sc_full[c]);
+                    bulk_load(ctl->sc[c].v, a.scales + vr, BN * 4, &ctl->sc_full[c]);
+                }
+            } else {
+                auto load = [&](int i, int which, uint64_t* full, uint64_t* empty, uint8_t* ring, int code) -> bool {
+                    const int s = i % STAGES;
+                    if (!mbar_wait(&empty[s], ((uint32_t)(i / STAGES) & 1u) ^ 1u, ctl, code)) return false;
+                    long long r = row_of(i, which);
+                    if (r < 0) r = a.n_pages * 2 * a.KVH * BN;       // outside the map: zeros
+                    mbar_expect_tx(&full[s], (uint32_t)T_BYTES);
+                    for (int sb = 0; sb < SUB; sb++)
+                        tma_load_2d(ring + s * T_BYTES + sb * (BN * 128), &map_kv, &full[s], sb * 64, (int)r);
+                    return true;
+                };
+                if (any > 0) ok = load(0, 0, ctl->k_full, ctl->k_empty, k_s, 1);
+                for (int i = 0; i < any && ok; i++) {
+                    if (i + 1 < any) ok = load(i + 1, 0, ctl->k_full, ctl->k_empty, k_s, 1);
+                    if (ok) ok = load(i, 1, ctl->v_full, ctl->v_empty, v_s, 10);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- the products: the whole warp waits, one elected lane issues ----------------
+        const uint32_t idesc_s = umma_idesc(BM, BN, false, !EIGHT), idesc_o = umma_idesc(BM, HD, true, !EIGHT);
+        const uint64_t q_desc = umma_desc(smem_u32(q_s), 16, 1024), k_desc = umma_desc(smem_u32(k_s), 16, 1024);
+        const uint64_t v_desc = umma_desc(smem_u32(v_s), BN * 128, 1024);
+        bool ok = warp_wait(&ctl->q_full, 0, ctl, 3);
+        auto issue_s = [&](int i) {                          // S_i of every tile that has page i, into its buffer i & 1
+            const int s = i % STAGES;
+            const uint64_t kd = k_desc + (uint64_t)(s * (T_BYTES >> 4));
+            if (elect_one()) {
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    if (i >= n_blocks[t]) continue;
+                    const uint32_t d = tmem_base + (uint32_t)((t * 2 + (i & 1)) * BN);
+#pragma unroll
+                    for (int h = 0; h < (EIGHT ? 1 : 2); h++) {
+                        const uint64_t qd = q_desc + (uint64_t)((t * (EIGHT ? 1 : 2) + h) * (Q_BYTES >> 4));
+#pragma unroll
+                        for (int k = 0; k < HD / 16; k++) {
+                            const uint32_t sb = k / 4, kk = k % 4;
+                            umma(d, qd + (uint64_t)((sb * (BM * 128) + kk * 32) >> 4), kd + (uint64_t)((sb * (BN * 128) + kk * 32) >> 4),
+                                 idesc_s, (k > 0 || h > 0) ? 1u : 0u);
+                        }
+                    }
+                    umma_commit(&ctl->s_full[t][i & 1]);
+                }
+                umma_commit(&ctl->k_empty[s]);
+            }
+            __syncwarp();
+        };
+        if (ok && any > 0) {
+            ok = warp_wait(&ctl->k_full[0], 0, ctl, 4);
+            fence_after();
+            if (ok) issue_s(0);
+        }
+        for (int i = 0; i < any && ok; i++) {
+            if (i + 1 < any) {
+                ok = warp_wait(&ctl->k_full[(i + 1) % STAGES], (uint32_t)((i + 1) / STAGES) & 1u, ctl, 4);
+                if (!ok) break;
+                fence_after();
+                issue_s(i + 1);
+            }
+            const int s = i % STAGES;
+            ok = warp_wait(&ctl->v_full[s], (uint32_t)(i / STAGES) & 1u, ctl, 5);
+            if (!ok) break;
+            const uint64_t vd = v_desc + (uint64_t)(s * (T_BYTES >> 4));
+#pragma unroll
+            for (int t = 0; t < MT; t++) {
+                if (i >= n_blocks[t] || !ok) continue;
+                ok = warp_wait(&ctl->p_ready[t][i & 1], (uint32_t)(i >> 1) & 1u, ctl, 6);
+                if (!ok) continue;
+                fence_after();
+                const uint32_t p = tmem_base + (uint32_t)((t * 2 + (i & 1)) * BN), o = tmem_base + Z::S_COLS + (uint32_t)(t * HD);
+                if (elect_one()) {
+#pragma unroll
+                    for (int h = 0; h < (EIGHT ? 1 : 2); h++) {
+#pragma unroll
+                        for (int k = 0; k < BN / 16; k++)
+                            umma_ts(o, p + (uint32_t)(h * (BN / 2) + k * 8), vd + (uint64_t)((k * (16 * 128)) >> 4), idesc_o,
+                                    (i > 0 || k > 0 || h > 0) ? 1u : 0u);
+                    }
+                    umma_commit(&ctl->pv_done[t]);
+                    if (i == n_blocks[t] - 1) umma_commit(&ctl->o_done[t]);
+                }
+                __syncwarp();
+            }
+            if (ok && elect_one()) umma_commit(&ctl->v_empty[s]);
+            __syncwarp();
+        }
+    } else if (warp == 2) {
+        // ---------------- the scales: relative to R, and what R grew by ----------------
+        if (EIGHT) {
+            float ref = kv8_above(0.f);
+            const int key_hi = PREFIX ? 0x7fffffff : start + min(t0 + MT * tpt, count) - 1;
+            for (int i = 0; i < any; i++) {
+                const int c = i % SC_SLOTS;
+                if (!warp_wait(&ctl->sc_full[c], (uint32_t)(i / SC_SLOTS) & 1u, ctl, 11)) break;
+                Scales* sc = &ctl->sc[c];
+                const bool mapped = *(volatile int*)&sc->mapped != 0;
+                float2 v = *(const float2*)&sc->v[lane * 2];
+                const int key = (j_lo + i) * BN + lane * 2;
+                if (!mapped || key < key_lo || key > key_hi) v.x = 0.f;
+                if (!mapped || key + 1 < key_lo || key + 1 > key_hi) v.y = 0.f;
+                float most = fmaxf(fmaxf(v.x, 0.f), v.y);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float next = fmaxf(ref, kv8_above(most)), inv = kv8_inverse(next);
+                *(float2*)&sc->v[lane * 2] = make_float2(v.x * inv, v.y * inv);
+                if (lane == 0) { sc->grown = ref * inv; sc->ref = next; }
+                ref = next;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->sc_ready[c]);
+            }
+        }
+    } else if (EIGHT && warp >= 4 && warp < Z::FIRST) {
+        // ---------------- codes to 16-bit tiles ----------------
+        const int t = threadIdx.x - 128;
+        for (int i = 0; i < any; i++) {
+            const int s = i % STAGES;
+            const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
+            if (!warp_wait(&ctl->raw_full[s], ph, ctl, 12)) break;
+            if (!warp_wait(&ctl->k_empty[s], ph ^ 1u, ctl, 13)) break;
+            convert_tile<KIND>(raw_s + s * 2 * RAW, k_s + s * T_BYTES, t);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->k_full[s]);
+            if (!warp_wait(&ctl->v_empty[s], ph ^ 1u, ctl, 14)) break;
+            convert_tile<KIND>(raw_s + s * 2 * RAW + RAW, v_s + s * T_BYTES, t);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&ctl->v_full[s]); mbar_arrive(&ctl->raw_empty[s]); }
+        }
+    } else if (warp >= Z::FIRST) {
+        // ---------------- queries, softmax, output: one row a thread ----------------
+        const int tile = (warp - Z::FIRST) / 4, quarter = warp & 3;
+        const int r = quarter * 32 + lane;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t s_addr = lane_addr + (uint32_t)(tile * 2 * BN), o_addr = lane_addr + Z::S_COLS + (uint32_t)(tile * HD);
+        const int tok = t0 + tile * tpt + r / G, head = kvh * G + r % G;
+        const bool valid = r < tpt * G && tok < count;
+        int pos = 0, low = 0;
+        long long row = 0;                                 // the packed row of q and out
+        long long part = 0;
+        if (valid) {
+            if (PREFIX) {
+                const int sq = a.members[a.first[blockIdx.y] + tok];
+                row = a.cu_q[sq];
+                pos = a.seq_start[sq];
+                part = (long long)sq * a.H + head;
+            } else {
+                row = a.cu_q[b] + tok;
+                pos = start + tok;
+                low = oe_first_key(pos, a.window);
+                part = row * a.H + head;
+            }
+        }
+        float scale = a.scale_log2;
+        const int nb = n_blocks[tile];
+        {
+            uint8_t* qt = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES + r * 128;
+            const bf16* src = a.q + row * a.q_stride + (long long)head * HD;
+            const float* cs = a.cos_tab != nullptr ? a.cos_tab + (long long)pos * (HD / 2) : nullptr;
+            const float* sn = a.cos_tab != nullptr ? a.sin_tab + (long long)pos * (HD / 2) : nullptr;
+            float lo[8], hi[8], down = 1.f;
+            if (EIGHT && valid && nb > 0) {
+                float most = 0.f;
+#pragma unroll 4
+                for (int d = 0; d < HD / 2; d += 8) {
+                    turned8(src, cs, sn, d, lo, hi);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+                }
+                float up;
+                down = kv8_row_factor(most, &up);
+                scale *= up;
+            }
+#pragma unroll 4
+            for (int d = 0; d < HD / 2; d += 8) {
+                if (valid && nb > 0) {
+                    turned8(src, cs, sn, d, lo, hi);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) lo[e] = hi[e] = 0.f;
+                }
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int dim = d + half * (HD / 2);
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = (half ? hi[e] : lo[e]) * down;
+                    uint32_t w[4], rest[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        w[e] = pack16<EIGHT>(x[2 * e], x[2 * e + 1]);
+                        if (!EIGHT) rest[e] = rest_bf16(x[2 * e], x[2 * e + 1], w[e]);
+                    }
+                    uint8_t* to = qt + (dim / 64) * (BM * 128) + ((((dim % 64) / 8) ^ (r & 7)) << 4);
+                    *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (!EIGHT) *(uint4*)(to + Q_BYTES) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->q_full);
+        }
+        float m_run = -INFINITY, l_run = 0.f, ref = 1.f;
+        bool ok = true;
+        for (int i = 0; i < nb; i++) {
+            const int c = i % SC_SLOTS;
+            const Scales* sc = &ctl->sc[c];
+            if (EIGHT) ok = mbar_wait(&ctl->sc_ready[c], (uint32_t)(i / SC_SLOTS) & 1u, ctl, 15);
+            if (ok) ok = mbar_wait(&ctl->s_full[tile][i & 1], (uint32_t)(i >> 1) & 1u, ctl, 7);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            fence_after();
+            float s[BN];
+#pragma unroll
+            for (int c0 = 0; c0 < BN; c0 += 16) tmem_ld16_nowait(s_addr + (uint32_t)((i & 1) * BN + c0), &s[c0]);
+            tmem_ld_wait();
+            const int key0 = (j_lo + i) * BN;
+            bool mapped;
+            float grown = 1.f;
+            if (EIGHT) {
+                mapped = sc->mapped != 0;
+                grown = sc->grown;
+                ref = sc->ref;
+#pragma unroll
+                for (int k = 0; k < BN; k += 4) {
+                    const float4 f = *(const float4*)&sc->k[k];
+                    s[k] *= f.x; s[k + 1] *= f.y; s[k + 2] *= f.z; s[k + 3] *= f.w;
+                }
+            } else {
+                const int j = j_lo + i, page = j < a.max_pages ? trow[j] : -1;
+                mapped = (unsigned)page < (unsigned long long)a.n_pages;
+            }
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // a page wholly before a row's position, inside its window and of the cache needs no mask; the decision is the warp's, and
+            // rows without a token, whose results nobody stores, take no part in it
+            const bool masked = __any_sync(0xffffffffu, !mapped || (!PREFIX && valid && !(key0 + BN - 1 <= pos && key0 >= low)));
+            if (masked) {
+                const int hi = !mapped ? -1 : PREFIX ? BN - 1 : min(pos - key0, BN - 1), lo = PREFIX ? 0 : max(low - key0, 0);
+                const unsigned span = hi >= lo ? (unsigned)(hi - lo) : 0u;
+                const bool some = hi >= lo;
+#pragma unroll
+                for (int k = 0; k < BN; k++) s[k] = some && (unsigned)(k - lo) <= span ? s[k] : -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < BN; k++) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
+            const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale);
+            if (i == 0) {
+                m_run = m_new;
+            } else if (__any_sync(0xffffffffu, grown != 1.f || (valid && m_new > m_run + RESCALE_STEP))) {
+                // P_{i-1} V_{i-1} must have been added to O before O is rescaled (S_i is complete, hence P_{i-2} V_{i-2} too)
+                ok = mbar_wait(&ctl->pv_done[tile], (uint32_t)(i - 1) & 1u, ctl, 8);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                fence_after();
+                const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new)), beta = alpha * grown;
+#pragma unroll
+                for (int c0 = 0; c0 < HD; c0 += 16) {
+                    float ob[16];
+                    uint32_t ow[16];
+                    tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int d = 0; d < 16; d++) ow[d] = __float_as_uint(ob[d] * beta);
+                    tmem_st16(o_addr + (uint32_t)c0, ow);
+                }
+                tmem_st_wait();
+                l_run *= alpha;
+                m_run = m_new;
+            }
+            const float neg_m = (m_run == -INFINITY ? 0.f : -m_run) + Z::HEADROOM;
+            float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t p_addr = s_addr + (uint32_t)((i & 1) * BN);
+#pragma unroll
+            for (int k0 = 0; k0 < BN; k0 += 16) {
+                uint32_t w[8], rest[8];
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
+                    if (EIGHT) f = *(const float4*)&sc->v[k0 + k];
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        p[e] = fast_exp2(fmaf(s[k0 + k + e], scale, neg_m));
+                        sum4[e] += p[e];
+                    }
+                    if (EIGHT) {
+                        const bool gone = masked;
+                        p[0] = gone && s[k0 + k] == -INFINITY ? 0.f : p[0] * f.x;
+                        p[1] = gone && s[k0 + k + 1] == -INFINITY ? 0.f : p[1] * f.y;
+                        p[2] = gone && s[k0 + k + 2] == -INFINITY ? 0.f : p[2] * f.z;
+                        p[3] = gone && s[k0 + k + 3] == -INFINITY ? 0.f : p[3] * f.w;
+                    }
+                    w[k / 2] = pack16<EIGHT>(p[0], p[1]);
+                    w[k / 2 + 1] = pack16<EIGHT>(p[2], p[3]);
+                    if (!EIGHT) {
+                        rest[k / 2] = rest_bf16(p[0], p[1], w[k / 2]);
+                        rest[k / 2 + 1] = rest_bf16(p[2], p[3], w[k / 2 + 1]);
+                    }
+                }
+                tmem_st8(p_addr + (uint32_t)(k0 / 2), w);
+                if (!EIGHT) tmem_st8(p_addr + (uint32_t)(BN / 2 + k0 / 2), rest);
+            }
+            tmem_st_wait();
+            l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&ctl->p_ready[tile][i & 1]);
+                if (EIGHT) mbar_arrive(&ctl->sc_empty[c]);
+            }
+        }
+        // pages that only the other tile has: their scales' slots are given back all the same
+        if (EIGHT && ok) {
+            for (int i = nb; i < any; i++) {
+                const int c = i % SC_SLOTS;
+                if (!warp_wait(&ctl->sc_ready[c], (uint32_t)(i / SC_SLOTS) & 1u, ctl, 15)) break;
+                if (lane == 0) mbar_arrive(&ctl->sc_empty[c]);
+            }
+        }
+        if (ok) {
+            if (nb > 0) {
+                ok = mbar_wait(&ctl->o_done[tile], 0, ctl, 16);
+                ok = __all_sync(0xffffffffu, ok);
+                fence_after();
+            }
+            if (ok && (PREFIX || a.splits > 1)) {
+                float* po = a.part_o + (part * a.splits + split) * HD;
+                if (nb > 0) {
+#pragma unroll
+                    for (int c0 = 0; c0 < HD; c0 += 16) {
+                        float ob[16];
+                        tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
+                        tmem_ld_wait();
+                        if (valid) {
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4)
+                                *(float4*)(po + c0 + e) = make_float4(ob[e] * ref, ob[e + 1] * ref, ob[e + 2] * ref, ob[e + 3] * ref);
+                        }
+                    }
+                }
+                if (valid) *(float2*)(a.part_ml + (part * a.splits + split) * 2) = make_float2(m_run, l_run);
+            } else if (ok && nb > 0) {
+                const float inv = l_run > 0.f ? ref / l_run : l_run == 0.f ? 0.f : l_run;
+                bf16* dst = a.out + row * (long long)(a.H * HD) + (long long)head * HD;
+#pragma unroll
+                for (int c0 = 0; c0 < HD; c0 += 16) {
+                    float ob[16];
+                    tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
+                    tmem_ld_wait();
+                    if (valid) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 8) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int x = 0; x < 4; x++) w[x] = pack16<false>(ob[e + 2 * x] * inv, ob[e + 2 * x + 1] * inv);
+                            *(uint4*)(dst + c0 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+            }
+        }
+        fence_before();
+    }
+
+    __syncthreads();
+    if (*(volatile int*)&ctl->abort_flag) {
+        const unsigned long long t0w = global_ns();
+        while (global_ns() - t0w < 2000000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Z::COLS) : "memory");
+    }
+}
+
+// The parts of a prompt's rows joined, in the order of the splits: a warp per row.
+__global__ void __launch_bounds__(256)
+join_parts_kernel(bf16* out, const float* part_o, const float* part_ml, long long rows, int splits) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (r >= rows) return;
+    constexpr int PER = HD / 32;
+    float m = -INFINITY;
+    for (int q = 0; q < splits; q++) m = fmaxf(m, part_ml[(r * splits + q) * 2]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float o[PER] = {}, l = 0.f;
+    for (int q = 0; q < splits; q++) {
+        const float2 ml = *(const float2*)(part_ml + (r * splits + q) * 2);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;               // no key of this row: its O was not stored
+        const float w = exp2f(ml.x - mu);
+        l += ml.y * w;
+        const float* p = part_o + (r * splits + q) * HD + lane * PER;
+#pragma unroll
+        for (int e = 0; e < PER; e++) o[e] += p[e] * w;
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) *(uint32_t*)(out + r * HD + lane * PER + e) = pack16<false>(o[e] * inv, o[e + 1] * inv);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::mutex g_mutex;
+
+int get_encode() {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (g_encode) return 0;
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
+    if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || fn == nullptr) return e != cudaSuccess ? (int)e : 999;
+    g_encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+    return 0;
+}
+
+template <int KIND, bool PREFIX, int MT>
+int launch(const CUtensorMap& map, const Args& a, dim3 grid, cudaStream_t st) {
+    using Z = Shape<KIND, MT>;
+    const size_t smem = (size_t)Z::BYTES + 1024;
+    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<KIND, PREFIX, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    return oe_launch(attn_rows_kernel<KIND, PREFIX, MT>, grid, dim3(Z::THREADS), smem, st, map, a);
+}
+template <int KIND, bool PREFIX>
+int launch_tiles(int mt, const CUtensorMap& map, const Args& a, dim3 grid, cudaStream_t st) {
+    return mt == 1 ? launch<KIND, PREFIX, 1>(map, a, grid, st) : launch<KIND, PREFIX, 2>(map, a, grid, st);
+}
+
+bool operands_ok(const Args& a, const void* cache) {
+    return a.KVH > 0 && a.H % a.KVH == 0 && a.H / a.KVH <= BM && a.q_stride % 8 == 0 && !((uintptr_t)a.q & 15) && !((uintptr_t)cache & 15) &&
+           !((uintptr_t)a.scales & 15) && !((uintptr_t)a.cos_tab & 15) && !((uintptr_t)a.sin_tab & 15) && a.splits >= 1 && a.n_pages >= 1;
+}
+
+}  // namespace
+
+extern "C" {
+
+// Attention of the step's tokens over the 8-bit cache (kind OE_KV_INT8 or OE_KV_E4M3), which has their rows already.  mt: tiles of 128
+// rows a CTA has (1 or 2); splits > 1: the pages of a tile are cut into as many runs, whose parts go through part_o
+// [T * H, splits, HD] and part_ml [T * H, splits, 2].
+int oe_attn_rows(int kind, bf16* out, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, const void* cache,
+                 const float* scales, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
+                 const int* seq_qlen, int n_seqs, int n_tokens, int max_qlen, int H, int KVH, int window, float scale, int mt, int splits,
+                 float* part_o, float* part_ml, cudaStream_t st) {
+    if (n_seqs <= 0 || max_qlen <= 0) return 0;
+    Args a = {};
+    a.out = out; a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.codes = (const uint8_t*)cache;
+    a.scales = scales; a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start;
+    a.seq_qlen = seq_qlen; a.H = H; a.KVH = KVH; a.window = window; a.scale_log2 = scale * LOG2E;
+    a.splits = splits; a.part_o = part_o; a.part_ml = part_ml;
+    if (!operands_ok(a, cache) || ((uintptr_t)out & 15) || (mt != 1 && mt != 2)) return OE_ERR_UNSUPPORTED;
+    if (splits > 1 && (part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
+    const int tpt = BM / (H / KVH) * mt;
+    const long long tiles = ((long long)max_qlen + tpt - 1) / tpt, x = (long long)KVH * splits;
+    if (tiles > 65535 || n_seqs > 65535 || x > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)x, n_seqs, (unsigned)tiles);
+    const CUtensorMap none = {};
+    int rc = OE_ERR_UNSUPPORTED;
+    if (kind == OE_KV_INT8) rc = launch_tiles<OE_KV_INT8, false>(mt, none, a, grid, st);
+    else if (kind == OE_KV_E4M3) rc = launch_tiles<OE_KV_E4M3, false>(mt, none, a, grid, st);
+    if (rc || splits == 1) return rc;
+    const long long rows = (long long)n_tokens * H;
+    return oe_launch(join_parts_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, out, (const float*)part_o, (const float*)part_ml,
+                     rows, splits);
+}
+
+// The parts of the groups' prefixes (see oe_attn_kv8_prefix) into part_o [B * H, splits, HD] and part_ml [B * H, splits, 2].
+int oe_attn_rows_prefix(int kind, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, const void* cache,
+                        const float* scales, long long n_pages, const int* tables, int max_pages, const int* cu_q,
+                        const int* seq_start, int H, int KVH, float scale, const int* members, const int* first, const int* pages,
+                        int n_groups, int n_members, int mt, int splits, float* part_o, float* part_ml, int ahead, cudaStream_t st) {
+    if (n_groups <= 0 || n_members <= 0) return 0;
+    Args a = {};
+    a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.codes = (const uint8_t*)cache; a.scales = scales;
+    a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start; a.H = H; a.KVH = KVH;
+    a.scale_log2 = scale * LOG2E; a.members = members; a.first = first; a.pages = pages; a.splits = splits;
+    a.part_o = part_o; a.part_ml = part_ml; a.ahead = ahead;
+    if (!operands_ok(a, cache) || (mt != 1 && mt != 2) || part_o == nullptr || part_ml == nullptr) return OE_ERR_UNSUPPORTED;
+    const int tpt = BM / (H / KVH) * mt;
+    const long long tiles = ((long long)n_members + tpt - 1) / tpt, x = (long long)KVH * splits;
+    if (tiles > 65535 || n_groups > 65535 || x > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)x, n_groups, (unsigned)tiles);
+    CUtensorMap map = {};
+    if (kind == OE_KV_BF16) {
+        // the cache entry as rows of HD: [pages * 2 * KVH * 64][HD]; a box is 64 rows x 64 dims
+        if (n_pages * 2 * KVH * BN > 0x7fffffffLL - BN) return OE_ERR_UNSUPPORTED;
+        int rc = get_encode();
+        if (rc) return rc;
+        cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)n_pages * 2 * KVH * BN};
+        cuuint64_t strides[1] = {(cuuint64_t)HD * 2};
+        cuuint32_t box[2] = {64, (cuuint32_t)BN};
+        cuuint32_t es[2] = {1, 1};
+        CUresult r = g_encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, es,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return 2000 + (int)r;
+        return launch_tiles<OE_KV_BF16, true>(mt, map, a, grid, st);
+    }
+    if (kind == OE_KV_INT8) return launch_tiles<OE_KV_INT8, true>(mt, map, a, grid, st);
+    if (kind == OE_KV_E4M3) return launch_tiles<OE_KV_E4M3, true>(mt, map, a, grid, st);
+    return OE_ERR_UNSUPPORTED;
+}
+
+int oe_attn_rows_error() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) cudaMemcpyToSymbol(g_error, &zero, sizeof(int));
+    return v;
+}
+
+}  // extern "C"

@@ -58,6 +58,7 @@ LIBRARIES = {
     "attention_split_tc": ("attention_split_mma.cu", []),
     "head_matmul_tc": ("head_matmul_mma.cu", []),
     "attention_kv8": ("attention_kv8.cu", []),
+    "attention_rows": ("attention_rows.cu", []),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}
@@ -200,7 +201,7 @@ def build_all(names=None, verbose: bool = True) -> list[Path]:
     for n in names:
         if n == "attention_tc":
             jobs.extend((n, {"OE_HD": hd}) for hd in DEFAULT_HEAD_DIMS)
-        elif n in ("attention_tc5", "attention_kv8"):
+        elif n in ("attention_tc5", "attention_kv8", "attention_rows"):
             jobs.extend((n, {"OE_HD": hd}) for hd in (64, 128))
         elif n == "attention_split_tc":
             jobs.extend((n, {"OE_DK": dk, "OE_DV": dv}) for dk, dv in ((64, 128), (128, 128)))

@@ -1,5 +1,5 @@
 """The 8-bit paged cache and the attention that reads it, and the attention of sequences that begin with the same pages
-(csrc/attention_kv8.cu, one library per head size).
+(csrc/attention_kv8.cu: the write, and few rows; csrc/attention_rows.cu: many; one library of each per head size).
 
 A `cache` argument is one cache entry: a pair (codes [pages, 2, KVH, PAGE, hd] int8 or float8_e4m3fn, scales float32 [pages, 2, KVH,
 PAGE]), or, where a function says so, the 16-bit entry [pages, 2, KVH, PAGE, hd] bfloat16.  A row (one token's key or value of one KV
@@ -21,6 +21,8 @@ from . import ops
 from .ops import PAGE, KernelError
 
 HEAD_DIMS = (64, 128)
+FEW_ROWS = 16        # rows of a tile of attention_kv8.cu
+TILE_ROWS = 128      # rows (a token's or member's heads of one KV head) of a tile of attention_rows.cu; must equal its BM
 CODE_TYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 _KINDS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
 _libs: dict = {}
@@ -34,16 +36,36 @@ def _lib(head_dim: int):
         lib = _build.load("attention_kv8", {"OE_HD": head_dim})
         P, I, F, L = c_void_p, c_int, c_float, c_longlong
         lib.oe_kv8_write.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, I, P]
-        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, P, I, P, I, P]
-        lib.oe_attn_kv8_prefix.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, F, P, P, P, I, I, I, P, I, P]
-        for f in (lib.oe_kv8_write, lib.oe_attn_kv8, lib.oe_attn_kv8_prefix):
-            f.restype = c_int
+        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, P, I, P, P, I, P]
+        lib.oe_kv8_write.restype = lib.oe_attn_kv8.restype = c_int
         _libs[head_dim] = lib
     return lib
 
 
+def _rows_lib(head_dim: int):
+    lib = _libs.get(("rows", head_dim))
+    if lib is None:
+        lib = _build.load("attention_rows", {"OE_HD": head_dim})
+        P, I, F, L = c_void_p, c_int, c_float, c_longlong
+        lib.oe_attn_rows.argtypes = [I, P, P, L, P, P, P, P, L, P, I, P, P, P, I, I, I, I, I, I, F, I, I, P, P, P]
+        lib.oe_attn_rows_prefix.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, F, P, P, P, I, I, I, I, P, P, I, P]
+        lib.oe_attn_rows_error.argtypes = []
+        lib.oe_attn_rows.restype = lib.oe_attn_rows_prefix.restype = lib.oe_attn_rows_error.restype = c_int
+        _libs[("rows", head_dim)] = lib
+    return lib
+
+
+def device_error() -> int:
+    """The code of a bounded wait that ran out since the last call (0: none).  Synchronises the device."""
+    code = 0
+    for key, lib in list(_libs.items()):
+        if isinstance(key, tuple):
+            code = code or int(lib.oe_attn_rows_error())
+    return code
+
+
 def supported(head_dim: int, n_heads: int, n_kv_heads: int) -> bool:
-    return head_dim in HEAD_DIMS and n_kv_heads >= 1 and n_heads % n_kv_heads == 0 and n_heads >= n_kv_heads
+    return head_dim in HEAD_DIMS and n_kv_heads >= 1 and n_heads % n_kv_heads == 0 and 1 <= n_heads // n_kv_heads <= TILE_ROWS
 
 
 def _cache_args(what: str, cache, n_kv_heads: int, head_dim: int, allow_16: bool) -> tuple:
@@ -135,7 +157,7 @@ def decode_cluster(n_seqs: int, n_kv_heads: int, context_class: int, sm_count: i
 
 
 def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float,
-                  has_kv: bool = True, ahead: bool = False, cluster: int | None = None) -> None:
+                  has_kv: bool = True, ahead: bool = False, cluster: int | None = None, form: tuple | None = None) -> None:
     """Rotation, cache write (has_kv) and attention of the step's tokens over the 8-bit cache: out[t] is the attention of token t's
     query heads over its sequence's keys up to its own position (window 0: all of them, n > 0: the last n, -n: those of the
     chunk of n positions it lies in), as the cache keeps them, the step's own among them.
@@ -155,19 +177,59 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
     single = bool(ctx.all_decode) and T == ctx.n_seqs
     if has_kv and not single:
         kv8_write(qkv, cos, sin, cache, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
-    if cluster is None:
-        cluster = decode_cluster(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0)) if single else 1
-    ops._check(_lib(head_dim).oe_attn_kv8(
-        kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(),
-        int(has_kv and single), codes.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
-        ctx.seq_qlen.data_ptr(), ctx.n_seqs, 1 if single else max(1, ctx.max_qlen), n_heads, n_kv_heads, int(window), float(scale),
-        int(cluster), None, 0, None, int(ahead), ops._stream()), what, {"cluster": int(cluster)})
+    few = max(1, ctx.max_qlen) * (n_heads // n_kv_heads) <= FEW_ROWS
+    if single or few:
+        if cluster is None:
+            cluster = decode_cluster(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0))
+        ops._check(_lib(head_dim).oe_attn_kv8(
+            kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(),
+            int(has_kv and single), codes.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
+            ctx.seq_qlen.data_ptr(), ctx.n_seqs, 1 if single else max(1, ctx.max_qlen), n_heads, n_kv_heads, int(window), float(scale),
+            int(cluster), None, 0, None, None, int(ahead), ops._stream()), what, {"cluster": int(cluster)})
+        return
+    if form is None:
+        form = prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
+    mt, splits = form
+    part = _parts(T * n_heads, splits, head_dim, out.device) if splits > 1 else None
+    ops._check(_rows_lib(head_dim).oe_attn_rows(
+        kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+        tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(), ctx.seq_qlen.data_ptr(), ctx.n_seqs, T,
+        ctx.max_qlen, n_heads, n_kv_heads, int(window), float(scale), mt, splits, *_part_ptrs(part, T * n_heads, splits, head_dim),
+        ops._stream()), what, {"tiles": mt, "splits": splits})
+    if splits > 1:
+        ops.LAUNCHES[0] += 1
 
 
-def prefix_splits(n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, sm_count: int | None = None) -> int:
-    """Into how many parts the pages of a prefix are cut."""
-    tiles = max(1, (n_members * group + 15) // 16) * n_kv_heads
-    return max(1, min(max_pages, 2 * (sm_count or ops.sm_count()) // tiles, 32))
+def _parts(rows: int, splits: int, head_dim: int, device):
+    """Room for the parts of `rows` rows: their sums, then maxima and sums of weights."""
+    return torch.empty(rows * splits * (head_dim + 2), dtype=torch.float32, device=device)
+
+
+def _part_ptrs(part, rows: int, splits: int, head_dim: int) -> tuple:
+    if part is None:
+        return None, None
+    return part.data_ptr(), part.data_ptr() + 4 * rows * splits * head_dim
+
+
+def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context_class: int, window: int, sm_count: int | None = None) -> tuple:
+    """(tiles of 128 rows a CTA has, runs that a tile's pages are cut into) of a step of prompts."""
+    sms = sm_count or ops.sm_count()
+    tiles = n_tokens // (TILE_ROWS // group) + n_seqs
+    mt = 2 if tiles > 1 else 1
+    ctas = -(-tiles // mt) * n_kv_heads
+    pages = (12, 24, 64, 128)[context_class]
+    if window:
+        pages = min(pages, abs(window) // PAGE + 2)
+    return mt, max(1, min(sms // ctas, pages // 4, 16))
+
+
+def prefix_form(n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, sm_count: int | None = None) -> tuple:
+    """(tiles of 128 rows a CTA has, runs that a prefix's pages are cut into)."""
+    sms = sm_count or ops.sm_count()
+    tiles = -(-n_members // (TILE_ROWS // group))
+    mt = 2 if tiles > 1 else 1
+    ctas = (-(-tiles // mt) + n_groups - 1) * n_kv_heads
+    return mt, max(1, min(max_pages, sms // ctas))
 
 
 def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
@@ -196,16 +258,16 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
             raise KernelError(f"{what}: {n} holds {t.numel()} numbers, {least} are needed")
     if B == 0:
         return
-    lib, group = _lib(head_dim), n_heads // n_kv_heads
-    splits = prefix_splits(prefix.n_members, prefix.n_groups, group, n_kv_heads, max(1, prefix.max_pages))
-    partial = torch.empty(B * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device)
     step = (rows.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr())
+    mt, splits = prefix_form(max(1, prefix.n_members), max(1, prefix.n_groups), n_heads // n_kv_heads, n_kv_heads, max(1, prefix.max_pages))
+    part = _parts(B * n_heads, splits, head_dim, out.device)
+    parts = _part_ptrs(part, B * n_heads, splits, head_dim)
     if prefix.n_groups > 0 and prefix.n_members > 0:
-        ops._check(lib.oe_attn_kv8_prefix(
+        ops._check(_rows_lib(head_dim).oe_attn_rows_prefix(
             kind, qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), *step, n_heads, n_kv_heads,
             float(scale), prefix.members.data_ptr(), prefix.first.data_ptr(), prefix.pages.data_ptr(), prefix.n_groups,
-            prefix.n_members, splits, partial.data_ptr(), int(ahead), ops._stream()), "attention_shared_prefix", {"splits": splits})
-    ops._check(lib.oe_attn_kv8(
+            prefix.n_members, mt, splits, *parts, int(ahead), ops._stream()), "attention_shared_prefix", {"tiles": mt, "splits": splits})
+    ops._check(_lib(head_dim).oe_attn_kv8(
         kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), int(has_kv),
         *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 1, prefix.seq_pages.data_ptr(), splits,
-        partial.data_ptr(), int(ahead), ops._stream()), what)
+        *parts, int(ahead), ops._stream()), what)

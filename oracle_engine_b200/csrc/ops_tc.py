@@ -13,7 +13,7 @@ from ctypes import c_float, c_int, c_longlong, c_void_p
 import torch
 
 from . import build as _build
-from . import ops
+from . import ops, ops_kv8
 from .ops import KernelError
 
 _state: dict = {}
@@ -334,7 +334,7 @@ def device_error() -> int:
     for key, lib in list(_state.items()):
         if isinstance(key, tuple) and key[0] == "attn_tc5":
             code = code or int(lib.oe_attn_tc_error())
-    return code
+    return code or ops_kv8.device_error()
 
 
 # ----------------------------------------------------------------------------------------

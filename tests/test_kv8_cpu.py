@@ -65,7 +65,11 @@ def test_split_and_cluster_rules():
                 c = ops_kv8.decode_cluster(n, kvh, cls, 148)
                 assert c in (1, 2, 4, 8) and (c == 1 or n * kvh * c <= 148)
             for pages in (1, 5, 500):
-                assert 1 <= ops_kv8.prefix_splits(n, 1, 4, kvh, pages, 148) <= pages
+                mt, splits = ops_kv8.prefix_form(n, 1, 4, kvh, pages, 148)
+                assert mt in (1, 2) and 1 <= splits <= pages
+            for tokens in (1, 40, 5000):
+                mt, splits = ops_kv8.prompt_form(tokens, n, 4, kvh, cls, 0, 148)
+                assert mt in (1, 2) and 1 <= splits <= 16
 
 
 def test_the_plain_rounding():

@@ -1,20 +1,23 @@
 // Attention of a few rows at a time over the paged cache in its 8-bit forms (kv8.cuh) or in bfloat16, and the write of the
 // 8-bit forms; compiled for one head size: -DOE_HD=64 or 128.
 //
-// A row is a (token, query head of the group) pair.  A CTA (or a cluster of CTAs) has 16 rows of one KV head and a range of
+// A row is a (token, query head of the group) pair.  A CTA (or a cluster of CTAs) has up to 8 NT rows of one KV head and a range of
 // keys; its warps split the keys in tiles of 32, each with a ring of tiles of its own that cp.async fills and a running
 // softmax of its own, and the results are added up in warp order, then in rank order, through shared memory.
-//   S = Q K^T, O += P V     mma.sync m16n8k16 with float32 sums.
+//   S^T = K Q^T, O^T += V^T P^T     mma.sync m16n8k16 with float32 sums: keys, then dimensions, are the 16 rows of a product and the
+//                           query rows its 8 columns, so that a group of up to 8 heads leaves nothing of it empty.
 //     8-bit forms           float16: a code is a float16 exactly, so K and V enter as codes.  The turned queries are rounded to float16
 //                           (2^-12 of themselves; a row is scaled by a power of two first), the key's scale multiplies the score's
 //                           sum, and the weight p times the value's scale is rounded to float16: relative to R, the largest power of
 //                           two above a value's scale so far, and times 2^8, so that what float16 cannot hold is below 2^-33 of the
-//                           row's largest weight.  When R grows, O is scaled down with the step that a grown maximum takes anyway.
+//                           row's largest weight.
 //     bfloat16              K and V as they are.  Turned queries and weights enter as the sum of two bfloat16 (2^-17 of themselves), which
 //                           costs a second product each in a kernel that waits for memory.
-//   Fragments               the dimensions of a product's inner axis and the columns of its result may be in any order that both
-//                           operands keep, so a lane takes 4 dimensions of a row that lie together: K needs one 32-bit load of
-//                           codes a k-step, V one for 4 dimensions of each of 4 keys, whose bytes are paired by permutes.
+//   Reference maximum       moves only when a row's maximum has grown by more than 2^7 since it was set; with it, or when R grows, O is
+//                           rescaled, which the factor in the sum cancels.
+//   Fragments               the dimensions of a product's inner axis and its rows may be in any order that both operands keep, so a
+//                           lane takes 4 dimensions of a row that lie together: K needs one 32-bit load of codes a k-step, V one for 4
+//                           dimensions of each of 4 keys, whose bytes are paired by permutes.  P^T comes from S^T by movmatrix.
 // Masks: key <= the row's position; window > 0 the last `window` keys, window < 0 the keys of the row's chunk.  A masked key's weight is
 // set to zero whatever its score and scale are, so rows behind the last token of a page may hold anything.
 // A page number outside the cache counts as a page without keys.
@@ -31,6 +34,7 @@ static_assert(HD == 64 || HD == 128, "built for head_dim 64 or 128");
 constexpr int KS = HD / 16;
 constexpr int TB = 32;                           // keys per tile: half a page
 constexpr int PARTS = OE_PAGE / TB;
+constexpr int MAX_JOINED = 160;                  // parts that a result is joined from: a cluster's CTAs and a prefix's splits
 constexpr float LOG2E = 1.4426950408889634f;
 
 // ------------------------------------------------------------------------------------------------ the write
@@ -171,11 +175,20 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
-__device__ __forceinline__ float ld_peer_f32(const float* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank) {
     uint32_t addr;
-    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return addr;
+}
+__device__ __forceinline__ float4 ld_peer4(const float* p, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_address(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_peer2(const float* p, uint32_t rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer_address(p, rank)) : "memory");
     return v;
 }
 
@@ -258,29 +271,47 @@ struct NewToken {
     }
 };
 
+// The largest value scale of a tile: lane k has key k's.
+__device__ __forceinline__ float warp_most(float v) {
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v, 0.f))));     // (an undefined one counts as none)
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+    return d;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // The rows are those of one sequence's new tokens (blockIdx.z), the keys its own, from behind its prefix on if it has one, whose
 // parts are joined with the result.
-template <int KIND, int NW, int ST>
+template <int KIND, int NT, int NW, int ST>
 __global__ void __launch_bounds__(NW * 32)
 attn_kv8_kernel(const Args a) {
     using L = Tile<KIND>;
-    constexpr int WARP_BYTES = ST * L::BYTES;
-    static_assert((NW + 1) * 16 * (HD + 2) * 4 <= NW * WARP_BYTES, "the parts lie where the rings were");
+    constexpr bool EIGHT = KIND != OE_KV_BF16;
+    constexpr int ROWS = 8 * NT, WARP_BYTES = ST * L::BYTES, OD = HD + 4;
+    constexpr float HEADROOM = EIGHT ? 8.f : 0.f, RESCALE_STEP = 7.f;
+    static_assert((NW + 1) * ROWS * OD * 4 + ROWS * (MAX_JOINED + NW + 1) * 4 <= NW * WARP_BYTES, "the parts lie where the rings were");
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     const int G = a.H / a.KVH, kvh = blockIdx.y;
     const int CR = a.cluster, rank = CR > 1 ? (int)cluster_ctarank() : 0;
     const int bx = blockIdx.x / CR;
-    const int b = blockIdx.z, row0 = bx * 16, qlen = a.seq_qlen[b], n_rows = qlen > 0 ? qlen * G : 0;
+    const int b = blockIdx.z, row0 = bx * ROWS, qlen = a.seq_qlen[b], n_rows = qlen > 0 ? qlen * G : 0;
     if (row0 >= n_rows) {                                            // the whole cluster
         pdl_wait();
         return;
     }
     const int start = a.seq_start[b];
     const long long packed0 = a.cu_q[b];
+    const int rows = min(ROWS, n_rows - row0);
     int key_lo = oe_first_key(start + row0 / G, a.window);
-    const int key_hi = start + min(row0 + 15, n_rows - 1) / G;
+    const int key_hi = start + (row0 + rows - 1) / G;
     const int common = a.seq_pages != nullptr ? a.seq_pages[b] : 0;
     key_lo = max(key_lo, common * OE_PAGE);
     const int* trow = a.tables + (size_t)b * a.max_pages;
@@ -303,81 +334,75 @@ attn_kv8_kernel(const Args a) {
     }
     if (ahead) pdl_wait();
 
-    // this thread's two rows
-    bool valid[2];
-    int head[2], pos[2], low[2];
-    long long tok[2];
+    // Q fragments, turned, of the rows nt * 8 + gid: qf, and for a 16-bit cache what its rounding leaves; a row's power of two
+    constexpr int KL = EIGHT ? 1 : KS;
+    uint32_t qf[NT][KS][2], ql[NT][KL][2];
+    float up[NT];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int r = row0 + gid + i * 8;
-        valid[i] = r < n_rows;
-        const int rr = valid[i] ? r : row0;
-        head[i] = kvh * G + rr % G;
-        tok[i] = packed0 + rr / G;
-        pos[i] = start + rr / G;
-        low[i] = oe_first_key(pos[i], a.window);
-    }
-    // Q fragments, turned: qf, and for a 16-bit cache what its rounding leaves
-    constexpr int KL = KIND == OE_KV_BF16 ? KS : 1;
-    uint32_t qf[KS][4], ql[KL][4];
-    float row_scale[2] = {a.scale_log2, a.scale_log2};
-    {
-        float qv[KS][4][2];
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = nt * 8 + gid, rr = row0 + (r < rows ? r : 0), pos = start + rr / G;
+        const bf16* src = a.q + (packed0 + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * HD + tig * 4;
+        float qv[KS][4];
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                uint2 w = make_uint2(0u, 0u);
-                if (valid[i]) w = *(const uint2*)(a.q + tok[i] * a.q_stride + (size_t)head[i] * HD + ks * 16 + tig * 4);
-                qv[ks][i][0] = kv8_from_bits(w.x & 0xffffu); qv[ks][i][1] = kv8_from_bits(w.x >> 16);
-                qv[ks][i + 2][0] = kv8_from_bits(w.y & 0xffffu); qv[ks][i + 2][1] = kv8_from_bits(w.y >> 16);
-            }
+            const uint2 w = r < rows ? *(const uint2*)(src + ks * 16) : make_uint2(0u, 0u);
+            qv[ks][0] = kv8_from_bits(w.x & 0xffffu); qv[ks][1] = kv8_from_bits(w.x >> 16);
+            qv[ks][2] = kv8_from_bits(w.y & 0xffffu); qv[ks][3] = kv8_from_bits(w.y >> 16);
         }
         if (a.cos_tab != nullptr) {
 #pragma unroll
             for (int ks = 0; ks < KS / 2; ks++) {
+                const float4 c = *(const float4*)(a.cos_tab + (size_t)pos * (HD / 2) + ks * 16 + tig * 4);
+                const float4 n = *(const float4*)(a.sin_tab + (size_t)pos * (HD / 2) + ks * 16 + tig * 4);
+                const float cc[4] = {c.x, c.y, c.z, c.w}, nn[4] = {n.x, n.y, n.z, n.w};
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int d = ks * 16 + tig * 4 + (x >> 1) * 2;
-                    const float2 cs = *(const float2*)(a.cos_tab + (size_t)pos[x & 1] * (HD / 2) + d);
-                    const float2 sn = *(const float2*)(a.sin_tab + (size_t)pos[x & 1] * (HD / 2) + d);
-                    const float x0 = qv[ks][x][0], x1 = qv[ks][x][1], y0 = qv[ks + KS / 2][x][0], y1 = qv[ks + KS / 2][x][1];
-                    qv[ks][x][0] = x0 * cs.x - y0 * sn.x;
-                    qv[ks][x][1] = x1 * cs.y - y1 * sn.y;
-                    qv[ks + KS / 2][x][0] = x0 * sn.x + y0 * cs.x;
-                    qv[ks + KS / 2][x][1] = x1 * sn.y + y1 * cs.y;
+                for (int e = 0; e < 4; e++) {
+                    const float x = qv[ks][e], y = qv[ks + KS / 2][e];
+                    qv[ks][e] = x * cc[e] - y * nn[e];
+                    qv[ks + KS / 2][e] = x * nn[e] + y * cc[e];
                 }
             }
         }
-        if (KIND == OE_KV_BF16) {
+        float down = 1.f;
+        up[nt] = 1.f;
+        if (EIGHT) {
+            float most = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    qf[ks][x] = pack_bf16(qv[ks][x][0], qv[ks][x][1]);
-                    ql[ks < KL ? ks : 0][x] = rest_bf16(qv[ks][x][0], qv[ks][x][1], qf[ks][x]);
+                for (int e = 0; e < 4; e++) most = fmaxf(most, fabsf(qv[ks][e]));
+            }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            down = kv8_row_factor(most, &up[nt]);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const float q0 = qv[ks][2 * x] * down, q1 = qv[ks][2 * x + 1] * down;
+                if (EIGHT) {
+                    qf[nt][ks][x] = pack_f16(q0, q1);
+                } else {
+                    qf[nt][ks][x] = pack_bf16(q0, q1);
+                    ql[nt][EIGHT ? 0 : ks][x] = rest_bf16(q0, q1, qf[nt][ks][x]);
                 }
             }
-        } else {
-            float most[2] = {0.f, 0.f}, down[2];
+        }
+    }
+    // this lane's columns of S^T and O^T: rows nt * 8 + tig * 2 + e
+    float row_scale[NT][2], m_run[NT][2], l_run[NT][2];
+    int pos[NT][2], low[NT][2];
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
+    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                for (int x = 0; x < 4; x++) most[x & 1] = fmaxf(most[x & 1], fmaxf(fabsf(qv[ks][x][0]), fabsf(qv[ks][x][1])));
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 1));
-                most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 2));
-                float up;
-                down[i] = kv8_row_factor(most[i], &up);
-                row_scale[i] *= up;
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-#pragma unroll
-                for (int x = 0; x < 4; x++) qf[ks][x] = pack_f16(qv[ks][x][0] * down[x & 1], qv[ks][x][1] * down[x & 1]);
-            }
+        for (int e = 0; e < 2; e++) {
+            const int r = nt * 8 + tig * 2 + e, rr = row0 + (r < rows ? r : 0);
+            pos[nt][e] = start + rr / G;
+            low[nt][e] = oe_first_key(pos[nt][e], a.window);
+            row_scale[nt][e] = a.scale_log2 * __shfl_sync(0xffffffffu, up[nt], (tig * 2 + e) * 4);
+            m_run[nt][e] = -INFINITY;
+            l_run[nt][e] = 0.f;
         }
     }
     // the warp that meets the new token's tile makes that token's rows and stores them in the cache
@@ -389,136 +414,153 @@ attn_kv8_kernel(const Args a) {
         if ((unsigned)page < (unsigned long long)a.n_pages) {
             const long long krow = (((long long)page * 2) * a.KVH + kvh) * OE_PAGE + start % OE_PAGE, vrow = krow + (long long)a.KVH * OE_PAGE;
             fresh.store((uint8_t*)a.cache_w + krow * (HD * L::ELEM), (uint8_t*)a.cache_w + vrow * (HD * L::ELEM), lane);
-            if (KIND != OE_KV_BF16 && lane == 0) { a.scales_w[krow] = fresh.ks; a.scales_w[vrow] = fresh.vs; }
+            if (EIGHT && lane == 0) { a.scales_w[krow] = fresh.ks; a.scales_w[vrow] = fresh.vs; }
         }
     }
 
-    float oacc[HD / 8][4];
+    float oacc[NT][HD / 16][4];
 #pragma unroll
-    for (int n = 0; n < HD / 8; n++) { oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f; }
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int n = 0; n < HD / 16; n++) { oacc[nt][n][0] = oacc[nt][n][1] = oacc[nt][n][2] = oacc[nt][n][3] = 0.f; }
+    }
     float ref = kv8_above(0.f);                             // R: what O is relative to
-    constexpr float HEADROOM = KIND == OE_KV_BF16 ? 0.f : 8.f;
     int stage = 0;
     for (int it = 0; it < n_my; it++) {
         const int tile = t_lo + gw + it * stride;
         uint8_t* cur = mine + (size_t)stage * L::BYTES;
-        const uint8_t* vs_cur = cur + L::V_AT;
         cp_async_wait<ST - 1>();
         __syncwarp();
         if (own_kv && tile == t_hi) {
             const int r = start % TB;
             fresh.store(cur + r * L::K_ROW, cur + L::V_AT + r * L::V_ROW, lane);
-            if (KIND != OE_KV_BF16 && lane == 0) { ((float*)(cur + L::S_AT))[r] = fresh.ks; ((float*)(cur + L::S_AT))[TB + r] = fresh.vs; }
+            if (EIGHT && lane == 0) { ((float*)(cur + L::S_AT))[r] = fresh.ks; ((float*)(cur + L::S_AT))[TB + r] = fresh.vs; }
             __syncwarp();
         }
-        const bool mapped = (unsigned)page_at(trow, tile / PARTS, a.max_pages) < (unsigned long long)a.n_pages;
-        if (mapped) {
-            float s[TB / 8][4];
+        if ((unsigned)page_at(trow, tile / PARTS, a.max_pages) < (unsigned long long)a.n_pages) {
+            float s[NT][TB / 16][4];
 #pragma unroll
-            for (int n = 0; n < TB / 8; n++) {
-                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-                const uint8_t* kr = cur + (n * 8 + gid) * L::K_ROW + tig * 4 * L::ELEM;
+            for (int mt = 0; mt < TB / 16; mt++) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
+                const uint8_t* kr = cur + (mt * 16 + gid) * L::K_ROW + tig * 4 * L::ELEM;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
-                    if (KIND == OE_KV_BF16) {
-                        const uint2 w = *(const uint2*)(kr + ks * 32);
-                        mma_bf16(s[n], qf[ks], w.x, w.y);
-                        mma_bf16(s[n], ql[ks < KL ? ks : 0], w.x, w.y);
+                    uint32_t f[4];
+                    if (EIGHT) {
+                        const uint32_t w0 = kv8_word<KIND>(*(const uint32_t*)(kr + ks * 16));
+                        const uint32_t w1 = kv8_word<KIND>(*(const uint32_t*)(kr + 8 * L::K_ROW + ks * 16));
+                        f[0] = kv8_pair<KIND>(w0, 0); f[2] = kv8_pair<KIND>(w0, 2);
+                        f[1] = kv8_pair<KIND>(w1, 0); f[3] = kv8_pair<KIND>(w1, 2);
                     } else {
-                        const uint32_t w = kv8_word<KIND>(*(const uint32_t*)(kr + ks * 16));
-                        mma_f16(s[n], qf[ks], kv8_pair<KIND>(w, 0), kv8_pair<KIND>(w, 2));
+                        const uint2 w0 = *(const uint2*)(kr + ks * 32), w1 = *(const uint2*)(kr + 8 * L::K_ROW + ks * 32);
+                        f[0] = w0.x; f[2] = w0.y; f[1] = w1.x; f[3] = w1.y;
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        if (EIGHT) {
+                            mma_f16(s[nt][mt], f, qf[nt][ks][0], qf[nt][ks][1]);
+                        } else {
+                            mma_bf16(s[nt][mt], f, qf[nt][ks][0], qf[nt][ks][1]);
+                            mma_bf16(s[nt][mt], f, ql[nt][EIGHT ? 0 : ks][0], ql[nt][EIGHT ? 0 : ks][1]);
+                        }
                     }
                 }
             }
             const float* sc = (const float*)(cur + L::S_AT);
             const int k0 = tile * TB;
-            // (key_lo: the first key of this CTA's range, beside each row's own)
-            const bool whole = k0 >= key_lo && k0 + TB - 1 <= key_hi &&
-                               k0 + TB - 1 <= min(pos[0], pos[1]) && k0 >= max(low[0], low[1]);
+            bool whole = k0 >= key_lo;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) whole = whole && k0 + TB - 1 <= min(pos[nt][0], pos[nt][1]) && k0 >= max(low[nt][0], low[nt][1]);
             const bool mask = !__all_sync(0xffffffffu, whole);
-            float rmax[2] = {-INFINITY, -INFINITY}, sv_most = 0.f;
-#pragma unroll
-            for (int n = 0; n < TB / 8; n++) {
-                float2 ksc = make_float2(1.f, 1.f), vsc = make_float2(0.f, 0.f);
-                if (KIND != OE_KV_BF16) {
-                    ksc = *(const float2*)(sc + n * 8 + tig * 2);
-                    vsc = *(const float2*)(sc + TB + n * 8 + tig * 2);
-                }
-                const int key = k0 + n * 8 + tig * 2;
-                if (KIND != OE_KV_BF16) {
-                    if (!mask || (key >= key_lo && key <= key_hi)) sv_most = fmaxf(sv_most, vsc.x);
-                    if (!mask || (key + 1 >= key_lo && key + 1 <= key_hi)) sv_most = fmaxf(sv_most, vsc.y);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = e >> 1, ke = key + (e & 1);
-                    float v = s[n][e] * (KIND == OE_KV_BF16 ? row_scale[i] : (e & 1 ? ksc.y : ksc.x) * row_scale[i]);
-                    if (mask) {
-                        const bool seen = ke >= key_lo && ke <= pos[i] && ke >= low[i];
-                        v = seen ? v : -INFINITY;
-                    }
-                    s[n][e] = v;
-                    rmax[i] = fmaxf(rmax[i], v);
-                }
-            }
-            float grown = 1.f, inv_ref = 1.f;
-            if (KIND != OE_KV_BF16) {
-                sv_most = fmaxf(sv_most, __shfl_xor_sync(0xffffffffu, sv_most, 1));
-                sv_most = fmaxf(sv_most, __shfl_xor_sync(0xffffffffu, sv_most, 2));
-                const float next = fmaxf(ref, kv8_above(sv_most));
-                inv_ref = kv8_inverse(next);
-                grown = ref * inv_ref;
+            float ksc[TB / 8], vsc[TB / 8], grown = 1.f;
+            if (EIGHT) {
+                float sv = sc[TB + lane];
+                if (mask && (k0 + lane < key_lo || k0 + lane > key_hi)) sv = 0.f;
+                const float next = fmaxf(ref, kv8_above(warp_most(sv))), inv = kv8_inverse(next);
+                grown = ref * inv;
                 ref = next;
+#pragma unroll
+                for (int o = 0; o < TB / 8; o++) { ksc[o] = sc[o * 8 + gid]; vsc[o] = sc[TB + o * 8 + gid] * inv; }
             }
-            float alpha[2], m_use[2];
+            float m_new[NT][2];
+            bool move = EIGHT && grown != 1.f;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 1));
-                rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 2));
-                const float m_new = fmaxf(m_run[i], rmax[i]);
-                m_use[i] = m_new == -INFINITY ? 0.f : m_new;
-                alpha[i] = exp2f(m_run[i] - m_use[i]);
-                m_use[i] -= HEADROOM;                       // l and O carry 2^8 beside the maximum's 2^-m
-                m_run[i] = m_new;
-            }
-            float rsum[2] = {0.f, 0.f};
+            for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-            for (int n = 0; n < TB / 8; n++) {
-                float2 vsc = make_float2(1.f, 1.f);
-                if (KIND != OE_KV_BF16) vsc = *(const float2*)(sc + TB + n * 8 + tig * 2);
+                for (int e = 0; e < 2; e++) {
+                    float most = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float p = exp2f(s[n][e] - m_use[e >> 1]);
-                    rsum[e >> 1] += p;
-                    float w = p;
-                    if (KIND != OE_KV_BF16) w = mask && s[n][e] == -INFINITY ? 0.f : p * ((e & 1 ? vsc.y : vsc.x) * inv_ref);
-                    s[n][e] = w;
+                    for (int o = 0; o < TB / 8; o++) {
+                        float& v = s[nt][o / 2][(o & 1) * 2 + e];
+                        if (EIGHT) v *= ksc[o];
+                        if (mask) {
+                            const int key = k0 + o * 8 + gid;
+                            v = key >= key_lo && key <= pos[nt][e] && key >= low[nt][e] ? v : -INFINITY;
+                        }
+                        most = fmaxf(most, v);
+                    }
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                    m_new[nt][e] = fmaxf(m_run[nt][e], most * row_scale[nt][e]);
+                    move = move || m_new[nt][e] > m_run[nt][e] + RESCALE_STEP;
                 }
             }
+            if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                l_run[i] = l_run[i] * alpha[i] + rsum[i];
-                alpha[i] *= grown;
+                for (int nt = 0; nt < NT; nt++) {
+                    float alpha[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        alpha[e] = fast_exp2(m_run[nt][e] - (m_new[nt][e] == -INFINITY ? 0.f : m_new[nt][e]));
+                        l_run[nt][e] *= alpha[e];
+                        alpha[e] *= grown;
+                        m_run[nt][e] = m_new[nt][e];
+                    }
+#pragma unroll
+                    for (int n = 0; n < HD / 16; n++) {
+                        oacc[nt][n][0] *= alpha[0]; oacc[nt][n][1] *= alpha[1];
+                        oacc[nt][n][2] *= alpha[0]; oacc[nt][n][3] *= alpha[1];
+                    }
+                }
             }
+            // weights, as the columns' fragments
+            uint32_t pf[NT][TB / 8], pl[NT][EIGHT ? 1 : TB / 8];
 #pragma unroll
-            for (int n = 0; n < HD / 8; n++) {
-                oacc[n][0] *= alpha[0]; oacc[n][1] *= alpha[0];
-                oacc[n][2] *= alpha[1]; oacc[n][3] *= alpha[1];
+            for (int nt = 0; nt < NT; nt++) {
+                const float n0 = (m_run[nt][0] == -INFINITY ? 0.f : -m_run[nt][0]) + HEADROOM;
+                const float n1 = (m_run[nt][1] == -INFINITY ? 0.f : -m_run[nt][1]) + HEADROOM;
+#pragma unroll
+                for (int o = 0; o < TB / 8; o++) {
+                    const float v0 = s[nt][o / 2][(o & 1) * 2], v1 = s[nt][o / 2][(o & 1) * 2 + 1];
+                    float p0 = fast_exp2(fmaf(v0, row_scale[nt][0], n0)), p1 = fast_exp2(fmaf(v1, row_scale[nt][1], n1));
+                    l_run[nt][0] += p0;
+                    l_run[nt][1] += p1;
+                    if (EIGHT) {
+                        p0 = mask && v0 == -INFINITY ? 0.f : p0 * vsc[o];
+                        p1 = mask && v1 == -INFINITY ? 0.f : p1 * vsc[o];
+                        pf[nt][o] = transposed(pack_f16(p0, p1));
+                    } else {
+                        const uint32_t h = pack_bf16(p0, p1);
+                        pf[nt][o] = transposed(h);
+                        pl[nt][EIGHT ? 0 : o] = transposed(rest_bf16(p0, p1, h));
+                    }
+                }
             }
 #pragma unroll
             for (int kk = 0; kk < TB / 16; kk++) {
-                uint32_t pa[4], pl[4];
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const float w0 = s[2 * kk + (x >> 1)][2 * (x & 1)], w1 = s[2 * kk + (x >> 1)][2 * (x & 1) + 1];
-                    pa[x] = KIND == OE_KV_BF16 ? pack_bf16(w0, w1) : pack_f16(w0, w1);
-                    if (KIND == OE_KV_BF16) pl[x] = rest_bf16(w0, w1, pa[x]);
-                }
-                const uint8_t* vr = vs_cur + (kk * 16 + tig * 2) * L::V_ROW + gid * 4 * L::ELEM;
+                const uint8_t* vr = cur + L::V_AT + (kk * 16 + tig * 2) * L::V_ROW + gid * 4 * L::ELEM;
 #pragma unroll
                 for (int c = 0; c < HD / 32; c++) {
-                    if (KIND == OE_KV_BF16) {
+                    uint32_t f[2][4];                       // dims c * 32 + gid * 4 + {0, 1} and + {2, 3}
+                    if (EIGHT) {
+                        const uint32_t w0 = kv8_word<KIND>(*(const uint32_t*)(vr + c * 32)), w1 = kv8_word<KIND>(*(const uint32_t*)(vr + L::V_ROW + c * 32));
+                        const uint32_t w2 = kv8_word<KIND>(*(const uint32_t*)(vr + 8 * L::V_ROW + c * 32)), w3 = kv8_word<KIND>(*(const uint32_t*)(vr + 9 * L::V_ROW + c * 32));
+                        const uint32_t x0 = kv8_prmt(w0, w1, 0x5140u), x1 = kv8_prmt(w0, w1, 0x7362u);
+                        const uint32_t y0 = kv8_prmt(w2, w3, 0x5140u), y1 = kv8_prmt(w2, w3, 0x7362u);
+                        f[0][0] = kv8_pair<KIND>(x0, 0); f[0][1] = kv8_pair<KIND>(x0, 2); f[0][2] = kv8_pair<KIND>(y0, 0); f[0][3] = kv8_pair<KIND>(y0, 2);
+                        f[1][0] = kv8_pair<KIND>(x1, 0); f[1][1] = kv8_pair<KIND>(x1, 2); f[1][2] = kv8_pair<KIND>(y1, 0); f[1][3] = kv8_pair<KIND>(y1, 2);
+                    } else {
                         uint2 w0 = *(const uint2*)(vr + c * 64), w1 = *(const uint2*)(vr + L::V_ROW + c * 64);
                         uint2 w2 = *(const uint2*)(vr + 8 * L::V_ROW + c * 64), w3 = *(const uint2*)(vr + 9 * L::V_ROW + c * 64);
                         if (mask) {            // a row behind the last token may hold anything, and 0 times that need not be 0
@@ -528,23 +570,22 @@ attn_kv8_kernel(const Args a) {
                             if (key + 8 < key_lo || key + 8 > key_hi) w2 = make_uint2(0u, 0u);
                             if (key + 9 < key_lo || key + 9 > key_hi) w3 = make_uint2(0u, 0u);
                         }
+                        f[0][0] = kv8_prmt(w0.x, w1.x, 0x5410u); f[0][1] = kv8_prmt(w0.x, w1.x, 0x7632u);
+                        f[0][2] = kv8_prmt(w2.x, w3.x, 0x5410u); f[0][3] = kv8_prmt(w2.x, w3.x, 0x7632u);
+                        f[1][0] = kv8_prmt(w0.y, w1.y, 0x5410u); f[1][1] = kv8_prmt(w0.y, w1.y, 0x7632u);
+                        f[1][2] = kv8_prmt(w2.y, w3.y, 0x5410u); f[1][3] = kv8_prmt(w2.y, w3.y, 0x7632u);
+                    }
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
-                            const uint32_t b0 = j < 2 ? kv8_prmt(w0.x, w1.x, sel) : kv8_prmt(w0.y, w1.y, sel);
-                            const uint32_t b1 = j < 2 ? kv8_prmt(w2.x, w3.x, sel) : kv8_prmt(w2.y, w3.y, sel);
-                            mma_bf16(oacc[c * 4 + j], pa, b0, b1);
-                            mma_bf16(oacc[c * 4 + j], pl, b0, b1);
+                    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            if (EIGHT) {
+                                mma_f16(oacc[nt][c * 2 + j], f[j], pf[nt][2 * kk], pf[nt][2 * kk + 1]);
+                            } else {
+                                mma_bf16(oacc[nt][c * 2 + j], f[j], pf[nt][2 * kk], pf[nt][2 * kk + 1]);
+                                mma_bf16(oacc[nt][c * 2 + j], f[j], pl[nt][EIGHT ? 0 : 2 * kk], pl[nt][EIGHT ? 0 : 2 * kk + 1]);
+                            }
                         }
-                    } else {
-                        const uint32_t w0 = kv8_word<KIND>(*(const uint32_t*)(vr + c * 32)), w1 = kv8_word<KIND>(*(const uint32_t*)(vr + L::V_ROW + c * 32));
-                        const uint32_t w2 = kv8_word<KIND>(*(const uint32_t*)(vr + 8 * L::V_ROW + c * 32)), w3 = kv8_word<KIND>(*(const uint32_t*)(vr + 9 * L::V_ROW + c * 32));
-                        const uint32_t x0 = kv8_prmt(w0, w1, 0x5140u), x1 = kv8_prmt(w0, w1, 0x7362u);
-                        const uint32_t y0 = kv8_prmt(w2, w3, 0x5140u), y1 = kv8_prmt(w2, w3, 0x7362u);
-                        mma_f16(oacc[c * 4 + 0], pa, kv8_pair<KIND>(x0, 0), kv8_pair<KIND>(y0, 0));
-                        mma_f16(oacc[c * 4 + 1], pa, kv8_pair<KIND>(x0, 2), kv8_pair<KIND>(y0, 2));
-                        mma_f16(oacc[c * 4 + 2], pa, kv8_pair<KIND>(x1, 0), kv8_pair<KIND>(y1, 0));
-                        mma_f16(oacc[c * 4 + 3], pa, kv8_pair<KIND>(x1, 2), kv8_pair<KIND>(y1, 2));
                     }
                 }
             }
@@ -558,90 +599,135 @@ attn_kv8_kernel(const Args a) {
         stage = stage + 1 == ST ? 0 : stage + 1;
     }
     cp_async_wait<0>();
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
-        l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
-    }
     // the warps' parts, added in warp order
     __syncthreads();                                        // every warp has left its ring
-    const int rows = min(16, n_rows - row0);
-    const float out_scale = KIND == OE_KV_BF16 ? 1.f : ref;
-    float* part = (float*)smem;                             // [NW][16][HD + 2]
-    float* cpart = part + (size_t)NW * 16 * (HD + 2);       // [16][HD + 2]: this CTA's sum
+    float* part = (float*)smem;                             // [NW][ROWS][OD]: O, m, l
+    float* cpart = part + (size_t)NW * ROWS * OD;           // [ROWS][OD]: this CTA's sum
+    float* wts = cpart + ROWS * OD;                         // [ROWS][MAX_JOINED + NW + 1]
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        float* p = part + ((size_t)warp * 16 + gid + i * 8) * (HD + 2);
+    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-        for (int c = 0; c < HD / 32; c++) {
+        for (int e = 0; e < 2; e++) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                p[c * 32 + tig * 8 + j] = oacc[c * 4 + j][2 * i] * out_scale;
-                p[c * 32 + tig * 8 + 4 + j] = oacc[c * 4 + j][2 * i + 1] * out_scale;
-            }
+            for (int d = 4; d < 32; d *= 2) l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], d);
+            const int r = nt * 8 + tig * 2 + e;
+            if (r >= rows) continue;
+            float* p = part + ((size_t)warp * ROWS + r) * OD;
+            const float f = EIGHT ? ref : 1.f;
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++)
+                *(float4*)(p + c * 32 + gid * 4) = make_float4(oacc[nt][c * 2][e] * f, oacc[nt][c * 2][2 + e] * f, oacc[nt][c * 2 + 1][e] * f, oacc[nt][c * 2 + 1][2 + e] * f);
+            if (gid == 0) *(float2*)(p + HD) = make_float2(m_run[nt][e], l_run[nt][e]);
         }
-        if (tig == 0) { p[HD] = m_run[i]; p[HD + 1] = l_run[i]; }
     }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < rows * HD; idx += NW * 32) {
-        const int r = idx / HD, d = idx % HD;
-        float m = -INFINITY, l = 0.f, o = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; w++) m = fmaxf(m, part[((size_t)w * 16 + r) * (HD + 2) + HD]);
+    // weights of n parts, whose (m, l) lane q < n of this warp has, once or in rounds: into w[0..n), the joined m and l behind it
+    constexpr int WT = MAX_JOINED + NW + 1;
+    for (int r = warp; r < rows; r += NW) {
+        const float2 ml = lane < NW ? *(const float2*)(part + ((size_t)lane * ROWS + r) * OD + HD) : make_float2(-INFINITY, 0.f);
+        const float m = warp_max(ml.x), mu = m == -INFINITY ? 0.f : m;
+        const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - mu);
+        const float l = warp_sum(w == 0.f && ml.y == 0.f ? 0.f : ml.y * w);
+        if (lane < NW) wts[r * WT + lane] = w;
+        if (lane == 0) *(float2*)(cpart + r * OD + HD) = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += NW * 32) {
+        const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float* p = part + ((size_t)w * 16 + r) * (HD + 2);
-            if (p[HD] == -INFINITY && p[HD + 1] == 0.f) continue;          // no key of this row
-            const float e = exp2f(p[HD] - (m == -INFINITY ? 0.f : m));
-            l += p[HD + 1] * e;
-            o += p[d] * e;
+            const float e = wts[r * WT + w];
+            const float4 p = *(const float4*)(part + ((size_t)w * ROWS + r) * OD + d);
+            o.x = fmaf(p.x, e, o.x); o.y = fmaf(p.y, e, o.y); o.z = fmaf(p.z, e, o.z); o.w = fmaf(p.w, e, o.w);
         }
-        cpart[r * (HD + 2) + d] = o;
-        if (d == 0) { cpart[r * (HD + 2) + HD] = m; cpart[r * (HD + 2) + HD + 1] = l; }
+        *(float4*)(cpart + r * OD + d) = o;
     }
     if (CR > 1) cluster_sync_all();
     else __syncthreads();
+    // this CTA's share of the rows' results: the cluster's sums in rank order, then the prefix's parts
     const int n_pre = common > 0 ? a.splits : 0;
-    for (int idx = threadIdx.x + rank * NW * 32; idx < rows * HD; idx += NW * 32 * CR) {
-        const int r = idx / HD, d = idx % HD;
-        float m = -INFINITY, l = 0.f, o = 0.f;
-        for (int q = 0; q < CR; q++) m = fmaxf(m, CR > 1 ? ld_peer_f32(cpart + r * (HD + 2) + HD, q) : cpart[r * (HD + 2) + HD]);
+    for (int r = warp; r < rows; r += NW) {
         const int h = kvh * G + (row0 + r) % G;
-        const float* pre_o = a.part_o + ((long long)b * a.H + h) * a.splits * HD;
         const float2* pre_ml = (const float2*)a.part_ml + ((long long)b * a.H + h) * a.splits;
-        for (int q = 0; q < n_pre; q++) m = fmaxf(m, pre_ml[q].x);
+        float2 ml[MAX_JOINED / 32];
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int j = 0; j < MAX_JOINED / 32; j++) {
+            const int q = j * 32 + lane;
+            ml[j] = make_float2(-INFINITY, 0.f);
+            if (q < CR) ml[j] = CR > 1 ? ld_peer2(cpart + r * OD + HD, q) : *(const float2*)(cpart + r * OD + HD);
+            else if (q < CR + n_pre) ml[j] = pre_ml[q - CR];
+            m = fmaxf(m, ml[j].x);
+        }
+        m = warp_max(m);
         const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < MAX_JOINED / 32; j++) {
+            const int q = j * 32 + lane;
+            const bool none = ml[j].x == -INFINITY && ml[j].y == 0.f;           // no key of this row: its O is not there
+            const float w = none ? 0.f : exp2f(ml[j].x - mu);
+            if (!none) l += ml[j].y * w;
+            if (q < CR + n_pre) wts[r * WT + q] = none ? -1.f : w;
+        }
+        l = warp_sum(l);
+        if (lane == 0) wts[r * WT + MAX_JOINED] = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x + rank * NW * 32; idx < rows * (HD / 4); idx += NW * 32 * CR) {
+        const int r = idx / (HD / 4), d = idx % (HD / 4) * 4, h = kvh * G + (row0 + r) % G;
+        const float* w = wts + r * WT;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int q = 0; q < CR; q++) {
-            const float pm = CR > 1 ? ld_peer_f32(cpart + r * (HD + 2) + HD, q) : cpart[r * (HD + 2) + HD];
-            const float pl = CR > 1 ? ld_peer_f32(cpart + r * (HD + 2) + HD + 1, q) : cpart[r * (HD + 2) + HD + 1];
-            if (pm == -INFINITY && pl == 0.f) continue;
-            const float e = exp2f(pm - mu);
-            l += pl * e;
-            o += (CR > 1 ? ld_peer_f32(cpart + r * (HD + 2) + d, q) : cpart[r * (HD + 2) + d]) * e;
+            if (w[q] < 0.f) continue;
+            const float4 p = CR > 1 ? ld_peer4(cpart + r * OD + d, q) : *(const float4*)(cpart + r * OD + d);
+            o.x = fmaf(p.x, w[q], o.x); o.y = fmaf(p.y, w[q], o.y); o.z = fmaf(p.z, w[q], o.z); o.w = fmaf(p.w, w[q], o.w);
         }
+        const float* pre = a.part_o + (((long long)b * a.H + h) * a.splits) * HD + d;
+#pragma unroll 8
         for (int q = 0; q < n_pre; q++) {
-            const float2 ml = pre_ml[q];
-            if (ml.x == -INFINITY && ml.y == 0.f) continue;
-            const float e = exp2f(ml.x - mu);
-            l += ml.y * e;
-            o += pre_o[q * HD + d] * e;
+            const float e = w[CR + q];
+            if (e < 0.f) continue;
+            const float4 p = *(const float4*)(pre + q * HD);
+            o.x = fmaf(p.x, e, o.x); o.y = fmaf(p.y, e, o.y); o.z = fmaf(p.z, e, o.z); o.w = fmaf(p.w, e, o.w);
         }
-        a.out[(packed0 + (row0 + r) / G) * (long long)(a.H * HD) + (long long)h * HD + d] = __float2bfloat16_rn(l > 0.f ? o / l : l == 0.f ? 0.f : l);
+        const float inv = w[MAX_JOINED];
+        *(uint2*)(a.out + (packed0 + (row0 + r) / G) * (long long)(a.H * HD) + (long long)h * HD + d) =
+            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
     if (CR > 1) cluster_sync_all();                         // nobody leaves while its shared memory is read
 }
 
-template <int KIND>
-int launch(const Args& a, int row_tiles, int n_seqs, cudaStream_t st) {
-    constexpr int NW = KIND == OE_KV_BF16 ? 3 : 4, ST = KIND == OE_KV_BF16 ? 2 : 3;
+template <int KIND, int NT, int NW, int ST>
+int launch(const Args& a, long long rows, int n_seqs, cudaStream_t st) {
+    auto kernel = attn_kv8_kernel<KIND, NT, NW, ST>;
     constexpr size_t smem = (size_t)NW * ST * Tile<KIND>::BYTES;
-    const long long x = (long long)row_tiles * a.cluster;
+    const long long x = (rows + 8 * NT - 1) / (8 * NT) * a.cluster;
     if (x > 0x7fffffffLL || a.KVH > 65535 || n_seqs > 65535) return OE_ERR_UNSUPPORTED;
-    cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<KIND, NW, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
     const dim3 grid((unsigned)x, a.KVH, n_seqs);
-    if (a.cluster > 1) return oe_launch_cluster(attn_kv8_kernel<KIND, NW, ST>, (unsigned)a.cluster, grid, dim3(NW * 32), smem, st, a);
-    return oe_launch(attn_kv8_kernel<KIND, NW, ST>, grid, dim3(NW * 32), smem, st, a);
+    if (a.cluster > 8) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return (int)e;
+    }
+    if (a.cluster > 1) return oe_launch_cluster(kernel, (unsigned)a.cluster, grid, dim3(NW * 32), smem, st, a);
+    return oe_launch(kernel, grid, dim3(NW * 32), smem, st, a);
+}
+// warps: 12 (a CTA has an SM to itself) or 4 (three an SM).
+template <int KIND, int NT>
+int launch_form(int warps, const Args& a, long long rows, int n_seqs, cudaStream_t st) {
+    if (warps == 12) return launch<KIND, NT, 12, 2>(a, rows, n_seqs, st);
+    if (warps == 4) return launch<KIND, NT, 4, 2>(a, rows, n_seqs, st);
+    return OE_ERR_UNSUPPORTED;
+}
+template <int KIND>
+int launch_rows(int warps, const Args& a, long long rows, int n_seqs, cudaStream_t st) {
+    if constexpr (KIND == OE_KV_BF16)
+        return rows <= 8 ? launch<KIND, 1, 3, 2>(a, rows, n_seqs, st) : launch<KIND, 2, 3, 2>(a, rows, n_seqs, st);
+    else
+        return rows <= 8 ? launch_form<KIND, 1>(warps, a, rows, n_seqs, st) : launch_form<KIND, 2>(warps, a, rows, n_seqs, st);
 }
 
 }  // namespace
@@ -670,12 +756,13 @@ int oe_kv8_write(int kind, const bf16* qkv, long long stride, const float* cos_t
 // oe_attn_rows_prefix left are added.
 int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, void* cache,
                 float* scales, int write, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
-                const int* seq_qlen, int n_seqs, int max_qlen, int H, int KVH, int window, float scale, int cluster,
+                const int* seq_qlen, int n_seqs, int max_qlen, int H, int KVH, int window, float scale, int warps, int cluster,
                 const int* seq_pages, int splits, const float* part_o, const float* part_ml, int ahead, cudaStream_t st) {
     if (n_seqs <= 0 || max_qlen <= 0) return 0;
-    if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15)) return OE_ERR_UNSUPPORTED;
-    if (cluster < 1 || cluster > 8 || (write && max_qlen != 1)) return OE_ERR_UNSUPPORTED;
-    if (seq_pages != nullptr && (window != 0 || max_qlen != 1 || splits < 1 || part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
+    if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15) ||
+        ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15) || ((uintptr_t)out & 15)) return OE_ERR_UNSUPPORTED;
+    if (cluster < 1 || cluster > 16 || (cluster & (cluster - 1)) || (write && max_qlen != 1)) return OE_ERR_UNSUPPORTED;
+    if (seq_pages != nullptr && (window != 0 || max_qlen != 1 || splits < 1 || splits + cluster > MAX_JOINED || part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
     Args a = {};
     a.out = out; a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab;
     a.cache = cache; a.scales = scales;
@@ -683,11 +770,10 @@ int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const fl
     a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start; a.seq_qlen = seq_qlen;
     a.H = H; a.KVH = KVH; a.window = window; a.scale_log2 = scale * LOG2E; a.cluster = cluster;
     a.seq_pages = seq_pages; a.splits = splits; a.part_o = part_o; a.part_ml = part_ml; a.ahead = ahead;
-    const long long rows = (long long)max_qlen * (H / KVH), tiles = (rows + 15) / 16;
-    if (tiles > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
-    if (kind == OE_KV_BF16) return launch<OE_KV_BF16>(a, (int)tiles, n_seqs, st);
-    if (kind == OE_KV_INT8) return launch<OE_KV_INT8>(a, (int)tiles, n_seqs, st);
-    if (kind == OE_KV_E4M3) return launch<OE_KV_E4M3>(a, (int)tiles, n_seqs, st);
+    const long long rows = (long long)max_qlen * (H / KVH);
+    if (kind == OE_KV_BF16) return launch_rows<OE_KV_BF16>(warps, a, rows, n_seqs, st);
+    if (kind == OE_KV_INT8) return launch_rows<OE_KV_INT8>(warps, a, rows, n_seqs, st);
+    if (kind == OE_KV_E4M3) return launch_rows<OE_KV_E4M3>(warps, a, rows, n_seqs, st);
     return OE_ERR_UNSUPPORTED;
 }
 

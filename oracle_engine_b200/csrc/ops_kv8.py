@@ -21,6 +21,7 @@ from . import ops
 from .ops import PAGE, KernelError
 
 HEAD_DIMS = (64, 128)
+MAX_SPLITS = 148     # of a prefix; with a cluster's CTAs at most MAX_JOINED of attention_kv8.cu
 FEW_ROWS = 16        # rows of a tile of attention_kv8.cu
 TILE_ROWS = 128      # rows (a token's or member's heads of one KV head) of a tile of attention_rows.cu; must equal its BM
 CODE_TYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
@@ -36,7 +37,7 @@ def _lib(head_dim: int):
         lib = _build.load("attention_kv8", {"OE_HD": head_dim})
         P, I, F, L = c_void_p, c_int, c_float, c_longlong
         lib.oe_kv8_write.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, I, P]
-        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, P, I, P, P, I, P]
+        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, I, P, I, P, P, I, P]
         lib.oe_kv8_write.restype = lib.oe_attn_kv8.restype = c_int
         _libs[head_dim] = lib
     return lib
@@ -145,26 +146,26 @@ def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv
         tables.data_ptr(), tables.shape[1], tok_seq.data_ptr(), tok_pos.data_ptr(), T, n_heads, n_kv_heads, ops._stream()), what)
 
 
-def decode_cluster(n_seqs: int, n_kv_heads: int, context_class: int, sm_count: int | None = None) -> int:
-    """How many CTAs (a thread-block cluster) share the keys of one (sequence, KV head) of a step of single tokens."""
-    if context_class < 1:
-        return 1
-    budget = sm_count or ops.sm_count()
-    for cr in (8, 4, 2):
-        if n_seqs * n_kv_heads * cr <= budget:
-            return cr
-    return 1
+def decode_form(n_seqs: int, n_kv_heads: int, context_class: int, sm_count: int | None = None) -> tuple:
+    """(warps of a CTA, CTAs (a thread-block cluster) that share the keys of one (sequence, KV head)) of a step of few rows."""
+    sms = sm_count or ops.sm_count()
+    pairs = n_seqs * n_kv_heads
+    for cr in (16, 8, 4, 2):
+        if context_class >= (1 if cr <= 4 else 2) and pairs * cr <= sms:
+            return 12, cr
+    return (12 if pairs <= sms else 4), 1
 
 
 def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float,
-                  has_kv: bool = True, ahead: bool = False, cluster: int | None = None, form: tuple | None = None) -> None:
+                  has_kv: bool = True, ahead: bool = False, form: tuple | None = None) -> None:
     """Rotation, cache write (has_kv) and attention of the step's tokens over the 8-bit cache: out[t] is the attention of token t's
     query heads over its sequence's keys up to its own position (window 0: all of them, n > 0: the last n, -n: those of the
     chunk of n positions it lies in), as the cache keeps them, the step's own among them.
 
     qkv bfloat16 [T, (H + 2 KVH) hd] (or [T, H hd] when has_kv is false: the rows are in the cache) before rotation, left as it
     is; out bfloat16 [T, H hd]; ctx: the step (StepContext: cu_q, seq_start, seq_qlen, tok_seq, tok_pos, n_seqs, max_qlen,
-    all_decode).  A step of one token a sequence is one launch, any other a write and an attention."""
+    all_decode).  A step of one token a sequence is one launch, any other a write and an attention.  form: the kernel's
+    form (decode_form where a sequence has few rows, prompt_form else); None: by those rules."""
     what = "attention_kv8"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
@@ -179,17 +180,14 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
         kv8_write(qkv, cos, sin, cache, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
     few = max(1, ctx.max_qlen) * (n_heads // n_kv_heads) <= FEW_ROWS
     if single or few:
-        if cluster is None:
-            cluster = decode_cluster(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0))
+        warps, cluster = form or decode_form(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0))
         ops._check(_lib(head_dim).oe_attn_kv8(
             kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(),
             int(has_kv and single), codes.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
             ctx.seq_qlen.data_ptr(), ctx.n_seqs, 1 if single else max(1, ctx.max_qlen), n_heads, n_kv_heads, int(window), float(scale),
-            int(cluster), None, 0, None, None, int(ahead), ops._stream()), what, {"cluster": int(cluster)})
+            warps, cluster, None, 0, None, None, int(ahead), ops._stream()), what, {"warps": warps, "cluster": cluster})
         return
-    if form is None:
-        form = prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
-    mt, splits = form
+    mt, splits = form or prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
     part = _parts(T * n_heads, splits, head_dim, out.device) if splits > 1 else None
     ops._check(_rows_lib(head_dim).oe_attn_rows(
         kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(), codes.shape[0],
@@ -229,7 +227,7 @@ def prefix_form(n_members: int, n_groups: int, group: int, n_kv_heads: int, max_
     tiles = -(-n_members // (TILE_ROWS // group))
     mt = 2 if tiles > 1 else 1
     ctas = (-(-tiles // mt) + n_groups - 1) * n_kv_heads
-    return mt, max(1, min(max_pages, sms // ctas))
+    return mt, max(1, min(max_pages, sms // ctas, MAX_SPLITS))
 
 
 def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
@@ -269,5 +267,5 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
             prefix.n_members, mt, splits, *parts, int(ahead), ops._stream()), "attention_shared_prefix", {"tiles": mt, "splits": splits})
     ops._check(_lib(head_dim).oe_attn_kv8(
         kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), int(has_kv),
-        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 1, prefix.seq_pages.data_ptr(), splits,
+        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 4, 1, prefix.seq_pages.data_ptr(), splits,
         *parts, int(ahead), ops._stream()), what)

@@ -79,13 +79,13 @@ def test_single_tokens(H, KVH, hd, dtype, window):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("cluster", [1, 2, 4, 8])
-def test_single_tokens_of_long_sequences(dtype, cluster):
+@pytest.mark.parametrize("form", [(4, 1), (12, 1), (4, 2), (12, 4), (4, 8), (12, 16)])
+def test_single_tokens_of_long_sequences(dtype, form):
     s = Step([0, 3000, 1279, 2111], [1] * 4, 6, 2, 128, dtype, seed=6, peaked=3.0)
     want, tol, cache = s.truth()
     for ahead in (False, True):
         torch.cuda.synchronize()
-        close(s.out(cluster=cluster, ahead=ahead), want, tol)
+        close(s.out(form=form, ahead=ahead), want, tol)
     s.check_cache(cache)
 
 
@@ -178,7 +178,7 @@ def test_strided_rows_no_rotation_another_stream_and_a_graph():
 
 def test_the_same_bits_every_time():
     s = Step([3000, 17, 900], [1, 1, 1], 24, 8, 128, torch.float8_e4m3fn, seed=14)
-    got = [s.out(cluster=4) for _ in range(4)]
+    got = [s.out(form=(12, 4)) for _ in range(4)]
     assert all(torch.equal(got[0], o) for o in got)
 
 
@@ -223,8 +223,8 @@ def test_refusals_on_the_device():
         with pytest.raises(KernelError):
             s.out()
     s = Step([10], [1], 4, 2, 64, torch.int8, seed=18)
-    for cluster in (0, 9, 16):
+    for form in ((4, 0), (4, 3), (12, 32), (5, 1)):
         with pytest.raises(KernelError):
-            s.out(cluster=cluster)
+            s.out(form=form)
     with pytest.raises(KernelError):
         ops_kv8.kv8_write(s.qkv, s.cos, s.sin, s.cache, s.tables, s.ctx.tok_seq[:0], s.ctx.tok_pos, 4, 2, 64)

@@ -47,35 +47,35 @@ kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ co
                  const int* __restrict__ tok_seq, const int* __restrict__ tok_pos, int n_tokens, int H, int KVH) {
     constexpr int LANES = HD / 16;
     pdl_wait();
-    const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long r = item / LANES;                        // (token, K or V, KV head)
+    const unsigned item = blockIdx.x * 256u + threadIdx.x, r = item / LANES;       // a row: (token, K or V, KV head)
     const int i = (int)(item % LANES) * 8;
-    const long long per_token = 2 * KVH;
-    const long long t = r / per_token;
-    const int which = (int)(r % per_token) / KVH, kvh = (int)(r % KVH);
-    const bool here = t < n_tokens;
-    const int b = here ? tok_seq[t] : -1;
+    const unsigned per_token = 2u * KVH, t = r / per_token, which_head = r - t * per_token;
+    const int which = which_head >= (unsigned)KVH, kvh = (int)which_head - (which ? KVH : 0);
+    const int b = t < (unsigned)n_tokens ? tok_seq[t] : -1;
     const int pos = b >= 0 ? tok_pos[t] : 0;
     const int page = b >= 0 && pos / OE_PAGE < max_pages ? tables[(long long)b * max_pages + pos / OE_PAGE] : -1;
     const bool ok = page >= 0 && page < n_pages;
     uint32_t lo[4] = {0, 0, 0, 0}, hi[4] = {0, 0, 0, 0};
     if (ok) {
-        const bf16* row = qkv + t * stride + (long long)(H + which * KVH + kvh) * HD;
+        const bf16* row = qkv + (long long)t * stride + (long long)(H + which * KVH + kvh) * HD;
         const uint4 a = *(const uint4*)(row + i), c = *(const uint4*)(row + i + HD / 2);
         lo[0] = a.x; lo[1] = a.y; lo[2] = a.z; lo[3] = a.w;
         hi[0] = c.x; hi[1] = c.y; hi[2] = c.z; hi[3] = c.w;
         if (which == 0 && cos_tab != nullptr) {
-            const float* cs = cos_tab + (long long)pos * (HD / 2) + i;
-            const float* sn = sin_tab + (long long)pos * (HD / 2) + i;
+            float cs[8], sn[8];
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                *(float4*)&cs[j] = *(const float4*)(cos_tab + (long long)pos * (HD / 2) + i + j);
+                *(float4*)&sn[j] = *(const float4*)(sin_tab + (long long)pos * (HD / 2) + i + j);
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 uint32_t nl = 0, nh = 0;
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const float x0 = kv8_from_bits((lo[j] >> (16 * e)) & 0xffffu), x1 = kv8_from_bits((hi[j] >> (16 * e)) & 0xffffu);
-                    const float c1 = cs[2 * j + e], s1 = sn[2 * j + e];
-                    nl |= kv8_turned_bits(x0, c1, x1, s1) << (16 * e);
-                    nh |= kv8_turned_bits(x0, s1, -x1, c1) << (16 * e);
+                    nl |= kv8_turned_bits(x0, cs[2 * j + e], x1, sn[2 * j + e]) << (16 * e);
+                    nh |= kv8_turned_bits(x0, sn[2 * j + e], -x1, cs[2 * j + e]) << (16 * e);
                 }
                 lo[j] = nl;
                 hi[j] = nh;
@@ -92,17 +92,9 @@ kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ co
     for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (ok) {
         const Kv8Row q = kv8_row<KIND>(m);
-        uint32_t w[4];
-    #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            w[j / 2] = kv8_code<KIND>(q, lo[j] & 0xffffu) | kv8_code<KIND>(q, lo[j] >> 16) << 8 |
-                       kv8_code<KIND>(q, lo[j + 1] & 0xffffu) << 16 | kv8_code<KIND>(q, lo[j + 1] >> 16) << 24;
-            w[2 + j / 2] = kv8_code<KIND>(q, hi[j] & 0xffffu) | kv8_code<KIND>(q, hi[j] >> 16) << 8 |
-                           kv8_code<KIND>(q, hi[j + 1] & 0xffffu) << 16 | kv8_code<KIND>(q, hi[j + 1] >> 16) << 24;
-    }
         const long long at = (((long long)page * 2 + which) * KVH + kvh) * OE_PAGE + pos % OE_PAGE;
-        *(uint2*)(codes + at * HD + i) = make_uint2(w[0], w[1]);
-        *(uint2*)(codes + at * HD + i + HD / 2) = make_uint2(w[2], w[3]);
+        *(uint2*)(codes + at * HD + i) = make_uint2(kv8_codes4<KIND>(q, lo[0], lo[1]), kv8_codes4<KIND>(q, lo[2], lo[3]));
+        *(uint2*)(codes + at * HD + i + HD / 2) = make_uint2(kv8_codes4<KIND>(q, hi[0], hi[1]), kv8_codes4<KIND>(q, hi[2], hi[3]));
         if (i == 0) scales[at] = q.scale;
     }
     // the kernel behind this one may ask for these rows before it waits
@@ -741,7 +733,7 @@ int oe_kv8_write(int kind, const bf16* qkv, long long stride, const float* cos_t
     if (n_tokens <= 0) return 0;
     if (stride % 8 || ((uintptr_t)qkv & 15) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15)) return OE_ERR_UNSUPPORTED;
     const long long blocks = ((long long)n_tokens * 2 * KVH * (HD / 16) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
+    if (blocks > 0x00ffffffLL || ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15)) return OE_ERR_UNSUPPORTED;   // (lanes are counted in 32 bits)
     if (kind == OE_KV_INT8)
         return oe_launch(kv8_write_kernel<OE_KV_INT8>, dim3((unsigned)blocks), dim3(256), 0, st, qkv, stride, cos_tab, sin_tab,
                          (uint8_t*)codes, scales, n_pages, tables, max_pages, tok_seq, tok_pos, n_tokens, H, KVH);

@@ -38,7 +38,7 @@ constexpr int BM = 128, BN = OE_PAGE, SUB = HD / 64;
 constexpr int Q_BYTES = BM * HD * 2;             // SUB sub-tiles of [128][64] 16-bit values
 constexpr int T_BYTES = BN * HD * 2;             // K or V of a page, SUB sub-tiles of [64][64] 16-bit values
 constexpr int RAW = BN * HD;                     // codes of a page's K or V
-constexpr int STAGES = 2, SC_SLOTS = 4;
+constexpr int STAGES = 2, RAW_STAGES = 4, SC_SLOTS = 6;
 constexpr float RESCALE_STEP = 7.f, LOG2E = 1.4426950408889634f;
 constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
 
@@ -51,7 +51,7 @@ struct Scales {
 };
 struct Ctl {
     Scales sc[SC_SLOTS];
-    uint64_t q_full, raw_full[STAGES], raw_empty[STAGES], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
+    uint64_t q_full, raw_full[RAW_STAGES], raw_empty[RAW_STAGES], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
     uint64_t sc_full[SC_SLOTS], sc_ready[SC_SLOTS], sc_empty[SC_SLOTS];
     uint64_t s_full[2][2], p_ready[2][2], pv_done[2], o_done[2];
     uint32_t tmem_base;
@@ -63,7 +63,7 @@ struct Shape {
     static constexpr bool EIGHT = KIND != OE_KV_BF16;
     static constexpr int Q_ALL = MT * Q_BYTES * (EIGHT ? 1 : 2);
     static constexpr int K_AT = Q_ALL, V_AT = K_AT + STAGES * T_BYTES, RAW_AT = V_AT + STAGES * T_BYTES;
-    static constexpr int CTL_AT = RAW_AT + (EIGHT ? STAGES * 2 * RAW : 0);
+    static constexpr int CTL_AT = RAW_AT + (EIGHT ? RAW_STAGES * 2 * RAW : 0);
     static constexpr int BYTES = CTL_AT + (int)sizeof(Ctl);
     static constexpr int CONVERT = EIGHT ? 4 : 0;                      // warps
     static constexpr int FIRST = 4 + CONVERT;                          // the first softmax warp
@@ -217,6 +217,22 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two float32 at once.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(uint64_t*)&d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(uint64_t*)&d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*(uint64_t*)&d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b), "l"(*(uint64_t*)&c));
+    return d;
+}
 template <bool EIGHT>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     if (EIGHT) {
@@ -228,30 +244,6 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t rest_bf16(float lo, float hi, uint32_t h) {
     return pack16<false>(lo - __uint_as_float(h << 16), hi - __uint_as_float(h & 0xffff0000u));
-}
-
-// Eight consecutive dimensions d..d+7 of a row of queries and the eight they are turned with, d + HD/2 ..., as float32.
-__device__ __forceinline__ void turned8(const bf16* row, const float* cs, const float* sn, int d, float (&lo)[8], float (&hi)[8]) {
-    const uint4 a = *(const uint4*)(row + d), b = *(const uint4*)(row + d + HD / 2);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        lo[2 * j] = kv8_from_bits(aw[j] & 0xffffu); lo[2 * j + 1] = kv8_from_bits(aw[j] >> 16);
-        hi[2 * j] = kv8_from_bits(bw[j] & 0xffffu); hi[2 * j + 1] = kv8_from_bits(bw[j] >> 16);
-    }
-    if (cs != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-            const float4 c = *(const float4*)(cs + d + j), s = *(const float4*)(sn + d + j);
-            const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float x = lo[j + e], y = hi[j + e];
-                lo[j + e] = x * cc[e] - y * ss[e];
-                hi[j + e] = x * ss[e] + y * cc[e];
-            }
-        }
-    }
 }
 
 // Warps 4-7: a page's codes to the swizzled 16-bit tile.  A lane takes 16 codes at a time; the lanes of the second sub-tile store their
@@ -272,6 +264,44 @@ __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* tile, 
         *(uint4*)(row + (((c + odd) ^ x) << 4)) = odd ? o[1] : o[0];
         *(uint4*)(row + (((c + 1 - odd) ^ x) << 4)) = odd ? o[0] : o[1];
     }
+}
+
+// A row's weights of a page: P into tensor memory, their sum.  GONE: some scores are -infinity, whose weights are zero whatever the
+// values' scales are.
+template <bool EIGHT, bool GONE>
+__device__ __forceinline__ float page_weights(const float (&s)[BN], const float* vscale, float scale, float neg_m, uint32_t p_addr) {
+    const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(neg_m, neg_m);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int k0 = 0; k0 < BN; k0 += 16) {
+        uint32_t w[8], rest[8];
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+            float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
+            if (EIGHT) f = *(const float4*)(vscale + k0 + k);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float2 x = make_float2(s[k0 + k + e], s[k0 + k + e + 1]);
+                float2 p = fma2(x, scale2, neg2);
+                p.x = fast_exp2(p.x);
+                p.y = fast_exp2(p.y);
+                sum[e / 2] = add2(sum[e / 2], p);
+                if (EIGHT) {
+                    p = mul2(p, e ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
+                    if (GONE) {
+                        p.x = x.x == -INFINITY ? 0.f : p.x;
+                        p.y = x.y == -INFINITY ? 0.f : p.y;
+                    }
+                }
+                w[(k + e) / 2] = pack16<EIGHT>(p.x, p.y);
+                if (!EIGHT) rest[(k + e) / 2] = rest_bf16(p.x, p.y, w[(k + e) / 2]);
+            }
+        }
+        tmem_st8(p_addr + (uint32_t)(k0 / 2), w);
+        if (!EIGHT) tmem_st8(p_addr + (uint32_t)(BN / 2 + k0 / 2), rest);
+    }
+    const float2 all = add2(sum[0], sum[1]);
+    return all.x + all.y;
 }
 
 // PREFIX false: the tiles are those of one sequence's tokens, keys up to each row's position.  PREFIX true: the rows are those of all
@@ -342,8 +372,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     const int* trow = a.tables + (size_t)b * a.max_pages;
     if (threadIdx.x == 0) {
         mbar_init(&ctl->q_full, MT * 4);
+        for (int s = 0; s < RAW_STAGES; s++) { mbar_init(&ctl->raw_full[s], 1); mbar_init(&ctl->raw_empty[s], 4); }
         for (int s = 0; s < STAGES; s++) {
-            mbar_init(&ctl->raw_full[s], 1); mbar_init(&ctl->raw_empty[s], 4);
             mbar_init(&ctl->k_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->k_empty[s], 1);
             mbar_init(&ctl->v_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->v_empty[s], 1);
         }
@@ -381,8 +411,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
             };
             if (EIGHT) {
                 for (int i = 0; i < any && ok; i++) {
-                    const int s = i % STAGES, c = i % SC_SLOTS;
-                    ok = mbar_wait(&ctl->raw_empty[s], ((uint32_t)(i / STAGES) & 1u) ^ 1u, ctl, 1);
+                    const int s = i % RAW_STAGES, c = i % SC_SLOTS;
+                    ok = mbar_wait(&ctl->raw_empty[s], ((uint32_t)(i / RAW_STAGES) & 1u) ^ 1u, ctl, 1);
                     if (ok) ok = mbar_wait(&ctl->sc_empty[c], ((uint32_t)(i / SC_SLOTS) & 1u) ^ 1u, ctl, 2);
                     if (!ok) break;
                     fence_async();                         // the slot's scales were written by threads before
@@ -512,19 +542,19 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         // ---------------- codes to 16-bit tiles ----------------
         const int t = threadIdx.x - 128;
         for (int i = 0; i < any; i++) {
-            const int s = i % STAGES;
+            const int s = i % STAGES, rs = i % RAW_STAGES;
             const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
-            if (!warp_wait(&ctl->raw_full[s], ph, ctl, 12)) break;
+            if (!warp_wait(&ctl->raw_full[rs], (uint32_t)(i / RAW_STAGES) & 1u, ctl, 12)) break;
             if (!warp_wait(&ctl->k_empty[s], ph ^ 1u, ctl, 13)) break;
-            convert_tile<KIND>(raw_s + s * 2 * RAW, k_s + s * T_BYTES, t);
+            convert_tile<KIND>(raw_s + rs * 2 * RAW, k_s + s * T_BYTES, t);
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl->k_full[s]);
             if (!warp_wait(&ctl->v_empty[s], ph ^ 1u, ctl, 14)) break;
-            convert_tile<KIND>(raw_s + s * 2 * RAW + RAW, v_s + s * T_BYTES, t);
+            convert_tile<KIND>(raw_s + rs * 2 * RAW + RAW, v_s + s * T_BYTES, t);
             fence_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&ctl->v_full[s]); mbar_arrive(&ctl->raw_empty[s]); }
+            if (lane == 0) { mbar_arrive(&ctl->v_full[s]); mbar_arrive(&ctl->raw_empty[rs]); }
         }
     } else if (warp >= Z::FIRST) {
         // ---------------- queries, softmax, output: one row a thread ----------------
@@ -552,53 +582,77 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         }
         float scale = a.scale_log2;
         const int nb = n_blocks[tile];
-        {
-            uint8_t* qt = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES + r * 128;
-            const bf16* src = a.q + row * a.q_stride + (long long)head * HD;
-            const float* cs = a.cos_tab != nullptr ? a.cos_tab + (long long)pos * (HD / 2) : nullptr;
-            const float* sn = a.cos_tab != nullptr ? a.sin_tab + (long long)pos * (HD / 2) : nullptr;
-            float lo[8], hi[8], down = 1.f;
-            if (EIGHT && valid && nb > 0) {
-                float most = 0.f;
-#pragma unroll 4
-                for (int d = 0; d < HD / 2; d += 8) {
-                    turned8(src, cs, sn, d, lo, hi);
+        // The warp's 32 rows of queries, turned: HD / 16 lanes have a row, 8 dimensions of its lower half and the 8 they are turned
+        // with each, so that a row's pieces are loaded together.
+        if (nb > 0) {
+            constexpr int PER = HD / 16, AT_ONCE = 32 / PER;
+            const int d = lane % PER * 8;
+            uint8_t* qt = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES;
+#pragma unroll 2
+            for (int k = 0; k < PER; k++) {
+                const int rl = k * AT_ONCE + lane / PER, rr = quarter * 32 + rl;        // this step's row
+                const bool there = __shfl_sync(0xffffffffu, (int)valid, rl) != 0;
+                const long long at = __shfl_sync(0xffffffffu, row, rl);
+                const int h = __shfl_sync(0xffffffffu, head, rl), ps = __shfl_sync(0xffffffffu, pos, rl);
+                float x[2][8];
+                if (there) {
+                    const bf16* src = a.q + at * a.q_stride + (long long)h * HD + d;
+                    const uint4 u = *(const uint4*)src, v = *(const uint4*)(src + HD / 2);
+                    const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (int e = 0; e < 8; e++) most = fmaxf(most, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-                }
-                float up;
-                down = kv8_row_factor(most, &up);
-                scale *= up;
-            }
-#pragma unroll 4
-            for (int d = 0; d < HD / 2; d += 8) {
-                if (valid && nb > 0) {
-                    turned8(src, cs, sn, d, lo, hi);
+                    for (int e = 0; e < 8; e++) {
+                        x[0][e] = kv8_from_bits((uw[e / 2] >> (16 * (e & 1))) & 0xffffu);
+                        x[1][e] = kv8_from_bits((vw[e / 2] >> (16 * (e & 1))) & 0xffffu);
+                    }
+                    if (a.cos_tab != nullptr) {
+                        const float* cs = a.cos_tab + (long long)ps * (HD / 2) + d;
+                        const float* sn = a.sin_tab + (long long)ps * (HD / 2) + d;
+#pragma unroll
+                        for (int j = 0; j < 8; j += 4) {
+                            const float4 c = *(const float4*)(cs + j), n = *(const float4*)(sn + j);
+                            const float cc[4] = {c.x, c.y, c.z, c.w}, nn[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float lo = x[0][j + e], hi = x[1][j + e];
+                                x[0][j + e] = lo * cc[e] - hi * nn[e];
+                                x[1][j + e] = lo * nn[e] + hi * cc[e];
+                            }
+                        }
+                    }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) lo[e] = hi[e] = 0.f;
+                    for (int e = 0; e < 8; e++) x[0][e] = x[1][e] = 0.f;
+                }
+                float down = 1.f;
+                if (EIGHT) {
+                    float most = 0.f, up;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, fmaxf(fabsf(x[0][e]), fabsf(x[1][e])));
+#pragma unroll
+                    for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    down = kv8_row_factor(most, &up);
+                    const float mine = __shfl_sync(0xffffffffu, up, lane % AT_ONCE * PER);
+                    if (lane / AT_ONCE == k) scale *= mine;
                 }
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     const int dim = d + half * (HD / 2);
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = (half ? hi[e] : lo[e]) * down;
                     uint32_t w[4], rest[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        w[e] = pack16<EIGHT>(x[2 * e], x[2 * e + 1]);
-                        if (!EIGHT) rest[e] = rest_bf16(x[2 * e], x[2 * e + 1], w[e]);
+                        const float q0 = x[half][2 * e] * down, q1 = x[half][2 * e + 1] * down;
+                        w[e] = pack16<EIGHT>(q0, q1);
+                        if (!EIGHT) rest[e] = rest_bf16(q0, q1, w[e]);
                     }
-                    uint8_t* to = qt + (dim / 64) * (BM * 128) + ((((dim % 64) / 8) ^ (r & 7)) << 4);
+                    uint8_t* to = qt + (dim / 64) * (BM * 128) + rr * 128 + ((((dim % 64) / 8) ^ (rr & 7)) << 4);
                     *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
                     if (!EIGHT) *(uint4*)(to + Q_BYTES) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
                 }
             }
             fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->q_full);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->q_full);
         float m_run = -INFINITY, l_run = 0.f, ref = 1.f;
         bool ok = true;
         for (int i = 0; i < nb; i++) {
@@ -622,7 +676,9 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
 #pragma unroll
                 for (int k = 0; k < BN; k += 4) {
                     const float4 f = *(const float4*)&sc->k[k];
-                    s[k] *= f.x; s[k + 1] *= f.y; s[k + 2] *= f.z; s[k + 3] *= f.w;
+                    const float2 x = mul2(make_float2(s[k], s[k + 1]), make_float2(f.x, f.y));
+                    const float2 y = mul2(make_float2(s[k + 2], s[k + 3]), make_float2(f.z, f.w));
+                    s[k] = x.x; s[k + 1] = x.y; s[k + 2] = y.x; s[k + 3] = y.y;
                 }
             } else {
                 const int j = j_lo + i, page = j < a.max_pages ? trow[j] : -1;
@@ -665,40 +721,10 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 m_run = m_new;
             }
             const float neg_m = (m_run == -INFINITY ? 0.f : -m_run) + Z::HEADROOM;
-            float sum4[4] = {0.f, 0.f, 0.f, 0.f};
             const uint32_t p_addr = s_addr + (uint32_t)((i & 1) * BN);
-#pragma unroll
-            for (int k0 = 0; k0 < BN; k0 += 16) {
-                uint32_t w[8], rest[8];
-#pragma unroll
-                for (int k = 0; k < 16; k += 4) {
-                    float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
-                    if (EIGHT) f = *(const float4*)&sc->v[k0 + k];
-                    float p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        p[e] = fast_exp2(fmaf(s[k0 + k + e], scale, neg_m));
-                        sum4[e] += p[e];
-                    }
-                    if (EIGHT) {
-                        const bool gone = masked;
-                        p[0] = gone && s[k0 + k] == -INFINITY ? 0.f : p[0] * f.x;
-                        p[1] = gone && s[k0 + k + 1] == -INFINITY ? 0.f : p[1] * f.y;
-                        p[2] = gone && s[k0 + k + 2] == -INFINITY ? 0.f : p[2] * f.z;
-                        p[3] = gone && s[k0 + k + 3] == -INFINITY ? 0.f : p[3] * f.w;
-                    }
-                    w[k / 2] = pack16<EIGHT>(p[0], p[1]);
-                    w[k / 2 + 1] = pack16<EIGHT>(p[2], p[3]);
-                    if (!EIGHT) {
-                        rest[k / 2] = rest_bf16(p[0], p[1], w[k / 2]);
-                        rest[k / 2 + 1] = rest_bf16(p[2], p[3], w[k / 2 + 1]);
-                    }
-                }
-                tmem_st8(p_addr + (uint32_t)(k0 / 2), w);
-                if (!EIGHT) tmem_st8(p_addr + (uint32_t)(BN / 2 + k0 / 2), rest);
-            }
+            const float* vs = EIGHT ? sc->v : nullptr;
+            l_run += EIGHT && masked ? page_weights<EIGHT, true>(s, vs, scale, neg_m, p_addr) : page_weights<EIGHT, false>(s, vs, scale, neg_m, p_addr);
             tmem_st_wait();
-            l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
             fence_before();
             __syncwarp();
             if (lane == 0) {

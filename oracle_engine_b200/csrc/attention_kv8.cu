@@ -34,6 +34,7 @@ static_assert(HD == 64 || HD == 128, "built for head_dim 64 or 128");
 constexpr int KS = HD / 16;
 constexpr int TB = 32;                           // keys per tile: half a page
 constexpr int PARTS = OE_PAGE / TB;
+constexpr int MAX_ORDERED = 256;
 constexpr int MAX_JOINED = 160;                  // parts that a result is joined from: a cluster's CTAs and a prefix's splits
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -46,60 +47,44 @@ kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ co
                  uint8_t* codes, float* scales, long long n_pages, const int* __restrict__ tables, int max_pages,
                  const int* __restrict__ tok_seq, const int* __restrict__ tok_pos, int n_tokens, int H, int KVH) {
     constexpr int LANES = HD / 16;
+    pdl_launch_dependents();
     pdl_wait();
     const unsigned item = blockIdx.x * 256u + threadIdx.x, r = item / LANES;       // a row: (token, K or V, KV head)
     const int i = (int)(item % LANES) * 8;
     const unsigned per_token = 2u * KVH, t = r / per_token, which_head = r - t * per_token;
     const int which = which_head >= (unsigned)KVH, kvh = (int)which_head - (which ? KVH : 0);
-    const int b = t < (unsigned)n_tokens ? tok_seq[t] : -1;
-    const int pos = b >= 0 ? tok_pos[t] : 0;
-    const int page = b >= 0 && pos / OE_PAGE < max_pages ? tables[(long long)b * max_pages + pos / OE_PAGE] : -1;
-    const bool ok = page >= 0 && page < n_pages;
-    uint32_t lo[4] = {0, 0, 0, 0}, hi[4] = {0, 0, 0, 0};
-    if (ok) {
-        const bf16* row = qkv + (long long)t * stride + (long long)(H + which * KVH + kvh) * HD;
-        const uint4 a = *(const uint4*)(row + i), c = *(const uint4*)(row + i + HD / 2);
-        lo[0] = a.x; lo[1] = a.y; lo[2] = a.z; lo[3] = a.w;
-        hi[0] = c.x; hi[1] = c.y; hi[2] = c.z; hi[3] = c.w;
-        if (which == 0 && cos_tab != nullptr) {
-            float cs[8], sn[8];
+    // (two rounds of loads: the row and the token's place, then the page's number and the angle)
+    const bool here = t < (unsigned)n_tokens;
+    const bf16* row = qkv + (long long)(here ? t : 0) * stride + (long long)(H + which * KVH + kvh) * HD;
+    const uint4 x0 = *(const uint4*)(row + i), x1 = *(const uint4*)(row + i + HD / 2);
+    const int b = here ? tok_seq[t] : -1, pos = here ? max(tok_pos[t], 0) : 0;
+    const bool turns = which == 0 && cos_tab != nullptr && b >= 0;
+    float cs[8], sn[8];
+    if (turns) {
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                *(float4*)&cs[j] = *(const float4*)(cos_tab + (long long)pos * (HD / 2) + i + j);
-                *(float4*)&sn[j] = *(const float4*)(sin_tab + (long long)pos * (HD / 2) + i + j);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t nl = 0, nh = 0;
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float x0 = kv8_from_bits((lo[j] >> (16 * e)) & 0xffffu), x1 = kv8_from_bits((hi[j] >> (16 * e)) & 0xffffu);
-                    nl |= kv8_turned_bits(x0, cs[2 * j + e], x1, sn[2 * j + e]) << (16 * e);
-                    nh |= kv8_turned_bits(x0, sn[2 * j + e], -x1, cs[2 * j + e]) << (16 * e);
-                }
-                lo[j] = nl;
-                hi[j] = nh;
-            }
+        for (int j = 0; j < 8; j += 4) {
+            *(float4*)&cs[j] = *(const float4*)(cos_tab + (long long)pos * (HD / 2) + i + j);
+            *(float4*)&sn[j] = *(const float4*)(sin_tab + (long long)pos * (HD / 2) + i + j);
         }
     }
-    uint32_t m = 0;
+    const int page = b >= 0 && pos / OE_PAGE < max_pages ? tables[(long long)b * max_pages + pos / OE_PAGE] : -1;
+    const bool ok = page >= 0 && page < n_pages;
+    uint32_t lo[4] = {x0.x, x0.y, x0.z, x0.w}, hi[4] = {x1.x, x1.y, x1.z, x1.w};      // dimensions i .. i + 7, and those they are turned with
+    if (turns) kv8_turn<8>(lo, hi, cs, sn);
+    uint32_t w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        m = max(m, max(lo[j] & 0x7fffu, (lo[j] >> 16) & 0x7fffu));
-        m = max(m, max(hi[j] & 0x7fffu, (hi[j] >> 16) & 0x7fffu));
-    }
+    for (int j = 0; j < 8; j++) most = kv8_most(most, w[j]);
+    most = kv8_most(most);
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (ok) {
-        const Kv8Row q = kv8_row<KIND>(m);
-        const long long at = (((long long)page * 2 + which) * KVH + kvh) * OE_PAGE + pos % OE_PAGE;
-        *(uint2*)(codes + at * HD + i) = make_uint2(kv8_codes4<KIND>(q, lo[0], lo[1]), kv8_codes4<KIND>(q, lo[2], lo[3]));
-        *(uint2*)(codes + at * HD + i + HD / 2) = make_uint2(kv8_codes4<KIND>(q, hi[0], hi[1]), kv8_codes4<KIND>(q, hi[2], hi[3]));
-        if (i == 0) scales[at] = q.scale;
-    }
-    // the kernel behind this one may ask for these rows before it waits
-    __threadfence();
-    pdl_launch_dependents();
+    for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (!ok) return;
+    float scale;
+    const float by = kv8_row<KIND>(most, w, &scale);
+    const long long at = (((long long)page * 2 + which) * KVH + kvh) * OE_PAGE + pos % OE_PAGE;
+    *(uint2*)(codes + at * HD + i) = make_uint2(kv8_codes4<KIND>(by, w[0], w[1]), kv8_codes4<KIND>(by, w[2], w[3]));
+    *(uint2*)(codes + at * HD + i + HD / 2) = make_uint2(kv8_codes4<KIND>(by, w[4], w[5]), kv8_codes4<KIND>(by, w[6], w[7]));
+    if (i == 0) scales[at] = scale;
 }
 
 // ------------------------------------------------------------------------------------------------ the attention
@@ -123,6 +108,7 @@ struct Args {
     float scale_log2;
     int cluster;               // CTAs that share a tile of rows
     int ahead;                 // rows of earlier tokens may be read before the wait
+    int ordered;               // n: blockIdx.z counts the n sequences by their lengths, the longest first
     // sequences that begin with the same pages: what attention_rows.cu has left of those pages
     const int* seq_pages;      // [B] pages of the sequence's prefix (0: none); null: no prefixes
     int splits;
@@ -130,8 +116,9 @@ struct Args {
     const float* part_ml;      // [B * H, splits, 2]
 };
 
-__device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem) : "memory");
+template <int S, int G>
+__device__ __forceinline__ void cp_async16(uint32_t smem, const uint8_t* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(smem), "l"(gmem), "n"(S), "n"(G) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -193,72 +180,93 @@ struct Tile {
     static constexpr int BYTES = S_AT + (KIND == OE_KV_BF16 ? 0 : 2 * TB * 4);
 };
 
+template <int KIND, int I>
+__device__ __forceinline__ void load_rows(uint32_t st, const uint8_t* kg, const uint8_t* vg) {
+    using L = Tile<KIND>;
+    constexpr int AT_ONCE = 512 / (HD * L::ELEM);             // rows that a warp asks for with one instruction
+    cp_async16<I * AT_ONCE * L::K_ROW, I * 512>(st, kg);
+    cp_async16<L::V_AT + I * AT_ONCE * L::V_ROW, I * 512>(st, vg);
+    if constexpr (I + 1 < TB / AT_ONCE) load_rows<KIND, I + 1>(st, kg, vg);
+}
+template <int I>
+__device__ __forceinline__ void load_rows_apart(uint32_t ks, uint32_t vs, const uint8_t* kg, const uint8_t* vg) {
+    using L = Tile<OE_KV_BF16>;
+    constexpr int AT_ONCE = 512 / (HD * 2);
+    cp_async16<I * AT_ONCE * L::K_ROW, I * 512>(ks, kg);
+    cp_async16<L::V_AT + I * AT_ONCE * L::V_ROW, I * 512>(vs, vg);
+    if constexpr (I + 1 < TB / AT_ONCE) load_rows_apart<I + 1>(ks, vs, kg, vg);
+}
 template <int KIND>
 __device__ __forceinline__ void load_tile(uint8_t* st, const Args& a, int page, int part, int kvh, int lane) {
     using L = Tile<KIND>;
     if ((unsigned)page < (unsigned long long)a.n_pages) {
         const long long krow = (((long long)page * 2) * a.KVH + kvh) * OE_PAGE + part * TB, vrow = krow + (long long)a.KVH * OE_PAGE;
         constexpr int PER_ROW = HD * L::ELEM / 16;
-        const uint8_t* kg = (const uint8_t*)a.cache + krow * (HD * L::ELEM);
-        const uint8_t* vg = (const uint8_t*)a.cache + vrow * (HD * L::ELEM);
-#pragma unroll
-        for (int c0 = 0; c0 < TB * PER_ROW; c0 += 32) {
-            const int c = c0 + lane, row = c / PER_ROW, col = c % PER_ROW;
-            cp_async16(st + row * L::K_ROW + col * 16, kg + (size_t)c * 16);
-            cp_async16(st + L::V_AT + row * L::V_ROW + col * 16, vg + (size_t)c * 16);
-        }
+        const uint8_t* kg = (const uint8_t*)a.cache + krow * (HD * L::ELEM) + lane * 16;
+        const uint8_t* vg = kg + (long long)a.KVH * (OE_PAGE * HD * L::ELEM);
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(st) + (lane / PER_ROW) * L::K_ROW + (lane % PER_ROW) * 16;
+        static_assert(L::K_ROW == L::V_ROW || KIND == OE_KV_BF16, "one offset for both");
+        if constexpr (KIND == OE_KV_BF16) load_rows_apart<0>(to, to - (lane / PER_ROW) * (L::K_ROW - L::V_ROW), kg, vg);
+        else load_rows<KIND, 0>(to, kg, vg);
         if (KIND != OE_KV_BF16 && lane < 2 * TB / 4)
-            cp_async16(st + L::S_AT + lane * 16, a.scales + (lane < TB / 4 ? krow : vrow - TB) + lane * 4);
+            cp_async16<L::S_AT, 0>((uint32_t)__cvta_generic_to_shared(st) + lane * 16, (const uint8_t*)(a.scales + (lane < TB / 4 ? krow : vrow - TB) + lane * 4));
     }
 }
 
 __device__ __forceinline__ int page_at(const int* trow, int j, int max_pages) { return j < max_pages ? trow[j] : -1; }
 
-// The new token's key and value, made by one warp: its cache rows' bytes, PP pairs (d, d + HD/2) a lane at d = PP lane.
+// The new token's key and value, made by one warp: its cache rows' bytes.  A lane with an even number has PP pairs of words (or of
+// bytes) of the key, one with an odd number of the value: dimensions d .. d + 2 PP - 1 and d + HD/2 .., d = lane / 2 * 2 PP.
 template <int KIND>
 struct NewToken {
-    static constexpr int PP = HD / 64;
-    uint32_t k0[PP], k1[PP], v0[PP], v1[PP];       // bfloat16 bits, or codes
-    float ks, vs;
+    static constexpr int PP = HD / 64;                      // words a half; HD / 32 dimensions
+    uint32_t w[2 * PP];                                     // bfloat16 pairs; in the 8-bit forms the codes in w[0] and w[1]
+    float scale;
     __device__ __forceinline__ void make(const Args& a, const bf16* row, int pos, int kvh, int lane) {
-        const bf16* kr = row + (size_t)(a.H + kvh) * HD;
-        const bf16* vr = kr + (size_t)a.KVH * HD;
-        uint32_t mk = 0, mv = 0;
+        const int d = lane / 2 * 2 * PP;
+        const bf16* src = row + (size_t)(a.H + (lane & 1) * a.KVH + kvh) * HD + d;
+        uint32_t lo[PP], hi[PP], most = 0;
 #pragma unroll
-        for (int u = 0; u < PP; u++) {
-            const int d = lane * PP + u;
-            k0[u] = __bfloat16_as_ushort(kr[d]); k1[u] = __bfloat16_as_ushort(kr[d + HD / 2]);
-            v0[u] = __bfloat16_as_ushort(vr[d]); v1[u] = __bfloat16_as_ushort(vr[d + HD / 2]);
-            if (a.cos_tab != nullptr) {
-                const float c = a.cos_tab[(size_t)pos * (HD / 2) + d], s = a.sin_tab[(size_t)pos * (HD / 2) + d];
-                const float x0 = kv8_from_bits(k0[u]), x1 = kv8_from_bits(k1[u]);
-                k0[u] = kv8_turned_bits(x0, c, x1, s);
-                k1[u] = kv8_turned_bits(x0, s, -x1, c);
-            }
-            mk = max(mk, max(k0[u] & 0x7fffu, k1[u] & 0x7fffu));
-            mv = max(mv, max(v0[u] & 0x7fffu, v1[u] & 0x7fffu));
+        for (int j = 0; j < PP; j++) { lo[j] = *(const uint32_t*)(src + 2 * j); hi[j] = *(const uint32_t*)(src + HD / 2 + 2 * j); }
+        if (!(lane & 1) && a.cos_tab != nullptr) {
+            float cs[2 * PP], sn[2 * PP];
+#pragma unroll
+            for (int j = 0; j < 2 * PP; j++) { cs[j] = a.cos_tab[(size_t)pos * (HD / 2) + d + j]; sn[j] = a.sin_tab[(size_t)pos * (HD / 2) + d + j]; }
+            kv8_turn<2 * PP>(lo, hi, cs, sn);
         }
-        if (KIND != OE_KV_BF16) {
-            const Kv8Row qk = kv8_row<KIND>(__reduce_max_sync(0xffffffffu, mk)), qv = kv8_row<KIND>(__reduce_max_sync(0xffffffffu, mv));
 #pragma unroll
-            for (int u = 0; u < PP; u++) {
-                k0[u] = kv8_code<KIND>(qk, k0[u]); k1[u] = kv8_code<KIND>(qk, k1[u]);
-                v0[u] = kv8_code<KIND>(qv, v0[u]); v1[u] = kv8_code<KIND>(qv, v1[u]);
+        for (int j = 0; j < PP; j++) { w[j] = lo[j]; w[PP + j] = hi[j]; most = kv8_most(kv8_most(most, lo[j]), hi[j]); }
+        if (KIND != OE_KV_BF16) {
+            most = kv8_most(most);
+#pragma unroll
+            for (int o = 2; o < 32; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float by = kv8_row<KIND>(most, w, &scale);
+            if (PP == 2) {
+                w[0] = kv8_codes4<KIND>(by, w[0], w[1]);
+                w[1] = kv8_codes4<KIND>(by, w[2], w[2 * PP - 1]);
+            } else {
+                const uint32_t c = kv8_codes4<KIND>(by, w[0], w[1]);
+                w[0] = c & 0xffffu;
+                w[1] = c >> 16;
             }
-            ks = qk.scale; vs = qv.scale;
         }
     }
-    __device__ __forceinline__ void store(uint8_t* krow, uint8_t* vrow, int lane) const {
+    // rows: where the key's row lies, and how far behind it the value's
+    __device__ __forceinline__ void store(uint8_t* krow, size_t to_value, int lane) const {
+        uint8_t* row = krow + (lane & 1) * to_value;
+        const int d = lane / 2 * 2 * PP;
+        if (KIND == OE_KV_BF16) {
 #pragma unroll
-        for (int u = 0; u < PP; u++) {
-            const int d = lane * PP + u;
-            if (KIND == OE_KV_BF16) {
-                ((uint16_t*)krow)[d] = (uint16_t)k0[u]; ((uint16_t*)krow)[d + HD / 2] = (uint16_t)k1[u];
-                ((uint16_t*)vrow)[d] = (uint16_t)v0[u]; ((uint16_t*)vrow)[d + HD / 2] = (uint16_t)v1[u];
-            } else {
-                krow[d] = (uint8_t)k0[u]; krow[d + HD / 2] = (uint8_t)k1[u];
-                vrow[d] = (uint8_t)v0[u]; vrow[d + HD / 2] = (uint8_t)v1[u];
+            for (int j = 0; j < PP; j++) {
+                *(uint32_t*)(row + (d + 2 * j) * 2) = w[j];
+                *(uint32_t*)(row + (d + HD / 2 + 2 * j) * 2) = w[PP + j];
             }
+        } else if (PP == 2) {
+            *(uint32_t*)(row + d) = w[0];
+            *(uint32_t*)(row + d + HD / 2) = w[1];
+        } else {
+            *(uint16_t*)(row + d) = (uint16_t)w[0];
+            *(uint16_t*)(row + d + HD / 2) = (uint16_t)w[1];
         }
     }
 };
@@ -294,7 +302,22 @@ attn_kv8_kernel(const Args a) {
     const int G = a.H / a.KVH, kvh = blockIdx.y;
     const int CR = a.cluster, rank = CR > 1 ? (int)cluster_ctarank() : 0;
     const int bx = blockIdx.x / CR;
-    const int b = blockIdx.z, row0 = bx * ROWS, qlen = a.seq_qlen[b], n_rows = qlen > 0 ? qlen * G : 0;
+    int b = blockIdx.z;
+    if (a.ordered) {
+        // more CTAs than there is room for: the long sequences' start first, so that the short ones' fill the end
+        __shared__ int len[MAX_ORDERED], which;
+        for (int t = threadIdx.x; t < a.ordered; t += NW * 32)
+            len[t] = a.seq_qlen[t] > 0 ? a.seq_start[t] + 1 - (a.seq_pages != nullptr ? a.seq_pages[t] * OE_PAGE : 0) : 0;
+        __syncthreads();
+        for (int t = threadIdx.x; t < a.ordered; t += NW * 32) {
+            int before = 0;
+            for (int j = 0; j < a.ordered; j++) before += len[j] > len[t] || (len[j] == len[t] && j < t);
+            if (before == b) which = t;
+        }
+        __syncthreads();
+        b = which;
+    }
+    const int row0 = bx * ROWS, qlen = a.seq_qlen[b], n_rows = qlen > 0 ? qlen * G : 0;
     if (row0 >= n_rows) {                                            // the whole cluster
         pdl_wait();
         return;
@@ -372,7 +395,8 @@ attn_kv8_kernel(const Args a) {
         for (int ks = 0; ks < KS; ks++) {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                const float q0 = qv[ks][2 * x] * down, q1 = qv[ks][2 * x + 1] * down;
+                // (a pair of the keys' codes: kv8_first and kv8_second)
+                const float q0 = qv[ks][KIND == OE_KV_INT8 ? x : 2 * x] * down, q1 = qv[ks][KIND == OE_KV_INT8 ? x + 2 : 2 * x + 1] * down;
                 if (EIGHT) {
                     qf[nt][ks][x] = pack_f16(q0, q1);
                 } else {
@@ -405,8 +429,8 @@ attn_kv8_kernel(const Args a) {
         const int page = page_at(trow, start / OE_PAGE, a.max_pages);
         if ((unsigned)page < (unsigned long long)a.n_pages) {
             const long long krow = (((long long)page * 2) * a.KVH + kvh) * OE_PAGE + start % OE_PAGE, vrow = krow + (long long)a.KVH * OE_PAGE;
-            fresh.store((uint8_t*)a.cache_w + krow * (HD * L::ELEM), (uint8_t*)a.cache_w + vrow * (HD * L::ELEM), lane);
-            if (EIGHT && lane == 0) { a.scales_w[krow] = fresh.ks; a.scales_w[vrow] = fresh.vs; }
+            fresh.store((uint8_t*)a.cache_w + krow * (HD * L::ELEM), (size_t)a.KVH * OE_PAGE * HD * L::ELEM, lane);
+            if (EIGHT && lane < 2) a.scales_w[lane ? vrow : krow] = fresh.scale;
         }
     }
 
@@ -425,8 +449,8 @@ attn_kv8_kernel(const Args a) {
         __syncwarp();
         if (own_kv && tile == t_hi) {
             const int r = start % TB;
-            fresh.store(cur + r * L::K_ROW, cur + L::V_AT + r * L::V_ROW, lane);
-            if (EIGHT && lane == 0) { ((float*)(cur + L::S_AT))[r] = fresh.ks; ((float*)(cur + L::S_AT))[TB + r] = fresh.vs; }
+            fresh.store(cur + r * L::K_ROW, L::V_AT + r * (L::V_ROW - L::K_ROW), lane);
+            if (EIGHT && lane < 2) ((float*)(cur + L::S_AT))[lane * TB + r] = fresh.scale;
             __syncwarp();
         }
         if ((unsigned)page_at(trow, tile / PARTS, a.max_pages) < (unsigned long long)a.n_pages) {
@@ -440,10 +464,9 @@ attn_kv8_kernel(const Args a) {
                 for (int ks = 0; ks < KS; ks++) {
                     uint32_t f[4];
                     if (EIGHT) {
-                        const uint32_t w0 = kv8_word<KIND>(*(const uint32_t*)(kr + ks * 16));
-                        const uint32_t w1 = kv8_word<KIND>(*(const uint32_t*)(kr + 8 * L::K_ROW + ks * 16));
-                        f[0] = kv8_pair<KIND>(w0, 0); f[2] = kv8_pair<KIND>(w0, 2);
-                        f[1] = kv8_pair<KIND>(w1, 0); f[3] = kv8_pair<KIND>(w1, 2);
+                        const uint32_t w0 = *(const uint32_t*)(kr + ks * 16), w1 = *(const uint32_t*)(kr + 8 * L::K_ROW + ks * 16);
+                        f[0] = kv8_first<KIND>(w0); f[2] = kv8_second<KIND>(w0);
+                        f[1] = kv8_first<KIND>(w1); f[3] = kv8_second<KIND>(w1);
                     } else {
                         const uint2 w0 = *(const uint2*)(kr + ks * 32), w1 = *(const uint2*)(kr + 8 * L::K_ROW + ks * 32);
                         f[0] = w0.x; f[2] = w0.y; f[1] = w1.x; f[3] = w1.y;
@@ -546,12 +569,13 @@ attn_kv8_kernel(const Args a) {
                 for (int c = 0; c < HD / 32; c++) {
                     uint32_t f[2][4];                       // dims c * 32 + gid * 4 + {0, 1} and + {2, 3}
                     if (EIGHT) {
-                        const uint32_t w0 = kv8_word<KIND>(*(const uint32_t*)(vr + c * 32)), w1 = kv8_word<KIND>(*(const uint32_t*)(vr + L::V_ROW + c * 32));
-                        const uint32_t w2 = kv8_word<KIND>(*(const uint32_t*)(vr + 8 * L::V_ROW + c * 32)), w3 = kv8_word<KIND>(*(const uint32_t*)(vr + 9 * L::V_ROW + c * 32));
-                        const uint32_t x0 = kv8_prmt(w0, w1, 0x5140u), x1 = kv8_prmt(w0, w1, 0x7362u);
-                        const uint32_t y0 = kv8_prmt(w2, w3, 0x5140u), y1 = kv8_prmt(w2, w3, 0x7362u);
-                        f[0][0] = kv8_pair<KIND>(x0, 0); f[0][1] = kv8_pair<KIND>(x0, 2); f[0][2] = kv8_pair<KIND>(y0, 0); f[0][3] = kv8_pair<KIND>(y0, 2);
-                        f[1][0] = kv8_pair<KIND>(x1, 0); f[1][1] = kv8_pair<KIND>(x1, 2); f[1][2] = kv8_pair<KIND>(y1, 0); f[1][3] = kv8_pair<KIND>(y1, 2);
+                        const uint32_t w0 = *(const uint32_t*)(vr + c * 32), w1 = *(const uint32_t*)(vr + L::V_ROW + c * 32);
+                        const uint32_t w2 = *(const uint32_t*)(vr + 8 * L::V_ROW + c * 32), w3 = *(const uint32_t*)(vr + 9 * L::V_ROW + c * 32);
+                        constexpr uint32_t LOWER = KIND == OE_KV_INT8 ? 0x5410u : 0x5140u, UPPER = KIND == OE_KV_INT8 ? 0x7632u : 0x7362u;
+                        const uint32_t x0 = kv8_prmt(w0, w1, LOWER), x1 = kv8_prmt(w0, w1, UPPER);
+                        const uint32_t y0 = kv8_prmt(w2, w3, LOWER), y1 = kv8_prmt(w2, w3, UPPER);
+                        f[0][0] = kv8_first<KIND>(x0); f[0][1] = kv8_second<KIND>(x0); f[0][2] = kv8_first<KIND>(y0); f[0][3] = kv8_second<KIND>(y0);
+                        f[1][0] = kv8_first<KIND>(x1); f[1][1] = kv8_second<KIND>(x1); f[1][2] = kv8_first<KIND>(y1); f[1][3] = kv8_second<KIND>(y1);
                     } else {
                         uint2 w0 = *(const uint2*)(vr + c * 64), w1 = *(const uint2*)(vr + L::V_ROW + c * 64);
                         uint2 w2 = *(const uint2*)(vr + 8 * L::V_ROW + c * 64), w3 = *(const uint2*)(vr + 9 * L::V_ROW + c * 64);
@@ -749,7 +773,7 @@ int oe_kv8_write(int kind, const bf16* qkv, long long stride, const float* cos_t
 int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, void* cache,
                 float* scales, int write, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
                 const int* seq_qlen, int n_seqs, int max_qlen, int H, int KVH, int window, float scale, int warps, int cluster,
-                const int* seq_pages, int splits, const float* part_o, const float* part_ml, int ahead, cudaStream_t st) {
+                int ordered, const int* seq_pages, int splits, const float* part_o, const float* part_ml, int ahead, cudaStream_t st) {
     if (n_seqs <= 0 || max_qlen <= 0) return 0;
     if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15) ||
         ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15) || ((uintptr_t)out & 15)) return OE_ERR_UNSUPPORTED;
@@ -762,6 +786,7 @@ int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const fl
     a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start; a.seq_qlen = seq_qlen;
     a.H = H; a.KVH = KVH; a.window = window; a.scale_log2 = scale * LOG2E; a.cluster = cluster;
     a.seq_pages = seq_pages; a.splits = splits; a.part_o = part_o; a.part_ml = part_ml; a.ahead = ahead;
+    a.ordered = ordered && window == 0 && n_seqs > 1 && n_seqs <= MAX_ORDERED ? n_seqs : 0;
     const long long rows = (long long)max_qlen * (H / KVH);
     if (kind == OE_KV_BF16) return launch_rows<OE_KV_BF16>(warps, a, rows, n_seqs, st);
     if (kind == OE_KV_INT8) return launch_rows<OE_KV_INT8>(warps, a, rows, n_seqs, st);

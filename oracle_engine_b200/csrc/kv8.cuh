@@ -8,9 +8,9 @@
 // The row is what a 16-bit cache would hold: the projected value, or the key turned by its position and rounded ONCE to bfloat16.
 // Everything is then exact up to the two roundings above.  With x = x' 2^i and a = a' 2^j, x' and a' of 8 bits, the quotient x c / a
 // differs from a border t between two codes by (x' c 2^k - t a') / a', a fraction with the denominator 2^k' a': it is t, or off it by
-// 2^-16 of itself or more.  A float32 product with the rounded c / a is within 2^-22 of the quotient, and a value within
-// 2^-19 of one of 12 bits, as borders are, is taken for that one: so it lies on the quotient's side of every border, or on it.  Codes
-// and scales therefore do not depend on which kernel wrote them.
+// 2^-16 of itself or more.  A float32 product with the rounded c / a is within 2^-22 of the quotient; rounded to 18 bits (Veltkamp's
+// splitting) it is the border itself where the quotient is one, and on the quotient's side of it where not.  Codes and scales
+// therefore do not depend on which kernel wrote them.
 // A row with an infinite or undefined value gets codes 0 and an undefined scale: it reads as undefined, and codes are always numbers.
 #pragma once
 #include "common.cuh"
@@ -36,52 +36,71 @@ __device__ __noinline__ uint32_t kv8_turned_near(float a, float c, float b, floa
     if ((u & 0xffffu) == 0x8000u && lo != 0.f) return ((lo > 0.f) == (hi > 0.f)) ? (u >> 16) + 1u : u >> 16;
     return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(hi));
 }
-__device__ __forceinline__ uint32_t kv8_turned_bits(float a, float c, float b, float s) {
+__device__ __forceinline__ uint32_t kv8_turned_fast(float a, float c, float b, float s, bool& near) {
     const float q = __fmul_rn(b, s), hi = __fmaf_rn(a, c, -q);
-    const uint32_t u = __float_as_uint(hi);
-    const float border = __uint_as_float((u & 0xffff0000u) | 0x8000u);
-    // (fabsf(hi) + fabsf(q) bounds |a c| as well: 2^-22 of it is more than either operation's error)
-    if (!(fabsf(hi - border) > 2.38418579e-7f * (fabsf(hi) + fabsf(q)))) return kv8_turned_near(a, c, b, s);
+    const float border = __uint_as_float((__float_as_uint(hi) & 0xffff0000u) | 0x8000u);
+    // (either operation's error is at most 2^-24 of its result: together less than 1.2e-7 > 2^-23 of the two)
+    near = near || !(fabsf(hi - border) > 1.2e-7f * (fabsf(hi) + fabsf(q)));
     return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(hi));
 }
 __device__ __forceinline__ float kv8_from_bits(uint32_t b) { return __uint_as_float(b << 16); }
 
-// What a row's codes are made from, of its largest magnitude as bfloat16 bits without the sign (an undefined value is the largest).
-struct Kv8Row {
-    float pre, by;         // a code is x * pre * by: pre a power of two that keeps c / (a pre) within float32's range
-    float scale;
-    bool bad;
-};
-template <int KIND>
-__device__ __forceinline__ Kv8Row kv8_row(uint32_t max_bits) {
+// N pairs (x0, x1) of a row, two bfloat16 to a word of lo and of hi, turned by cs and sn: x0 cs - x1 sn and x0 sn + x1 cs.
+template <int N>
+__device__ __forceinline__ void kv8_turn(uint32_t (&lo)[N / 2], uint32_t (&hi)[N / 2], const float (&cs)[N], const float (&sn)[N]) {
+    uint32_t nl[N / 2], nh[N / 2];
+    bool near = false;
+#pragma unroll
+    for (int j = 0; j < N / 2; j++) {
+        const float x0 = kv8_from_bits(lo[j]), y0 = __uint_as_float(lo[j] & 0xffff0000u), x1 = kv8_from_bits(hi[j]), y1 = __uint_as_float(hi[j] & 0xffff0000u);
+        nl[j] = kv8_turned_fast(x0, cs[2 * j], x1, sn[2 * j], near) | kv8_turned_fast(y0, cs[2 * j + 1], y1, sn[2 * j + 1], near) << 16;
+        nh[j] = kv8_turned_fast(x0, sn[2 * j], -x1, cs[2 * j], near) | kv8_turned_fast(y0, sn[2 * j + 1], -y1, cs[2 * j + 1], near) << 16;
+    }
+    if (near) {
+#pragma unroll
+        for (int j = 0; j < N / 2; j++) {
+            const float x0 = kv8_from_bits(lo[j]), y0 = __uint_as_float(lo[j] & 0xffff0000u), x1 = kv8_from_bits(hi[j]), y1 = __uint_as_float(hi[j] & 0xffff0000u);
+            nl[j] = kv8_turned_near(x0, cs[2 * j], x1, sn[2 * j]) | kv8_turned_near(y0, cs[2 * j + 1], y1, sn[2 * j + 1]) << 16;
+            nh[j] = kv8_turned_near(x0, sn[2 * j], -x1, cs[2 * j]) | kv8_turned_near(y0, sn[2 * j + 1], -y1, cs[2 * j + 1]) << 16;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N / 2; j++) { lo[j] = nl[j]; hi[j] = nh[j]; }
+}
+// The largest magnitudes of two words' halves, as bfloat16 bits (an undefined value is the largest).
+__device__ __forceinline__ uint32_t kv8_most(uint32_t a, uint32_t b) { return __vmaxu2(a, b & 0x7fff7fffu); }
+__device__ __forceinline__ uint32_t kv8_most(uint32_t a) { return max(a & 0xffffu, a >> 16); }
+
+// From the bits of a row's largest magnitude: c / a for its codes, and its scale.  The words of a row that cannot be had that way
+// are changed: to zero where there is no largest magnitude, and times 2^64 where c / a would leave float32's range.
+template <int KIND, int N>
+__device__ __forceinline__ float kv8_row(uint32_t max_bits, uint32_t (&words)[N], float* scale) {
     constexpr float C = KIND == OE_KV_INT8 ? 127.f : 448.f;
-    Kv8Row r;
-    const float a = kv8_from_bits(max_bits);
-    r.bad = max_bits >= 0x7f80u;
-    r.pre = a >= 1.26765060e30f ? 5.42101086e-20f : a < 7.88860905e-31f ? 1.84467441e19f : 1.f;      // 2^100: 2^-64; below 2^-100: 2^64
-    r.by = a > 0.f ? __fdiv_rn(C, a * r.pre) : 0.f;
-    r.scale = r.bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a, C);
-    if (r.bad) r.by = 0.f;
-    return r;
+    float a = kv8_from_bits(max_bits);
+    *scale = max_bits >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a, C);
+    if (max_bits >= 0x7f80u || max_bits == 0u) {
+#pragma unroll
+        for (int j = 0; j < N; j++) words[j] = 0u;
+        return 0.f;
+    }
+    if (a < 7.88860905e-31f) {                              // 2^-100
+        a *= 1.84467441e19f;                                // 2^64
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            words[j] = __float_as_uint(kv8_from_bits(words[j]) * 1.84467441e19f) >> 16 |
+                       (__float_as_uint(__uint_as_float(words[j] & 0xffff0000u) * 1.84467441e19f) & 0xffff0000u);
+    }
+    return __fdiv_rn(C, a);
 }
-template <int KIND>
-__device__ __forceinline__ float kv8_quotient(const Kv8Row& r, uint32_t bits) {
-    const float y = __fmul_rn(__fmul_rn(kv8_from_bits(bits), r.pre), r.by);
-    const uint32_t u = __float_as_uint(y) + 16u;            // within 16 of a multiple of 2^11 in the last place: that multiple
-    const uint32_t v = (u & 0x7ffu) <= 32u ? u & 0xfffff800u : u - 16u;
-    return r.bad ? 0.f : __uint_as_float(v);
+__device__ __forceinline__ float kv8_quotient(float x, float by) {
+    const float y = __fmul_rn(x, by), t = __fmul_rn(y, 65.f);
+    return __fsub_rn(t, __fsub_rn(t, y));
 }
+// The codes of two words' four values, the first in the lowest byte.
 template <int KIND>
-__device__ __forceinline__ uint32_t kv8_code(const Kv8Row& r, uint32_t bits) {
-    const float x = kv8_quotient<KIND>(r, bits);
-    if (KIND == OE_KV_INT8) return (uint32_t)(__float2int_rn(x) & 0xff);
-    return (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
-}
-// Four codes of consecutive values, two to a word of `bits`, the first in the lowest byte.
-template <int KIND>
-__device__ __forceinline__ uint32_t kv8_codes4(const Kv8Row& r, uint32_t b01, uint32_t b23) {
-    const float x0 = kv8_quotient<KIND>(r, b01 & 0xffffu), x1 = kv8_quotient<KIND>(r, b01 >> 16);
-    const float x2 = kv8_quotient<KIND>(r, b23 & 0xffffu), x3 = kv8_quotient<KIND>(r, b23 >> 16);
+__device__ __forceinline__ uint32_t kv8_codes4(float by, uint32_t b01, uint32_t b23) {
+    const float x0 = kv8_quotient(kv8_from_bits(b01), by), x1 = kv8_quotient(__uint_as_float(b01 & 0xffff0000u), by);
+    const float x2 = kv8_quotient(kv8_from_bits(b23), by), x3 = kv8_quotient(__uint_as_float(b23 & 0xffff0000u), by);
     if (KIND == OE_KV_INT8) {
         // 1.5 * 2^23 + x, rounded to nearest even as the sum is: its lowest byte is the code
         const uint32_t i0 = __float_as_uint(__fadd_rn(x0, 12582912.f)), i1 = __float_as_uint(__fadd_rn(x1, 12582912.f));
@@ -107,6 +126,19 @@ __device__ __forceinline__ uint32_t kv8_pair(uint32_t x, int lo) {
         asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(lo == 0 ? x : x >> 16));
     }
     return d;
+}
+// The same in an order that costs less: int8's first pair are the bytes 0 and 2, its second the bytes 1 and 3; e4m3's 0 and 1, and 2 and 3.
+// (The shift is a product's upper half: shifts, permutes and logic share the pipe that conversions are bound by.)
+template <int KIND>
+__device__ __forceinline__ uint32_t kv8_first(uint32_t w) {
+    if (KIND != OE_KV_INT8) return kv8_pair<KIND>(w, 0);
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"((w & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
+    return d;
+}
+template <int KIND>
+__device__ __forceinline__ uint32_t kv8_second(uint32_t w) {
+    return KIND == OE_KV_INT8 ? kv8_first<KIND>(__umulhi(w, 1u << 24)) : kv8_pair<KIND>(w, 2);
 }
 // A query row as float16: multiplied by the power of two that brings its largest magnitude into [1, 2), so that nothing leaves
 // float16's range and 11 bits are kept of every value within 2^-14 of the largest.  `up`: the inverse, for the scores.

@@ -37,7 +37,7 @@ def _lib(head_dim: int):
         lib = _build.load("attention_kv8", {"OE_HD": head_dim})
         P, I, F, L = c_void_p, c_int, c_float, c_longlong
         lib.oe_kv8_write.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, I, P]
-        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, I, P, I, P, P, I, P]
+        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, I, I, P, I, P, P, I, P]
         lib.oe_kv8_write.restype = lib.oe_attn_kv8.restype = c_int
         _libs[head_dim] = lib
     return lib
@@ -146,6 +146,11 @@ def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv
         tables.data_ptr(), tables.shape[1], tok_seq.data_ptr(), tok_pos.data_ptr(), T, n_heads, n_kv_heads, ops._stream()), what)
 
 
+def many_pairs(n_seqs: int, n_kv_heads: int, sm_count: int | None = None) -> bool:
+    """More (sequence, KV head) pairs than CTAs of four warps that are resident at once: the longest sequences go first."""
+    return n_seqs * n_kv_heads > 3 * (sm_count or ops.sm_count())
+
+
 def decode_form(n_seqs: int, n_kv_heads: int, context_class: int, sm_count: int | None = None) -> tuple:
     """(warps of a CTA, CTAs (a thread-block cluster) that share the keys of one (sequence, KV head)) of a step of few rows."""
     sms = sm_count or ops.sm_count()
@@ -185,7 +190,7 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
             kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(),
             int(has_kv and single), codes.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
             ctx.seq_qlen.data_ptr(), ctx.n_seqs, 1 if single else max(1, ctx.max_qlen), n_heads, n_kv_heads, int(window), float(scale),
-            warps, cluster, None, 0, None, None, int(ahead), ops._stream()), what, {"warps": warps, "cluster": cluster})
+            warps, cluster, int(many_pairs(ctx.n_seqs, n_kv_heads)), None, 0, None, None, int(ahead), ops._stream()), what, {"warps": warps, "cluster": cluster})
         return
     mt, splits = form or prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
     part = _parts(T * n_heads, splits, head_dim, out.device) if splits > 1 else None
@@ -267,5 +272,5 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
             prefix.n_members, mt, splits, *parts, int(ahead), ops._stream()), "attention_shared_prefix", {"tiles": mt, "splits": splits})
     ops._check(_lib(head_dim).oe_attn_kv8(
         kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), int(has_kv),
-        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 4, 1, prefix.seq_pages.data_ptr(), splits,
+        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 4, 1, int(many_pairs(B, n_kv_heads)), prefix.seq_pages.data_ptr(), splits,
         *parts, int(ahead), ops._stream()), what)

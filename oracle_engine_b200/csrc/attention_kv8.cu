@@ -114,6 +114,10 @@ struct Args {
     int splits;
     const float* part_o;       // [B * H, splits, HD]
     const float* part_ml;      // [B * H, splits, 2]
+    // 1, or how many CTAs that are no cluster share a tile of rows: each leaves a part for the kernel that joins them
+    int shares;
+    float* own_o;              // [T * H, shares, HD]
+    float* own_ml;             // [T * H, shares, 2]
 };
 
 template <int S, int G>
@@ -301,7 +305,7 @@ attn_kv8_kernel(const Args a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     const int G = a.H / a.KVH, kvh = blockIdx.y;
     const int CR = a.cluster, rank = CR > 1 ? (int)cluster_ctarank() : 0;
-    const int bx = blockIdx.x / CR;
+    const int bx = blockIdx.x / (CR * a.shares);
     int b = blockIdx.z;
     if (a.ordered) {
         // more CTAs than there is room for: the long sequences' start first, so that the short ones' fill the end
@@ -331,7 +335,7 @@ attn_kv8_kernel(const Args a) {
     key_lo = max(key_lo, common * OE_PAGE);
     const int* trow = a.tables + (size_t)b * a.max_pages;
     uint8_t* mine = smem + (size_t)warp * WARP_BYTES;
-    const int gw = rank * NW + warp, stride = NW * CR;
+    const int share = a.shares > 1 ? (int)blockIdx.x % a.shares : rank, gw = share * NW + warp, stride = NW * CR * a.shares;
     const int t_lo = key_lo / TB, t_hi = key_hi >= key_lo ? key_hi / TB : t_lo - 1;
     const int n_my = t_lo + gw <= t_hi ? (t_hi - t_lo - gw) / stride + 1 : 0;
     const bool own_kv = a.cache_w != nullptr;
@@ -339,12 +343,13 @@ attn_kv8_kernel(const Args a) {
     // come from the kernel before this one
     const bool ahead = a.ahead && own_kv;
     if (!ahead) pdl_wait();
+    // the page numbers of this warp's next 32 tiles, one a lane, and of the 32 behind them
+    auto pages_from = [&](int it) { return it + lane < n_my ? page_at(trow, (t_lo + gw + (it + lane) * stride) / PARTS, a.max_pages) : -1; };
+    int pages = pages_from(0), pages_next = pages_from(32);
 #pragma unroll
     for (int pre = 0; pre < ST; pre++) {
-        if (pre < n_my) {
-            const int tile = t_lo + gw + pre * stride;
-            load_tile<KIND>(mine + pre * L::BYTES, a, page_at(trow, tile / PARTS, a.max_pages), tile % PARTS, kvh, lane);
-        }
+        const int page = __shfl_sync(0xffffffffu, pages, pre);
+        if (pre < n_my) load_tile<KIND>(mine + pre * L::BYTES, a, page, (t_lo + gw + pre * stride) % PARTS, kvh, lane);
         cp_async_commit();
     }
     if (ahead) pdl_wait();
@@ -445,6 +450,12 @@ attn_kv8_kernel(const Args a) {
     for (int it = 0; it < n_my; it++) {
         const int tile = t_lo + gw + it * stride;
         uint8_t* cur = mine + (size_t)stage * L::BYTES;
+        const int page = __shfl_sync(0xffffffffu, pages, it & 31);
+        const int page_ahead = __shfl_sync(0xffffffffu, (it & 31) + ST < 32 ? pages : pages_next, (it + ST) & 31);
+        if ((it & 31) == 31) {
+            pages = pages_next;
+            pages_next = pages_from(it + 33);
+        }
         cp_async_wait<ST - 1>();
         __syncwarp();
         if (own_kv && tile == t_hi) {
@@ -453,7 +464,7 @@ attn_kv8_kernel(const Args a) {
             if (EIGHT && lane < 2) ((float*)(cur + L::S_AT))[lane * TB + r] = fresh.scale;
             __syncwarp();
         }
-        if ((unsigned)page_at(trow, tile / PARTS, a.max_pages) < (unsigned long long)a.n_pages) {
+        if ((unsigned)page < (unsigned long long)a.n_pages) {
             float s[NT][TB / 16][4];
 #pragma unroll
             for (int mt = 0; mt < TB / 16; mt++) {
@@ -608,8 +619,7 @@ attn_kv8_kernel(const Args a) {
         }
         __syncwarp();                                       // every lane has read the stage: refill it
         if (it + ST < n_my) {
-            const int next = tile + ST * stride;
-            load_tile<KIND>(cur, a, page_at(trow, next / PARTS, a.max_pages), next % PARTS, kvh, lane);
+            load_tile<KIND>(cur, a, page_ahead, (tile + ST * stride) % PARTS, kvh, lane);
         }
         cp_async_commit();
         stage = stage + 1 == ST ? 0 : stage + 1;
@@ -658,6 +668,15 @@ attn_kv8_kernel(const Args a) {
             o.x = fmaf(p.x, e, o.x); o.y = fmaf(p.y, e, o.y); o.z = fmaf(p.z, e, o.z); o.w = fmaf(p.w, e, o.w);
         }
         *(float4*)(cpart + r * OD + d) = o;
+    }
+    if (a.shares > 1) {                                      // (each thread stores what it has added up)
+        for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += NW * 32) {
+            const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+            const long long at = ((packed0 + (row0 + r) / G) * a.H + kvh * G + (row0 + r) % G) * a.shares + share;
+            *(float4*)(a.own_o + at * HD + d) = *(const float4*)(cpart + r * OD + d);
+            if (d == 0) *(float2*)(a.own_ml + at * 2) = *(const float2*)(cpart + r * OD + HD);
+        }
+        return;
     }
     if (CR > 1) cluster_sync_all();
     else __syncthreads();
@@ -719,7 +738,7 @@ template <int KIND, int NT, int NW, int ST>
 int launch(const Args& a, long long rows, int n_seqs, cudaStream_t st) {
     auto kernel = attn_kv8_kernel<KIND, NT, NW, ST>;
     constexpr size_t smem = (size_t)NW * ST * Tile<KIND>::BYTES;
-    const long long x = (rows + 8 * NT - 1) / (8 * NT) * a.cluster;
+    const long long x = (rows + 8 * NT - 1) / (8 * NT) * a.cluster * a.shares;
     if (x > 0x7fffffffLL || a.KVH > 65535 || n_seqs > 65535) return OE_ERR_UNSUPPORTED;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
@@ -769,16 +788,19 @@ int oe_kv8_write(int kind, const bf16* qkv, long long stride, const float* cos_t
 
 // Attention of the step's tokens over their sequences' caches (kind: OE_KV_*).  write != 0: every sequence brings one token, whose
 // key and value this kernel writes.  With seq_pages the pages before a sequence's own are left out and the parts that
-// oe_attn_rows_prefix left are added.
+// oe_attn_rows_prefix left are added.  shares > 1: as many CTAs share a tile's keys and leave their parts in own_o [T * H, shares, HD]
+// and own_ml [T * H, shares, 2] (oe_join_parts).
 int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, void* cache,
                 float* scales, int write, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
                 const int* seq_qlen, int n_seqs, int max_qlen, int H, int KVH, int window, float scale, int warps, int cluster,
-                int ordered, const int* seq_pages, int splits, const float* part_o, const float* part_ml, int ahead, cudaStream_t st) {
+                int ordered, const int* seq_pages, int splits, const float* part_o, const float* part_ml, int shares, float* own_o, float* own_ml, int ahead,
+                cudaStream_t st) {
     if (n_seqs <= 0 || max_qlen <= 0) return 0;
     if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15) ||
         ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15) || ((uintptr_t)out & 15)) return OE_ERR_UNSUPPORTED;
     if (cluster < 1 || cluster > 16 || (cluster & (cluster - 1)) || (write && max_qlen != 1)) return OE_ERR_UNSUPPORTED;
     if (seq_pages != nullptr && (window != 0 || max_qlen != 1 || splits < 1 || splits + cluster > MAX_JOINED || part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
+    if (shares < 1 || (shares > 1 && (cluster != 1 || seq_pages != nullptr || own_o == nullptr || own_ml == nullptr))) return OE_ERR_UNSUPPORTED;
     Args a = {};
     a.out = out; a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab;
     a.cache = cache; a.scales = scales;
@@ -786,6 +808,7 @@ int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const fl
     a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start; a.seq_qlen = seq_qlen;
     a.H = H; a.KVH = KVH; a.window = window; a.scale_log2 = scale * LOG2E; a.cluster = cluster;
     a.seq_pages = seq_pages; a.splits = splits; a.part_o = part_o; a.part_ml = part_ml; a.ahead = ahead;
+    a.shares = shares; a.own_o = own_o; a.own_ml = own_ml;
     a.ordered = ordered && window == 0 && n_seqs > 1 && n_seqs <= MAX_ORDERED ? n_seqs : 0;
     const long long rows = (long long)max_qlen * (H / KVH);
     if (kind == OE_KV_BF16) return launch_rows<OE_KV_BF16>(warps, a, rows, n_seqs, st);

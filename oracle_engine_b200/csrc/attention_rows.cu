@@ -16,7 +16,7 @@
 // weights are relative to R, the power of two above the largest value scale so far, and times 2^8 (what float16 cannot hold is
 // then below 2^-33 of a row's largest weight).  R grows for the whole CTA at once, with the rescaling of O.
 // bfloat16: K and V as they are (TMA); queries and weights are sums of two bfloat16, a second product each.
-// Roles (warps): 0 asks for the pages, 1 issues the products, 2 prepares the scales, 4-7 turn codes into float16 (8-bit forms),
+// Roles (warps): 0 asks for the pages, 1 issues the products, 2 prepares the scales, 4-11 turn codes into float16 (8-bit forms),
 // the last 4 MT load and turn the queries, then do the softmax and store.
 // Few tiles: the pages are cut into `splits` runs, whose parts (O, m, l) are joined by the kernel that runs next.
 // Every wait on an mbarrier is bounded in time; one that runs out raises an error flag, every role leaves its loop, copies in
@@ -65,7 +65,7 @@ struct Shape {
     static constexpr int K_AT = Q_ALL, V_AT = K_AT + STAGES * T_BYTES, RAW_AT = V_AT + STAGES * T_BYTES;
     static constexpr int CTL_AT = RAW_AT + (EIGHT ? RAW_STAGES * 2 * RAW : 0);
     static constexpr int BYTES = CTL_AT + (int)sizeof(Ctl);
-    static constexpr int CONVERT = EIGHT ? 4 : 0;                      // warps
+    static constexpr int CONVERT = EIGHT ? 8 : 0;                      // warps: four for keys, four for values
     static constexpr int FIRST = 4 + CONVERT;                          // the first softmax warp
     static constexpr int THREADS = (FIRST + 4 * MT) * 32;
     static constexpr uint32_t S_COLS = MT * 2 * BN, O_COLS = MT * HD;
@@ -233,6 +233,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*(uint64_t*)&d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b), "l"(*(uint64_t*)&c));
     return d;
 }
+// The registers of this warpgroup's threads from here on.
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <bool EIGHT>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     if (EIGHT) {
@@ -246,7 +249,7 @@ __device__ __forceinline__ uint32_t rest_bf16(float lo, float hi, uint32_t h) {
     return pack16<false>(lo - __uint_as_float(h << 16), hi - __uint_as_float(h & 0xffff0000u));
 }
 
-// Warps 4-7: a page's codes to the swizzled 16-bit tile.  A lane takes 16 codes at a time; the lanes of the second sub-tile store their
+// A page's codes to the swizzled 16-bit tile, by four warps.  A lane takes 16 codes at a time; the lanes of the second sub-tile store their
 // two pieces in the other order, so that 8 lanes fill 8 different bank groups.
 template <int KIND>
 __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* tile, int t) {
@@ -372,7 +375,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     const int* trow = a.tables + (size_t)b * a.max_pages;
     if (threadIdx.x == 0) {
         mbar_init(&ctl->q_full, MT * 4);
-        for (int s = 0; s < RAW_STAGES; s++) { mbar_init(&ctl->raw_full[s], 1); mbar_init(&ctl->raw_empty[s], 4); }
+        for (int s = 0; s < RAW_STAGES; s++) { mbar_init(&ctl->raw_full[s], 1); mbar_init(&ctl->raw_empty[s], 8); }
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&ctl->k_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->k_empty[s], 1);
             mbar_init(&ctl->v_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->v_empty[s], 1);
@@ -401,6 +404,10 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     const bool ahead = PREFIX && a.ahead;
     if (!ahead || warp >= Z::FIRST) pdl_wait();
 
+    // 8-bit forms: the launch gives every thread of the 3 + MT warpgroups 96 registers (two tiles) or 128 (one), 480 or 512 for a lane of
+    // each; the softmax needs more of them than the others: 80 + 56 + 56 + 2 * 144 = 480, 80 + 56 + 56 + 200 < 512
+    constexpr int SOFTMAX_REGISTERS = MT == 2 ? 144 : 200;
+    if (EIGHT && warp < 4) fewer_registers<80>();
     if (warp == 0) {
         // ---------------- the pages ----------------
         if (lane == 0) {
@@ -539,25 +546,23 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
             }
         }
     } else if (EIGHT && warp >= 4 && warp < Z::FIRST) {
-        // ---------------- codes to 16-bit tiles ----------------
-        const int t = threadIdx.x - 128;
+        // ---------------- codes to 16-bit tiles: four warps the keys', four the values' ----------------
+        fewer_registers<56>();
+        const int t = threadIdx.x & 127;
+        const bool values = warp >= 8;
+        uint64_t *full = values ? ctl->v_full : ctl->k_full, *empty = values ? ctl->v_empty : ctl->k_empty;
         for (int i = 0; i < any; i++) {
             const int s = i % STAGES, rs = i % RAW_STAGES;
-            const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
             if (!warp_wait(&ctl->raw_full[rs], (uint32_t)(i / RAW_STAGES) & 1u, ctl, 12)) break;
-            if (!warp_wait(&ctl->k_empty[s], ph ^ 1u, ctl, 13)) break;
-            convert_tile<KIND>(raw_s + rs * 2 * RAW, k_s + s * T_BYTES, t);
+            if (!warp_wait(&empty[s], ((uint32_t)(i / STAGES) & 1u) ^ 1u, ctl, 13)) break;
+            convert_tile<KIND>(raw_s + (rs * 2 + values) * RAW, (values ? v_s : k_s) + s * T_BYTES, t);
             fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->k_full[s]);
-            if (!warp_wait(&ctl->v_empty[s], ph ^ 1u, ctl, 14)) break;
-            convert_tile<KIND>(raw_s + rs * 2 * RAW + RAW, v_s + s * T_BYTES, t);
-            fence_async();
-            __syncwarp();
-            if (lane == 0) { mbar_arrive(&ctl->v_full[s]); mbar_arrive(&ctl->raw_empty[rs]); }
+            if (lane == 0) { mbar_arrive(&full[s]); mbar_arrive(&ctl->raw_empty[rs]); }
         }
     } else if (warp >= Z::FIRST) {
         // ---------------- queries, softmax, output: one row a thread ----------------
+        if (EIGHT) more_registers<SOFTMAX_REGISTERS>();
         const int tile = (warp - Z::FIRST) / 4, quarter = warp & 3;
         const int r = quarter * 32 + lane;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
@@ -797,31 +802,39 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     }
 }
 
-// The parts of a prompt's rows joined, in the order of the splits: a warp per row.
+// Rows' parts joined, in their order: a warp per row.
 __global__ void __launch_bounds__(256)
-join_parts_kernel(bf16* out, const float* part_o, const float* part_ml, long long rows, int splits) {
+join_parts_kernel(bf16* out, const float* part_o, const float* part_ml, long long rows, int n) {
     pdl_launch_dependents();
     pdl_wait();
     const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (r >= rows) return;
     constexpr int PER = HD / 32;
+    const float2* ml = (const float2*)part_ml + r * n;
     float m = -INFINITY;
-    for (int q = 0; q < splits; q++) m = fmaxf(m, part_ml[(r * splits + q) * 2]);
+    for (int q = lane; q < n; q += 32) m = fmaxf(m, ml[q].x);
+    m = warp_max(m);
     const float mu = m == -INFINITY ? 0.f : m;
     float o[PER] = {}, l = 0.f;
-    for (int q = 0; q < splits; q++) {
-        const float2 ml = *(const float2*)(part_ml + (r * splits + q) * 2);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;               // no key of this row: its O was not stored
-        const float w = exp2f(ml.x - mu);
-        l += ml.y * w;
-        const float* p = part_o + (r * splits + q) * HD + lane * PER;
+    for (int q0 = 0; q0 < n; q0 += 32) {
+        const float2 mine = q0 + lane < n ? ml[q0 + lane] : make_float2(-INFINITY, 0.f);
+        const bool none = mine.x == -INFINITY && mine.y == 0.f;             // no key of this row: its O was not stored
+        const float w = none ? -1.f : exp2f(mine.x - mu);
+        if (!none) l += mine.y * w;
+        const float* p = part_o + (r * n + q0) * HD + lane * PER;
+#pragma unroll 8
+        for (int q = 0; q < min(32, n - q0); q++) {
+            const float e = __shfl_sync(0xffffffffu, w, q);
+            if (e < 0.f) continue;
 #pragma unroll
-        for (int e = 0; e < PER; e++) o[e] += p[e] * w;
+            for (int x = 0; x < PER; x++) o[x] += p[q * HD + x] * e;
+        }
     }
+    l = warp_sum(l);
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
 #pragma unroll
-    for (int e = 0; e < PER; e += 2) *(uint32_t*)(out + r * HD + lane * PER + e) = pack16<false>(o[e] * inv, o[e + 1] * inv);
+    for (int x = 0; x < PER; x += 2) *(uint32_t*)(out + r * HD + lane * PER + x) = pack16<false>(o[x] * inv, o[x + 1] * inv);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
@@ -860,6 +873,13 @@ bool operands_ok(const Args& a, const void* cache) {
 
 extern "C" {
 
+// out [rows, HD] from each row's n parts: part_o [rows, n, HD] and part_ml [rows, n, 2].
+int oe_join_parts(bf16* out, const float* part_o, const float* part_ml, long long rows, int n, cudaStream_t st) {
+    if (rows <= 0) return 0;
+    if (n < 1 || (rows + 7) / 8 > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
+    return oe_launch(join_parts_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, out, part_o, part_ml, rows, n);
+}
+
 // Attention of the step's tokens over the 8-bit cache (kind OE_KV_INT8 or OE_KV_E4M3), which has their rows already.  mt: tiles of 128
 // rows a CTA has (1 or 2); splits > 1: the pages of a tile are cut into as many runs, whose parts go through part_o
 // [T * H, splits, HD] and part_ml [T * H, splits, 2].
@@ -884,9 +904,7 @@ int oe_attn_rows(int kind, bf16* out, const bf16* q, long long q_stride, const f
     if (kind == OE_KV_INT8) rc = launch_tiles<OE_KV_INT8, false>(mt, none, a, grid, st);
     else if (kind == OE_KV_E4M3) rc = launch_tiles<OE_KV_E4M3, false>(mt, none, a, grid, st);
     if (rc || splits == 1) return rc;
-    const long long rows = (long long)n_tokens * H;
-    return oe_launch(join_parts_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, out, (const float*)part_o, (const float*)part_ml,
-                     rows, splits);
+    return oe_join_parts(out, part_o, part_ml, (long long)n_tokens * H, splits, st);
 }
 
 // The parts of the groups' prefixes (see oe_attn_kv8_prefix) into part_o [B * H, splits, HD] and part_ml [B * H, splits, 2].

@@ -37,7 +37,7 @@ def _lib(head_dim: int):
         lib = _build.load("attention_kv8", {"OE_HD": head_dim})
         P, I, F, L = c_void_p, c_int, c_float, c_longlong
         lib.oe_kv8_write.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, I, P]
-        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, I, I, P, I, P, P, I, P]
+        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, I, I, P, I, P, P, I, P, P, I, P]
         lib.oe_kv8_write.restype = lib.oe_attn_kv8.restype = c_int
         _libs[head_dim] = lib
     return lib
@@ -50,6 +50,8 @@ def _rows_lib(head_dim: int):
         P, I, F, L = c_void_p, c_int, c_float, c_longlong
         lib.oe_attn_rows.argtypes = [I, P, P, L, P, P, P, P, L, P, I, P, P, P, I, I, I, I, I, I, F, I, I, P, P, P]
         lib.oe_attn_rows_prefix.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, F, P, P, P, I, I, I, I, P, P, I, P]
+        lib.oe_join_parts.argtypes = [P, P, P, L, I, P]
+        lib.oe_join_parts.restype = c_int
         lib.oe_attn_rows_error.argtypes = []
         lib.oe_attn_rows.restype = lib.oe_attn_rows_prefix.restype = lib.oe_attn_rows_error.restype = c_int
         _libs[("rows", head_dim)] = lib
@@ -152,13 +154,18 @@ def many_pairs(n_seqs: int, n_kv_heads: int, sm_count: int | None = None) -> boo
 
 
 def decode_form(n_seqs: int, n_kv_heads: int, context_class: int, sm_count: int | None = None) -> tuple:
-    """(warps of a CTA, CTAs (a thread-block cluster) that share the keys of one (sequence, KV head)) of a step of few rows."""
+    """(warps of a CTA, CTAs (a thread-block cluster) that share the keys of one (sequence, KV head), or CTAs that do so without being
+    a cluster) of a step of few rows."""
     sms = sm_count or ops.sm_count()
     pairs = n_seqs * n_kv_heads
-    for cr in (16, 8, 4, 2):
-        if context_class >= (1 if cr <= 4 else 2) and pairs * cr <= sms:
-            return 12, cr
-    return (12 if pairs <= sms else 4), 1
+    if context_class >= 3 and pairs * 8 <= sms:
+        return 12, 1, sms // pairs
+    if context_class >= 2 and pairs * 16 <= sms:
+        return 12, 8, 1
+    for cr in (4, 2):
+        if context_class >= 1 and pairs * cr <= sms:
+            return 12, cr, 1
+    return (12 if pairs <= sms else 4), 1, 1
 
 
 def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: int, scale: float,
@@ -185,12 +192,17 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
         kv8_write(qkv, cos, sin, cache, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
     few = max(1, ctx.max_qlen) * (n_heads // n_kv_heads) <= FEW_ROWS
     if single or few:
-        warps, cluster = form or decode_form(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0))
+        warps, cluster, shares = form or decode_form(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0))
+        part = _parts(T * n_heads, shares, head_dim, out.device) if shares > 1 else None
+        parts = _part_ptrs(part, T * n_heads, shares, head_dim)
         ops._check(_lib(head_dim).oe_attn_kv8(
             kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(),
             int(has_kv and single), codes.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
             ctx.seq_qlen.data_ptr(), ctx.n_seqs, 1 if single else max(1, ctx.max_qlen), n_heads, n_kv_heads, int(window), float(scale),
-            warps, cluster, int(many_pairs(ctx.n_seqs, n_kv_heads)), None, 0, None, None, int(ahead), ops._stream()), what, {"warps": warps, "cluster": cluster})
+            warps, cluster, int(many_pairs(ctx.n_seqs, n_kv_heads)), None, 0, None, None, shares, *parts, int(ahead), ops._stream()),
+            what, {"warps": warps, "cluster": cluster, "shares": shares})
+        if shares > 1:
+            ops._check(_rows_lib(head_dim).oe_join_parts(out.data_ptr(), *parts, T * n_heads, shares, ops._stream()), "join_parts")
         return
     mt, splits = form or prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
     part = _parts(T * n_heads, splits, head_dim, out.device) if splits > 1 else None
@@ -273,4 +285,4 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     ops._check(_lib(head_dim).oe_attn_kv8(
         kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), int(has_kv),
         *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 4, 1, int(many_pairs(B, n_kv_heads)), prefix.seq_pages.data_ptr(), splits,
-        *parts, int(ahead), ops._stream()), what)
+        *parts, 1, None, None, int(ahead), ops._stream()), what)

@@ -79,7 +79,7 @@ def test_single_tokens(H, KVH, hd, dtype, window):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("form", [(4, 1), (12, 1), (4, 2), (12, 4), (4, 8), (12, 16)])
+@pytest.mark.parametrize("form", [(4, 1, 1), (12, 1, 1), (4, 2, 1), (12, 4, 1), (4, 8, 1), (12, 8, 1), (4, 1, 7), (12, 1, 40)])
 def test_single_tokens_of_long_sequences(dtype, form):
     s = Step([0, 3000, 1279, 2111], [1] * 4, 6, 2, 128, dtype, seed=6, peaked=3.0)
     want, tol, cache = s.truth()
@@ -178,7 +178,7 @@ def test_strided_rows_no_rotation_another_stream_and_a_graph():
 
 def test_the_same_bits_every_time():
     s = Step([3000, 17, 900], [1, 1, 1], 24, 8, 128, torch.float8_e4m3fn, seed=14)
-    got = [s.out(form=(12, 4)) for _ in range(4)]
+    got = [s.out(form=(12, 4, 1)) for _ in range(4)]
     assert all(torch.equal(got[0], o) for o in got)
 
 
@@ -223,7 +223,7 @@ def test_refusals_on_the_device():
         with pytest.raises(KernelError):
             s.out()
     s = Step([10], [1], 4, 2, 64, torch.int8, seed=18)
-    for form in ((4, 0), (4, 3), (12, 32), (5, 1)):
+    for form in ((4, 0, 1), (4, 3, 1), (12, 32, 1), (5, 1, 1), (4, 2, 2), (4, 1, 0)):
         with pytest.raises(KernelError):
             s.out(form=form)
     with pytest.raises(KernelError):

@@ -62,8 +62,8 @@ def test_split_and_cluster_rules():
     for n in (1, 2, 7, 64, 500):
         for kvh in (1, 2, 8):
             for cls in range(4):
-                warps, c = ops_kv8.decode_form(n, kvh, cls, 148)
-                assert warps in (4, 12) and c in (1, 2, 4, 8, 16) and (c == 1 or n * kvh * c <= 148)
+                warps, c, shares = ops_kv8.decode_form(n, kvh, cls, 148)
+                assert warps in (4, 12) and c in (1, 2, 4, 8) and shares >= 1 and (c == 1 or shares == 1) and (c == 1 or n * kvh * c <= 148)
             for pages in (1, 5, 500):
                 mt, splits = ops_kv8.prefix_form(n, 1, 4, kvh, pages, 148)
                 assert mt in (1, 2) and 1 <= splits <= pages

@@ -38,6 +38,7 @@ constexpr int BM = 128, BN = OE_PAGE, SUB = HD / 64;
 constexpr int Q_BYTES = BM * HD * 2;             // SUB sub-tiles of [128][64] 16-bit values
 constexpr int T_BYTES = BN * HD * 2;             // K or V of a page, SUB sub-tiles of [64][64] 16-bit values
 constexpr int RAW = BN * HD;                     // codes of a page's K or V
+static_assert(OE_PAGE == 64, "a block of keys is a page");
 constexpr int STAGES = 2, RAW_STAGES = 4, SC_SLOTS = 6;
 constexpr float RESCALE_STEP = 7.f, LOG2E = 1.4426950408889634f;
 constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
@@ -199,9 +200,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
           "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
+// (no "memory": loads of the scales may move across it; tmem_st_wait orders it)
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -216,6 +218,11 @@ __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 // Two float32 at once.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -457,46 +464,44 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         const uint64_t q_desc = umma_desc(smem_u32(q_s), 16, 1024), k_desc = umma_desc(smem_u32(k_s), 16, 1024);
         const uint64_t v_desc = umma_desc(smem_u32(v_s), BN * 128, 1024);
         bool ok = warp_wait(&ctl->q_full, 0, ctl, 3);
-        auto issue_s = [&](int i) {                          // S_i of every tile that has page i, into its buffer i & 1
-            const int s = i % STAGES;
-            const uint64_t kd = k_desc + (uint64_t)(s * (T_BYTES >> 4));
+        auto issue_s = [&](int t, int i) {                   // S_i of tile t, into its buffer i & 1
+            const uint64_t kd = k_desc + (uint64_t)(i % STAGES * (T_BYTES >> 4));
+            const uint32_t d = tmem_base + (uint32_t)((t * 2 + (i & 1)) * BN);
             if (elect_one()) {
 #pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    if (i >= n_blocks[t]) continue;
-                    const uint32_t d = tmem_base + (uint32_t)((t * 2 + (i & 1)) * BN);
+                for (int h = 0; h < (EIGHT ? 1 : 2); h++) {
+                    const uint64_t qd = q_desc + (uint64_t)((t * (EIGHT ? 1 : 2) + h) * (Q_BYTES >> 4));
 #pragma unroll
-                    for (int h = 0; h < (EIGHT ? 1 : 2); h++) {
-                        const uint64_t qd = q_desc + (uint64_t)((t * (EIGHT ? 1 : 2) + h) * (Q_BYTES >> 4));
-#pragma unroll
-                        for (int k = 0; k < HD / 16; k++) {
-                            const uint32_t sb = k / 4, kk = k % 4;
-                            umma(d, qd + (uint64_t)((sb * (BM * 128) + kk * 32) >> 4), kd + (uint64_t)((sb * (BN * 128) + kk * 32) >> 4),
-                                 idesc_s, (k > 0 || h > 0) ? 1u : 0u);
-                        }
+                    for (int k = 0; k < HD / 16; k++) {
+                        const uint32_t sb = k / 4, kk = k % 4;
+                        umma(d, qd + (uint64_t)((sb * (BM * 128) + kk * 32) >> 4), kd + (uint64_t)((sb * (BN * 128) + kk * 32) >> 4),
+                             idesc_s, (k > 0 || h > 0) ? 1u : 0u);
                     }
-                    umma_commit(&ctl->s_full[t][i & 1]);
                 }
-                umma_commit(&ctl->k_empty[s]);
+                umma_commit(&ctl->s_full[t][i & 1]);
             }
             __syncwarp();
         };
-        if (ok && any > 0) {
-            ok = warp_wait(&ctl->k_full[0], 0, ctl, 4);
+        auto release = [&](uint64_t* bar) {                  // when everything issued so far is done
+            if (elect_one()) umma_commit(bar);
+            __syncwarp();
+        };
+        // A tile's S of page i + 2 is issued right behind its P V of page i, whose buffer it takes: neither waits for the other tile.
+        for (int i = 0; i < min(any, 2) && ok; i++) {
+            ok = warp_wait(&ctl->k_full[i % STAGES], (uint32_t)(i / STAGES) & 1u, ctl, 4);
             fence_after();
-            if (ok) issue_s(0);
+            if (!ok) break;
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+                if (i < n_blocks[t]) issue_s(t, i);
+            release(&ctl->k_empty[i % STAGES]);
         }
         for (int i = 0; i < any && ok; i++) {
-            if (i + 1 < any) {
-                ok = warp_wait(&ctl->k_full[(i + 1) % STAGES], (uint32_t)((i + 1) / STAGES) & 1u, ctl, 4);
-                if (!ok) break;
-                fence_after();
-                issue_s(i + 1);
-            }
             const int s = i % STAGES;
             ok = warp_wait(&ctl->v_full[s], (uint32_t)(i / STAGES) & 1u, ctl, 5);
             if (!ok) break;
             const uint64_t vd = v_desc + (uint64_t)(s * (T_BYTES >> 4));
+            bool keys = false;                               // page i + 2's are there
 #pragma unroll
             for (int t = 0; t < MT; t++) {
                 if (i >= n_blocks[t] || !ok) continue;
@@ -516,9 +521,17 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                     if (i == n_blocks[t] - 1) umma_commit(&ctl->o_done[t]);
                 }
                 __syncwarp();
+                if (i + 2 < n_blocks[t]) {
+                    if (!keys) ok = warp_wait(&ctl->k_full[s], (uint32_t)((i + 2) / STAGES) & 1u, ctl, 4);
+                    if (!ok) continue;
+                    keys = true;
+                    fence_after();
+                    issue_s(t, i + 2);
+                }
             }
-            if (ok && elect_one()) umma_commit(&ctl->v_empty[s]);
-            __syncwarp();
+            if (!ok) break;
+            release(&ctl->v_empty[s]);
+            if (i + 2 < any) release(&ctl->k_empty[s]);
         }
     } else if (warp == 2) {
         // ---------------- the scales: relative to R, and what R grew by ----------------
@@ -701,7 +714,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 for (int k = 0; k < BN; k++) s[k] = some && (unsigned)(k - lo) <= span ? s[k] : -INFINITY;
             }
 #pragma unroll
-            for (int k = 0; k < BN; k++) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
+            for (int k = 0; k < BN; k += 2) mx4[k / 2 & 3] = max3(mx4[k / 2 & 3], s[k], s[k + 1]);
             const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale);
             if (i == 0) {
                 m_run = m_new;

@@ -57,6 +57,7 @@ struct Ctl {
     uint64_t s_full[2][2], p_ready[2][2], pv_done[2], o_done[2];
     uint32_t tmem_base;
     int abort_flag;
+    float up[2 * BM];                            // what a row of queries was divided by
 };
 
 template <int KIND, int MT>
@@ -381,7 +382,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     }
     const int* trow = a.tables + (size_t)b * a.max_pages;
     if (threadIdx.x == 0) {
-        mbar_init(&ctl->q_full, MT * 4);
+        mbar_init(&ctl->q_full, Z::CONVERT + MT * 4);
         for (int s = 0; s < RAW_STAGES; s++) { mbar_init(&ctl->raw_full[s], 1); mbar_init(&ctl->raw_empty[s], 8); }
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&ctl->k_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->k_empty[s], 1);
@@ -409,8 +410,97 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     pdl_launch_dependents();
     // prefixes: where the caller says so, the pages are asked for before the wait; the queries come from the kernel before
     const bool ahead = PREFIX && a.ahead;
-    if (!ahead || warp >= Z::FIRST) pdl_wait();
+    if (!ahead || warp >= 4) pdl_wait();
 
+    // The queries, turned, by all warps from 4 on: HD / 16 lanes have a row, 8 dimensions of its lower half and the 8 that they are
+    // turned with each.  Several rows' pieces are asked for before the first is used: the start of a CTA is these loads.
+    if (warp >= 4) {
+        constexpr int PER = HD / 16, AT_ONCE = 32 / PER, WARPS = Z::CONVERT + 4 * MT, GROUPS = MT * BM / AT_ONCE;
+        constexpr int ROUND = EIGHT && MT == 2 ? 2 : GROUPS / WARPS >= 4 ? 4 : (GROUPS + WARPS - 1) / WARPS;     // (two: what 96 registers hold)
+        const int d = lane % PER * 8;
+        for (int g0 = warp - 4; g0 < GROUPS; g0 += ROUND * WARPS) {
+            uint4 u[ROUND], v[ROUND];
+            int pos[ROUND];
+#pragma unroll
+            for (int k = 0; k < ROUND; k++) {
+                const int rr = (g0 + k * WARPS) * AT_ONCE + lane / PER, tile = rr / BM, r = rr % BM, tok = t0 + tile * tpt + r / G;
+                u[k] = v[k] = make_uint4(0u, 0u, 0u, 0u);
+                pos[k] = 0;
+                if (g0 + k * WARPS < GROUPS && r < tpt * G && tok < count) {
+                    long long at;
+                    if (PREFIX) {
+                        const int sq = a.members[a.first[blockIdx.y] + tok];
+                        at = a.cu_q[sq];
+                        pos[k] = a.seq_start[sq];
+                    } else {
+                        at = a.cu_q[b] + tok;
+                        pos[k] = start + tok;
+                    }
+                    const bf16* src = a.q + at * a.q_stride + (long long)(kvh * G + r % G) * HD + d;
+                    u[k] = *(const uint4*)src;
+                    v[k] = *(const uint4*)(src + HD / 2);
+                }
+            }
+            float cs[ROUND][8], sn[ROUND][8];
+            if (a.cos_tab != nullptr) {
+#pragma unroll
+                for (int k = 0; k < ROUND; k++) {
+#pragma unroll
+                    for (int j = 0; j < 8; j += 4) {
+                        *(float4*)&cs[k][j] = *(const float4*)(a.cos_tab + (long long)pos[k] * (HD / 2) + d + j);
+                        *(float4*)&sn[k][j] = *(const float4*)(a.sin_tab + (long long)pos[k] * (HD / 2) + d + j);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < ROUND; k++) {
+                if (g0 + k * WARPS >= GROUPS) break;         // (the warp's)
+                const int rr = (g0 + k * WARPS) * AT_ONCE + lane / PER, tile = rr / BM, r = rr % BM;
+                const uint32_t uw[4] = {u[k].x, u[k].y, u[k].z, u[k].w}, vw[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                float x[2][8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[0][e] = kv8_from_bits((uw[e / 2] >> (16 * (e & 1))) & 0xffffu);
+                    x[1][e] = kv8_from_bits((vw[e / 2] >> (16 * (e & 1))) & 0xffffu);
+                }
+                if (a.cos_tab != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float lo = x[0][e], hi = x[1][e];
+                        x[0][e] = lo * cs[k][e] - hi * sn[k][e];
+                        x[1][e] = lo * sn[k][e] + hi * cs[k][e];
+                    }
+                }
+                float down = 1.f, up = 1.f;
+                if (EIGHT) {
+                    float most = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, fmaxf(fabsf(x[0][e]), fabsf(x[1][e])));
+#pragma unroll
+                    for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    down = kv8_row_factor(most, &up);
+                }
+                if (d == 0) ctl->up[rr] = up;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int dim = d + half * (HD / 2);
+                    uint32_t w[4], rest[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float q0 = x[half][2 * e] * down, q1 = x[half][2 * e + 1] * down;
+                        w[e] = pack16<EIGHT>(q0, q1);
+                        if (!EIGHT) rest[e] = rest_bf16(q0, q1, w[e]);
+                    }
+                    uint8_t* to = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES + (dim / 64) * (BM * 128) + r * 128 + ((((dim % 64) / 8) ^ (r & 7)) << 4);
+                    *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (!EIGHT) *(uint4*)(to + Q_BYTES) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                }
+            }
+        }
+        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->q_full);
+    }
     // 8-bit forms: the launch gives every thread of the 3 + MT warpgroups 96 registers (two tiles) or 128 (one), 480 or 512 for a lane of
     // each; the softmax needs more of them than the others: 80 + 56 + 56 + 2 * 144 = 480, 80 + 56 + 56 + 200 < 512
     constexpr int SOFTMAX_REGISTERS = MT == 2 ? 144 : 200;
@@ -598,82 +688,15 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 part = row * a.H + head;
             }
         }
-        float scale = a.scale_log2;
         const int nb = n_blocks[tile];
-        // The warp's 32 rows of queries, turned: HD / 16 lanes have a row, 8 dimensions of its lower half and the 8 they are turned
-        // with each, so that a row's pieces are loaded together.
-        if (nb > 0) {
-            constexpr int PER = HD / 16, AT_ONCE = 32 / PER;
-            const int d = lane % PER * 8;
-            uint8_t* qt = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES;
-#pragma unroll 2
-            for (int k = 0; k < PER; k++) {
-                const int rl = k * AT_ONCE + lane / PER, rr = quarter * 32 + rl;        // this step's row
-                const bool there = __shfl_sync(0xffffffffu, (int)valid, rl) != 0;
-                const long long at = __shfl_sync(0xffffffffu, row, rl);
-                const int h = __shfl_sync(0xffffffffu, head, rl), ps = __shfl_sync(0xffffffffu, pos, rl);
-                float x[2][8];
-                if (there) {
-                    const bf16* src = a.q + at * a.q_stride + (long long)h * HD + d;
-                    const uint4 u = *(const uint4*)src, v = *(const uint4*)(src + HD / 2);
-                    const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[0][e] = kv8_from_bits((uw[e / 2] >> (16 * (e & 1))) & 0xffffu);
-                        x[1][e] = kv8_from_bits((vw[e / 2] >> (16 * (e & 1))) & 0xffffu);
-                    }
-                    if (a.cos_tab != nullptr) {
-                        const float* cs = a.cos_tab + (long long)ps * (HD / 2) + d;
-                        const float* sn = a.sin_tab + (long long)ps * (HD / 2) + d;
-#pragma unroll
-                        for (int j = 0; j < 8; j += 4) {
-                            const float4 c = *(const float4*)(cs + j), n = *(const float4*)(sn + j);
-                            const float cc[4] = {c.x, c.y, c.z, c.w}, nn[4] = {n.x, n.y, n.z, n.w};
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const float lo = x[0][j + e], hi = x[1][j + e];
-                                x[0][j + e] = lo * cc[e] - hi * nn[e];
-                                x[1][j + e] = lo * nn[e] + hi * cc[e];
-                            }
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[0][e] = x[1][e] = 0.f;
-                }
-                float down = 1.f;
-                if (EIGHT) {
-                    float most = 0.f, up;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) most = fmaxf(most, fmaxf(fabsf(x[0][e]), fabsf(x[1][e])));
-#pragma unroll
-                    for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    down = kv8_row_factor(most, &up);
-                    const float mine = __shfl_sync(0xffffffffu, up, lane % AT_ONCE * PER);
-                    if (lane / AT_ONCE == k) scale *= mine;
-                }
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const int dim = d + half * (HD / 2);
-                    uint32_t w[4], rest[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float q0 = x[half][2 * e] * down, q1 = x[half][2 * e + 1] * down;
-                        w[e] = pack16<EIGHT>(q0, q1);
-                        if (!EIGHT) rest[e] = rest_bf16(q0, q1, w[e]);
-                    }
-                    uint8_t* to = qt + (dim / 64) * (BM * 128) + rr * 128 + ((((dim % 64) / 8) ^ (rr & 7)) << 4);
-                    *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
-                    if (!EIGHT) *(uint4*)(to + Q_BYTES) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-                }
-            }
-            fence_async();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->q_full);
-        float m_run = -INFINITY, l_run = 0.f, ref = 1.f;
         bool ok = true;
-        for (int i = 0; i < nb; i++) {
+        float scale = a.scale_log2;
+        if (nb > 0) {
+            ok = warp_wait(&ctl->q_full, 0, ctl, 17);
+            scale *= ctl->up[tile * BM + r];
+        }
+        float m_run = -INFINITY, l_run = 0.f, ref = 1.f;
+        for (int i = 0; i < nb && ok; i++) {
             const int c = i % SC_SLOTS;
             const Scales* sc = &ctl->sc[c];
             if (EIGHT) ok = mbar_wait(&ctl->sc_ready[c], (uint32_t)(i / SC_SLOTS) & 1u, ctl, 15);
@@ -764,41 +787,37 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 ok = __all_sync(0xffffffffu, ok);
                 fence_after();
             }
-            if (ok && (PREFIX || a.splits > 1)) {
-                float* po = a.part_o + (part * a.splits + split) * HD;
-                if (nb > 0) {
-#pragma unroll
-                    for (int c0 = 0; c0 < HD; c0 += 16) {
-                        float ob[16];
-                        tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
-                        tmem_ld_wait();
-                        if (valid) {
-#pragma unroll
-                            for (int e = 0; e < 16; e += 4)
-                                *(float4*)(po + c0 + e) = make_float4(ob[e] * ref, ob[e + 1] * ref, ob[e + 2] * ref, ob[e + 3] * ref);
-                        }
-                    }
-                }
-                if (valid) *(float2*)(a.part_ml + (part * a.splits + split) * 2) = make_float2(m_run, l_run);
-            } else if (ok && nb > 0) {
-                const float inv = l_run > 0.f ? ref / l_run : l_run == 0.f ? 0.f : l_run;
-                bf16* dst = a.out + row * (long long)(a.H * HD) + (long long)head * HD;
-#pragma unroll
-                for (int c0 = 0; c0 < HD; c0 += 16) {
-                    float ob[16];
+            if (ok && nb > 0) {
+                // 32 columns of the warp's rows at a time go through the tile of its queries, which nothing reads any more, so that a row's
+                // values are stored side by side
+                const bool parts = PREFIX || a.splits > 1;
+                const float f = parts ? ref : l_run > 0.f ? ref / l_run : l_run == 0.f ? 0.f : l_run;
+                uint8_t* stage = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES + quarter * (32 * 128);
+                const long long to = parts ? (part * a.splits + split) * HD : row * (long long)(a.H * HD) + (long long)head * HD;
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    float ob[32];
                     tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
+                    tmem_ld16_nowait(o_addr + (uint32_t)(c0 + 16), ob + 16);
                     tmem_ld_wait();
-                    if (valid) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 8) {
-                            uint32_t w[4];
+                    for (int c = 0; c < 8; c++)
+                        *(float4*)(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(ob[4 * c] * f, ob[4 * c + 1] * f, ob[4 * c + 2] * f, ob[4 * c + 3] * f);
+                    __syncwarp();
 #pragma unroll
-                            for (int x = 0; x < 4; x++) w[x] = pack16<false>(ob[e + 2 * x] * inv, ob[e + 2 * x + 1] * inv);
-                            *(uint4*)(dst + c0 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int k = 0; k < 8; k++) {
+                        const int rl = k * 4 + lane / 8, c = lane % 8;
+                        const float4 x = *(const float4*)(stage + rl * 128 + ((c ^ (rl & 7)) << 4));
+                        const long long at = __shfl_sync(0xffffffffu, to, rl) + c0 + c * 4;
+                        if (__shfl_sync(0xffffffffu, (int)valid, rl)) {
+                            if (parts) *(float4*)(a.part_o + at) = x;
+                            else *(uint2*)(a.out + at) = make_uint2(pack16<false>(x.x, x.y), pack16<false>(x.z, x.w));
                         }
                     }
+                    __syncwarp();
                 }
             }
+            if (ok && valid && (PREFIX || a.splits > 1)) *(float2*)(a.part_ml + (part * a.splits + split) * 2) = make_float2(m_run, l_run);
         }
         fence_before();
     }

@@ -720,12 +720,16 @@ attn_kv8_kernel(const Args a) {
             o.x = fmaf(p.x, w[q], o.x); o.y = fmaf(p.y, w[q], o.y); o.z = fmaf(p.z, w[q], o.z); o.w = fmaf(p.w, w[q], o.w);
         }
         const float* pre = a.part_o + (((long long)b * a.H + h) * a.splits) * HD + d;
-#pragma unroll 8
-        for (int q = 0; q < n_pre; q++) {
-            const float e = w[CR + q];
-            if (e < 0.f) continue;
-            const float4 p = *(const float4*)(pre + q * HD);
-            o.x = fmaf(p.x, e, o.x); o.y = fmaf(p.y, e, o.y); o.z = fmaf(p.z, e, o.z); o.w = fmaf(p.w, e, o.w);
+        for (int q = 0; q < n_pre; q += 8) {                // (eight at a time, whether they count or not: their loads overlap)
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = *(const float4*)(pre + min(q + k, n_pre - 1) * HD);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float e = q + k < n_pre ? w[CR + q + k] : -1.f;
+                if (e < 0.f) continue;
+                o.x = fmaf(v[k].x, e, o.x); o.y = fmaf(v[k].y, e, o.y); o.z = fmaf(v[k].z, e, o.z); o.w = fmaf(v[k].w, e, o.w);
+            }
         }
         const float inv = w[MAX_JOINED];
         *(uint2*)(a.out + (packed0 + (row0 + r) / G) * (long long)(a.H * HD) + (long long)h * HD + d) =
@@ -740,29 +744,27 @@ int launch(const Args& a, long long rows, int n_seqs, cudaStream_t st) {
     constexpr size_t smem = (size_t)NW * ST * Tile<KIND>::BYTES;
     const long long x = (rows + 8 * NT - 1) / (8 * NT) * a.cluster * a.shares;
     if (x > 0x7fffffffLL || a.KVH > 65535 || n_seqs > 65535) return OE_ERR_UNSUPPORTED;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    const dim3 grid((unsigned)x, a.KVH, n_seqs);
-    if (a.cluster > 8) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static Kv8Devices set;
+    if (set.first()) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
+        set.done();
     }
+    const dim3 grid((unsigned)x, a.KVH, n_seqs);
     if (a.cluster > 1) return oe_launch_cluster(kernel, (unsigned)a.cluster, grid, dim3(NW * 32), smem, st, a);
     return oe_launch(kernel, grid, dim3(NW * 32), smem, st, a);
 }
-// warps: 12 (a CTA has an SM to itself) or 4 (three an SM).
+// warps: 12 (a CTA has an SM to itself) or 4 (three an SM); of a 16-bit cache, whose tiles are twice as large, 6 or 3.
 template <int KIND, int NT>
 int launch_form(int warps, const Args& a, long long rows, int n_seqs, cudaStream_t st) {
-    if (warps == 12) return launch<KIND, NT, 12, 2>(a, rows, n_seqs, st);
-    if (warps == 4) return launch<KIND, NT, 4, 2>(a, rows, n_seqs, st);
+    constexpr int MANY = KIND == OE_KV_BF16 ? 6 : 12, FEW = KIND == OE_KV_BF16 ? 3 : 4;
+    if (warps == MANY) return launch<KIND, NT, MANY, 2>(a, rows, n_seqs, st);
+    if (warps == FEW) return launch<KIND, NT, FEW, 2>(a, rows, n_seqs, st);
     return OE_ERR_UNSUPPORTED;
 }
 template <int KIND>
 int launch_rows(int warps, const Args& a, long long rows, int n_seqs, cudaStream_t st) {
-    if constexpr (KIND == OE_KV_BF16)
-        return rows <= 8 ? launch<KIND, 1, 3, 2>(a, rows, n_seqs, st) : launch<KIND, 2, 3, 2>(a, rows, n_seqs, st);
-    else
-        return rows <= 8 ? launch_form<KIND, 1>(warps, a, rows, n_seqs, st) : launch_form<KIND, 2>(warps, a, rows, n_seqs, st);
+    return rows <= 8 ? launch_form<KIND, 1>(warps, a, rows, n_seqs, st) : launch_form<KIND, 2>(warps, a, rows, n_seqs, st);
 }
 
 }  // namespace
@@ -798,7 +800,7 @@ int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const fl
     if (n_seqs <= 0 || max_qlen <= 0) return 0;
     if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15) ||
         ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15) || ((uintptr_t)out & 15)) return OE_ERR_UNSUPPORTED;
-    if (cluster < 1 || cluster > 16 || (cluster & (cluster - 1)) || (write && max_qlen != 1)) return OE_ERR_UNSUPPORTED;
+    if (cluster < 1 || cluster > 8 || (cluster & (cluster - 1)) || (write && max_qlen != 1)) return OE_ERR_UNSUPPORTED;
     if (seq_pages != nullptr && (window != 0 || max_qlen != 1 || splits < 1 || splits + cluster > MAX_JOINED || part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
     if (shares < 1 || (shares > 1 && (cluster != 1 || seq_pages != nullptr || own_o == nullptr || own_ml == nullptr))) return OE_ERR_UNSUPPORTED;
     Args a = {};

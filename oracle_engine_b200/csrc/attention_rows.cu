@@ -418,27 +418,41 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         constexpr int PER = HD / 16, AT_ONCE = 32 / PER, WARPS = Z::CONVERT + 4 * MT, GROUPS = MT * BM / AT_ONCE;
         constexpr int ROUND = EIGHT && MT == 2 ? 2 : GROUPS / WARPS >= 4 ? 4 : (GROUPS + WARPS - 1) / WARPS;     // (two: what 96 registers hold)
         const int d = lane % PER * 8;
-        for (int g0 = warp - 4; g0 < GROUPS; g0 += ROUND * WARPS) {
+        // where the rows are, of all rounds
+        constexpr int ALL = (GROUPS + WARPS - 1) / WARPS;
+        const bf16* src[ALL];
+        int pos_of[ALL];
+#pragma unroll
+        for (int k = 0; k < ALL; k++) {
+            const int g = warp - 4 + k * WARPS, rr = g * AT_ONCE + lane / PER, r = rr % BM, tok = t0 + rr / BM * tpt + r / G;
+            src[k] = nullptr;
+            pos_of[k] = 0;
+            if (g < GROUPS && r < tpt * G && tok < count) {
+                long long at;
+                if (PREFIX) {
+                    const int sq = a.members[a.first[blockIdx.y] + tok];
+                    at = a.cu_q[sq];
+                    pos_of[k] = a.seq_start[sq];
+                } else {
+                    at = a.cu_q[b] + tok;
+                    pos_of[k] = start + tok;
+                }
+                src[k] = a.q + at * a.q_stride + (long long)(kvh * G + r % G) * HD + d;
+            }
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < ALL; k0 += ROUND) {
+            const int g0 = warp - 4 + k0 * WARPS;
             uint4 u[ROUND], v[ROUND];
             int pos[ROUND];
 #pragma unroll
             for (int k = 0; k < ROUND; k++) {
-                const int rr = (g0 + k * WARPS) * AT_ONCE + lane / PER, tile = rr / BM, r = rr % BM, tok = t0 + tile * tpt + r / G;
+                const bf16* from = k0 + k < ALL ? src[k0 + k < ALL ? k0 + k : 0] : nullptr;
+                pos[k] = k0 + k < ALL ? pos_of[k0 + k < ALL ? k0 + k : 0] : 0;
                 u[k] = v[k] = make_uint4(0u, 0u, 0u, 0u);
-                pos[k] = 0;
-                if (g0 + k * WARPS < GROUPS && r < tpt * G && tok < count) {
-                    long long at;
-                    if (PREFIX) {
-                        const int sq = a.members[a.first[blockIdx.y] + tok];
-                        at = a.cu_q[sq];
-                        pos[k] = a.seq_start[sq];
-                    } else {
-                        at = a.cu_q[b] + tok;
-                        pos[k] = start + tok;
-                    }
-                    const bf16* src = a.q + at * a.q_stride + (long long)(kvh * G + r % G) * HD + d;
-                    u[k] = *(const uint4*)src;
-                    v[k] = *(const uint4*)(src + HD / 2);
+                if (from != nullptr) {
+                    u[k] = *(const uint4*)from;
+                    v[k] = *(const uint4*)(from + HD / 2);
                 }
             }
             float cs[ROUND][8], sn[ROUND][8];
@@ -793,7 +807,11 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 const bool parts = PREFIX || a.splits > 1;
                 const float f = parts ? ref : l_run > 0.f ? ref / l_run : l_run == 0.f ? 0.f : l_run;
                 uint8_t* stage = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES + quarter * (32 * 128);
-                const long long to = parts ? (part * a.splits + split) * HD : row * (long long)(a.H * HD) + (long long)head * HD;
+                const long long mine = parts ? (part * a.splits + split) * HD : row * (long long)(a.H * HD) + (long long)head * HD;
+                const uint32_t there = __ballot_sync(0xffffffffu, valid);
+                long long to[8];                            // of the rows whose values this lane stores
+#pragma unroll
+                for (int k = 0; k < 8; k++) to[k] = __shfl_sync(0xffffffffu, mine, k * 4 + lane / 8) + lane % 8 * 4;
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD; c0 += 32) {
                     float ob[32];
@@ -808,10 +826,9 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                     for (int k = 0; k < 8; k++) {
                         const int rl = k * 4 + lane / 8, c = lane % 8;
                         const float4 x = *(const float4*)(stage + rl * 128 + ((c ^ (rl & 7)) << 4));
-                        const long long at = __shfl_sync(0xffffffffu, to, rl) + c0 + c * 4;
-                        if (__shfl_sync(0xffffffffu, (int)valid, rl)) {
-                            if (parts) *(float4*)(a.part_o + at) = x;
-                            else *(uint2*)(a.out + at) = make_uint2(pack16<false>(x.x, x.y), pack16<false>(x.z, x.w));
+                        if (there >> rl & 1u) {
+                            if (parts) *(float4*)(a.part_o + to[k] + c0) = x;
+                            else *(uint2*)(a.out + to[k] + c0) = make_uint2(pack16<false>(x.x, x.y), pack16<false>(x.z, x.w));
                         }
                     }
                     __syncwarp();
@@ -855,12 +872,20 @@ join_parts_kernel(bf16* out, const float* part_o, const float* part_ml, long lon
         const float w = none ? -1.f : exp2f(mine.x - mu);
         if (!none) l += mine.y * w;
         const float* p = part_o + (r * n + q0) * HD + lane * PER;
-#pragma unroll 8
-        for (int q = 0; q < min(32, n - q0); q++) {
-            const float e = __shfl_sync(0xffffffffu, w, q);
-            if (e < 0.f) continue;
+        const int here = min(32, n - q0);
+        for (int q = 0; q < here; q += 8) {                 // (eight at a time, whether they count or not: their loads overlap)
+            float v[8][PER];
 #pragma unroll
-            for (int x = 0; x < PER; x++) o[x] += p[q * HD + x] * e;
+            for (int k = 0; k < 8; k++) {
+#pragma unroll
+                for (int x = 0; x < PER; x += 2) *(float2*)&v[k][x] = *(const float2*)(p + min(q + k, here - 1) * HD + x);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float e = q + k < here ? __shfl_sync(0xffffffffu, w, q + k) : -1.f;
+#pragma unroll
+                for (int x = 0; x < PER; x++) o[x] = e < 0.f ? o[x] : o[x] + v[k][x] * e;
+            }
         }
     }
     l = warp_sum(l);
@@ -887,8 +912,12 @@ template <int KIND, bool PREFIX, int MT>
 int launch(const CUtensorMap& map, const Args& a, dim3 grid, cudaStream_t st) {
     using Z = Shape<KIND, MT>;
     const size_t smem = (size_t)Z::BYTES + 1024;
-    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<KIND, PREFIX, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
+    static Kv8Devices set;
+    if (set.first()) {
+        const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<KIND, PREFIX, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (int)e;
+        set.done();
+    }
     return oe_launch(attn_rows_kernel<KIND, PREFIX, MT>, grid, dim3(Z::THREADS), smem, st, map, a);
 }
 template <int KIND, bool PREFIX>

@@ -14,8 +14,17 @@
 // A row with an infinite or undefined value gets codes 0 and an undefined scale: it reads as undefined, and codes are always numbers.
 #pragma once
 #include "common.cuh"
+#include <atomic>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+// On which devices a kernel's attributes have been set (they are a device's; setting them again does no harm).
+struct Kv8Devices {
+    std::atomic<unsigned long long> bits{0};
+    static int current() { int d = 0; return cudaGetDevice(&d) == cudaSuccess && d < 64 ? d : -1; }
+    bool first() const { const int d = current(); return d < 0 || !(bits.load(std::memory_order_acquire) >> d & 1ull); }
+    void done() { const int d = current(); if (d >= 0) bits.fetch_or(1ull << d, std::memory_order_release); }
+};
 
 #define OE_KV_BF16 0
 #define OE_KV_INT8 1

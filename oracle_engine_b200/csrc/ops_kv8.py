@@ -74,15 +74,17 @@ def supported(head_dim: int, n_heads: int, n_kv_heads: int) -> bool:
 def _cache_args(what: str, cache, n_kv_heads: int, head_dim: int, allow_16: bool) -> tuple:
     """(kind, rows, scales or None) of a cache entry."""
     rows, scales = (cache, None) if isinstance(cache, torch.Tensor) else cache
-    if rows.dtype not in _KINDS or (scales is None) != (rows.dtype == torch.bfloat16):
+    kind = _KINDS.get(rows.dtype)
+    if kind is None or (scales is None) != (kind == 0):
         raise KernelError(f"{what}: a cache entry is (codes, scales) with int8 or float8_e4m3fn codes, or a bfloat16 tensor")
     if scales is None and not allow_16:
         raise KernelError(f"{what}: codes and scales expected")
-    if tuple(rows.shape[1:]) != (2, n_kv_heads, PAGE, head_dim) or not rows.is_contiguous():
+    shape = rows.shape
+    if len(shape) != 5 or shape[1] != 2 or shape[2] != n_kv_heads or shape[3] != PAGE or shape[4] != head_dim or not rows.is_contiguous():
         raise KernelError(f"{what}: cache entry must be contiguous [pages, 2, KVH, PAGE, head_dim]")
-    if scales is not None and (scales.dtype != torch.float32 or not scales.is_contiguous() or scales.shape != rows.shape[:-1]):
+    if scales is not None and (scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.shape != shape[:4]):
         raise KernelError(f"{what}: scales must be contiguous float32 [pages, 2, KVH, PAGE]")
-    return _KINDS[rows.dtype], rows, scales
+    return kind, rows, scales
 
 
 def _check_heads(what: str, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
@@ -92,33 +94,44 @@ def _check_heads(what: str, n_heads: int, n_kv_heads: int, head_dim: int) -> Non
 
 
 def _check_rows(what: str, qkv, cos, sin, width: int, head_dim: int) -> None:
-    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or qkv.stride(0) % 8 or \
+    if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or qkv.stride(0) % 8 or \
             qkv.data_ptr() % 16:
         raise KernelError(f"{what}: qkv must be bfloat16 [T, {width}] with rows of multiples of 16 bytes")
-    if (cos is None) != (sin is None) or cos is not None and (
-            cos.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != head_dim // 2 or not cos.is_contiguous()
-            or sin.dtype != torch.float32 or sin.shape != cos.shape or not sin.is_contiguous()):
-        raise KernelError(f"{what}: cos/sin must be contiguous float32 [max_pos, head_dim/2]")
+    if cos is None and sin is None:
+        return
+    for t in (cos, sin):
+        if t is None or t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] != head_dim // 2 or not t.is_contiguous() or \
+                t.data_ptr() % 16:
+            raise KernelError(f"{what}: cos/sin must be contiguous float32 [max_pos, head_dim/2]")
+    if cos.shape[0] != sin.shape[0]:
+        raise KernelError(f"{what}: cos and sin must have equally many rows")
+
+
+def _check_ints(what: str, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
 
 
 def _here(what: str, *tensors) -> None:
     """Every tensor is on the current device, whose stream the kernel is launched on."""
-    ops._dev(*tensors)
-    dev = torch.cuda.current_device()
+    if tensors[0].get_device() < 0:
+        ops._dev(*tensors)
+    dev = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and t.device.index != dev:
+        if t is not None and t.get_device() != dev:
+            ops._dev(t)
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
 
 
 def _check_step(what: str, out, qkv, cos, tables, ctx, n_heads: int, head_dim: int) -> None:
-    for t, n in ((tables, "tables"), (ctx.cu_q, "cu_q"), (ctx.seq_start, "seq_start"), (ctx.seq_qlen, "seq_qlen")):
-        ops._i32(t, f"{what}: {n}")
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != (qkv.shape[0], n_heads * head_dim) or not out.is_contiguous():
+    n, longest = ctx.n_seqs, getattr(ctx, "max_kvlen", 0)
+    _check_ints(what, tables=tables, cu_q=ctx.cu_q, seq_start=ctx.seq_start, seq_qlen=ctx.seq_qlen)
+    if out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != qkv.shape[0] or out.shape[1] != n_heads * head_dim or \
+            not out.is_contiguous() or out.data_ptr() % 16:
         raise KernelError(f"{what}: out must be contiguous bfloat16 [T, {n_heads * head_dim}]")
-    if tables.dim() != 2 or tables.shape[0] < ctx.n_seqs or ctx.cu_q.numel() < ctx.n_seqs + 1 or \
-            ctx.seq_start.numel() < ctx.n_seqs or ctx.seq_qlen.numel() < ctx.n_seqs:
-        raise KernelError(f"{what}: the step's tables are shorter than its {ctx.n_seqs} sequences")
-    longest = getattr(ctx, "max_kvlen", 0)
+    if tables.dim() != 2 or tables.shape[0] < n or ctx.cu_q.numel() <= n or ctx.seq_start.numel() < n or ctx.seq_qlen.numel() < n:
+        raise KernelError(f"{what}: the step's tables are shorter than its {n} sequences")
     if longest > tables.shape[1] * PAGE or cos is not None and longest > cos.shape[0]:
         raise KernelError(f"{what}: a sequence of {longest} tokens is longer than its page table or the position tables")
 
@@ -136,8 +149,7 @@ def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
     _here(what, qkv, cos, sin, codes, scales, tables, tok_seq, tok_pos)
     _check_rows(what, qkv, cos, sin, (n_heads + 2 * n_kv_heads) * head_dim, head_dim)
-    for t, n in ((tables, "tables"), (tok_seq, "tok_seq"), (tok_pos, "tok_pos")):
-        ops._i32(t, f"{what}: {n}")
+    _check_ints(what, tables=tables, tok_seq=tok_seq, tok_pos=tok_pos)
     T = qkv.shape[0]
     if tables.dim() != 2 or tok_seq.numel() < T or tok_pos.numel() < T:
         raise KernelError(f"{what}: fewer places than the {T} tokens")
@@ -247,6 +259,13 @@ def prefix_form(n_members: int, n_groups: int, group: int, n_kv_heads: int, max_
     return mt, max(1, min(max_pages, sms // ctas, MAX_SPLITS))
 
 
+def own_form(n_seqs: int, n_kv_heads: int, eight: bool, sm_count: int | None = None) -> tuple:
+    """(warps of a CTA, CTAs of a cluster) for the keys behind the prefixes."""
+    sms = sm_count or ops.sm_count()
+    pairs = n_seqs * n_kv_heads
+    return (12 if eight else 6) if pairs <= sms else (4 if eight else 3), 2 if pairs * 2 <= sms else 1
+
+
 def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                      has_kv: bool = True, ahead: bool = False) -> None:
     """A step of one token a sequence in which groups of sequences begin with the same pages: rotation, cache write (has_kv) and
@@ -267,14 +286,15 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     B = ctx.n_seqs
     if not ctx.all_decode or qkv.shape[0] != B:
         raise KernelError(f"{what}: one token a sequence expected")
+    _check_ints(what, members=prefix.members, first=prefix.first, pages=prefix.pages, seq_pages=prefix.seq_pages)
     for t, n, least in zip(lists, ("members", "first", "pages", "seq_pages"), (prefix.n_members, prefix.n_groups + 1, prefix.n_groups, B)):
-        ops._i32(t, f"{what}: {n}")
         if t.numel() < least:
             raise KernelError(f"{what}: {n} holds {t.numel()} numbers, {least} are needed")
     if B == 0:
         return
     step = (rows.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr())
     mt, splits = prefix_form(max(1, prefix.n_members), max(1, prefix.n_groups), n_heads // n_kv_heads, n_kv_heads, max(1, prefix.max_pages))
+    warps, cluster = own_form(B, n_kv_heads, scales is not None)
     part = _parts(B * n_heads, splits, head_dim, out.device)
     parts = _part_ptrs(part, B * n_heads, splits, head_dim)
     if prefix.n_groups > 0 and prefix.n_members > 0:
@@ -284,5 +304,6 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
             prefix.n_members, mt, splits, *parts, int(ahead), ops._stream()), "attention_shared_prefix", {"tiles": mt, "splits": splits})
     ops._check(_lib(head_dim).oe_attn_kv8(
         kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), int(has_kv),
-        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), 4, 1, int(many_pairs(B, n_kv_heads)), prefix.seq_pages.data_ptr(), splits,
+        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), warps, cluster,
+        int(many_pairs(B, n_kv_heads)), prefix.seq_pages.data_ptr(), splits,
         *parts, 1, None, None, int(ahead), ops._stream()), what)

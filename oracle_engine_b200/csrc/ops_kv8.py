@@ -250,24 +250,21 @@ def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context
     return mt, max(1, min(sms // ctas, pages // 4, 16))
 
 
-def prefix_form(n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, sm_count: int | None = None) -> tuple:
-    """(tiles of 128 rows a CTA has, runs that a prefix's pages are cut into)."""
+def shared_form(n_seqs: int, n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, eight: bool,
+                sm_count: int | None = None) -> tuple:
+    """(tiles of 128 rows a CTA has, runs that a prefix's pages are cut into; warps of a CTA and CTAs of a cluster for the keys behind
+    the prefixes)."""
     sms = sm_count or ops.sm_count()
     tiles = -(-n_members // (TILE_ROWS // group))
-    mt = 2 if tiles > 1 else 1
-    ctas = (-(-tiles // mt) + n_groups - 1) * n_kv_heads
-    return mt, max(1, min(max_pages, sms // ctas, MAX_SPLITS))
-
-
-def own_form(n_seqs: int, n_kv_heads: int, eight: bool, sm_count: int | None = None) -> tuple:
-    """(warps of a CTA, CTAs of a cluster) for the keys behind the prefixes."""
-    sms = sm_count or ops.sm_count()
+    mt = 2 if tiles * n_kv_heads > sms else 1
+    ctas = max(-(-tiles // mt), n_groups) * n_kv_heads          # (groups of equal size)
     pairs = n_seqs * n_kv_heads
-    return (12 if eight else 6) if pairs <= sms else (4 if eight else 3), 2 if pairs * 2 <= sms else 1
+    return (mt, max(1, min(max_pages, sms // ctas, MAX_SPLITS)),
+            (12 if eight else 6) if pairs <= sms else (4 if eight else 3), 2 if pairs * 2 <= sms else 1)
 
 
 def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
-                     has_kv: bool = True, ahead: bool = False) -> None:
+                     has_kv: bool = True, ahead: bool = False, form: tuple | None = None) -> None:
     """A step of one token a sequence in which groups of sequences begin with the same pages: rotation, cache write (has_kv) and
     attention over all keys, as attention_kv8 with window 0, but a group's common pages are read once for all of its members.
     cache: the 8-bit pair or the 16-bit entry.
@@ -275,7 +272,8 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     prefix: n_groups and n_members (host numbers, or bounds for them: what first and members hold beyond the real ones are
     groups without members), max_pages (the most pages a group has in common), and int32 tensors members (sequences in the order of
     their groups), first [n_groups + 1] (where each group's members begin), pages [n_groups] (full pages that the group's
-    tables begin with), seq_pages [n_seqs] (those of the sequence's group, 0 for a sequence in none)."""
+    tables begin with), seq_pages [n_seqs] (those of the sequence's group, 0 for a sequence in none).
+    form: the kernels' form; None: by shared_form."""
     what = "attention_shared"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
     kind, rows, scales = _cache_args(what, cache, n_kv_heads, head_dim, True)
@@ -293,8 +291,8 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     if B == 0:
         return
     step = (rows.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr())
-    mt, splits = prefix_form(max(1, prefix.n_members), max(1, prefix.n_groups), n_heads // n_kv_heads, n_kv_heads, max(1, prefix.max_pages))
-    warps, cluster = own_form(B, n_kv_heads, scales is not None)
+    mt, splits, warps, cluster = form or shared_form(
+        B, max(1, prefix.n_members), max(1, prefix.n_groups), n_heads // n_kv_heads, n_kv_heads, max(1, prefix.max_pages), scales is not None)
     part = _parts(B * n_heads, splits, head_dim, out.device)
     parts = _part_ptrs(part, B * n_heads, splits, head_dim)
     if prefix.n_groups > 0 and prefix.n_members > 0:

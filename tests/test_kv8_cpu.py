@@ -65,8 +65,10 @@ def test_split_and_cluster_rules():
                 warps, c, shares = ops_kv8.decode_form(n, kvh, cls, 148)
                 assert warps in (4, 12) and c in (1, 2, 4, 8) and shares >= 1 and (c == 1 or shares == 1) and (c == 1 or n * kvh * c <= 148)
             for pages in (1, 5, 500):
-                mt, splits = ops_kv8.prefix_form(n, 1, 4, kvh, pages, 148)
-                assert mt in (1, 2) and 1 <= splits <= pages
+                for eight in (False, True):
+                    mt, splits, warps, c = ops_kv8.shared_form(n, n, 1, 4, kvh, pages, eight, 148)
+                    assert mt in (1, 2) and 1 <= splits <= min(pages, ops_kv8.MAX_SPLITS) and c in (1, 2)
+                    assert warps in ((4, 12) if eight else (3, 6))
             for tokens in (1, 40, 5000):
                 mt, splits = ops_kv8.prompt_form(tokens, n, 4, kvh, cls, 0, 148)
                 assert mt in (1, 2) and 1 <= splits <= 16

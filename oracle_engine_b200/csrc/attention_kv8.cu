@@ -321,17 +321,17 @@ attn_kv8_kernel(const Args a) {
         __syncthreads();
         b = which;
     }
-    const int row0 = bx * ROWS, qlen = a.seq_qlen[b], n_rows = qlen > 0 ? qlen * G : 0;
+    // (the step's integers, asked for together; they were written before its first kernel)
+    const int qlen = a.seq_qlen[b], start = a.seq_start[b], common = a.seq_pages != nullptr ? a.seq_pages[b] : 0;
+    const long long packed0 = a.cu_q[b];
+    const int row0 = bx * ROWS, n_rows = qlen > 0 ? qlen * G : 0;
     if (row0 >= n_rows) {                                            // the whole cluster
         pdl_wait();
         return;
     }
-    const int start = a.seq_start[b];
-    const long long packed0 = a.cu_q[b];
     const int rows = min(ROWS, n_rows - row0);
     int key_lo = oe_first_key(start + row0 / G, a.window);
     const int key_hi = start + (row0 + rows - 1) / G;
-    const int common = a.seq_pages != nullptr ? a.seq_pages[b] : 0;
     key_lo = max(key_lo, common * OE_PAGE);
     const int* trow = a.tables + (size_t)b * a.max_pages;
     uint8_t* mine = smem + (size_t)warp * WARP_BYTES;
@@ -343,6 +343,28 @@ attn_kv8_kernel(const Args a) {
     // come from the kernel before this one
     const bool ahead = a.ahead && own_kv;
     if (!ahead) pdl_wait();
+    // The queries of the rows nt * 8 + gid, 4 dimensions that lie together a k-step, and their angles: asked for before the tiles where
+    // the kernel before this one has been waited for, since a score needs both.
+    uint2 qw[NT][KS];
+    float4 qc[NT][KS / 2], qs[NT][KS / 2];
+    auto ask_for_queries = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int r = nt * 8 + gid, rr = row0 + (r < rows ? r : 0);
+            const bf16* src = a.q + (packed0 + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * HD + tig * 4;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) qw[nt][ks] = r < rows ? *(const uint2*)(src + ks * 16) : make_uint2(0u, 0u);
+            if (a.cos_tab != nullptr) {
+                const size_t at = (size_t)(start + rr / G) * (HD / 2) + tig * 4;
+#pragma unroll
+                for (int ks = 0; ks < KS / 2; ks++) {
+                    qc[nt][ks] = *(const float4*)(a.cos_tab + at + ks * 16);
+                    qs[nt][ks] = *(const float4*)(a.sin_tab + at + ks * 16);
+                }
+            }
+        }
+    };
+    if (!ahead) ask_for_queries();
     // the page numbers of this warp's next 32 tiles, one a lane, and of the 32 behind them
     auto pages_from = [&](int it) { return it + lane < n_my ? page_at(trow, (t_lo + gw + (it + lane) * stride) / PARTS, a.max_pages) : -1; };
     int pages = pages_from(0), pages_next = pages_from(32);
@@ -352,29 +374,27 @@ attn_kv8_kernel(const Args a) {
         if (pre < n_my) load_tile<KIND>(mine + pre * L::BYTES, a, page, (t_lo + gw + pre * stride) % PARTS, kvh, lane);
         cp_async_commit();
     }
-    if (ahead) pdl_wait();
-
-    // Q fragments, turned, of the rows nt * 8 + gid: qf, and for a 16-bit cache what its rounding leaves; a row's power of two
+    if (ahead) {
+        pdl_wait();
+        ask_for_queries();
+    }
+    // Q fragments, turned: qf, and for a 16-bit cache what its rounding leaves; a row's power of two
     constexpr int KL = EIGHT ? 1 : KS;
     uint32_t qf[NT][KS][2], ql[NT][KL][2];
     float up[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int r = nt * 8 + gid, rr = row0 + (r < rows ? r : 0), pos = start + rr / G;
-        const bf16* src = a.q + (packed0 + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * HD + tig * 4;
         float qv[KS][4];
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            const uint2 w = r < rows ? *(const uint2*)(src + ks * 16) : make_uint2(0u, 0u);
-            qv[ks][0] = kv8_from_bits(w.x & 0xffffu); qv[ks][1] = kv8_from_bits(w.x >> 16);
-            qv[ks][2] = kv8_from_bits(w.y & 0xffffu); qv[ks][3] = kv8_from_bits(w.y >> 16);
+            const uint2 w = qw[nt][ks];
+            qv[ks][0] = kv8_from_bits(w.x); qv[ks][1] = __uint_as_float(w.x & 0xffff0000u);
+            qv[ks][2] = kv8_from_bits(w.y); qv[ks][3] = __uint_as_float(w.y & 0xffff0000u);
         }
         if (a.cos_tab != nullptr) {
 #pragma unroll
             for (int ks = 0; ks < KS / 2; ks++) {
-                const float4 c = *(const float4*)(a.cos_tab + (size_t)pos * (HD / 2) + ks * 16 + tig * 4);
-                const float4 n = *(const float4*)(a.sin_tab + (size_t)pos * (HD / 2) + ks * 16 + tig * 4);
-                const float cc[4] = {c.x, c.y, c.z, c.w}, nn[4] = {n.x, n.y, n.z, n.w};
+                const float cc[4] = {qc[nt][ks].x, qc[nt][ks].y, qc[nt][ks].z, qc[nt][ks].w}, nn[4] = {qs[nt][ks].x, qs[nt][ks].y, qs[nt][ks].z, qs[nt][ks].w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float x = qv[ks][e], y = qv[ks + KS / 2][e];
@@ -655,9 +675,14 @@ attn_kv8_kernel(const Args a) {
         const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - mu);
         const float l = warp_sum(w == 0.f && ml.y == 0.f ? 0.f : ml.y * w);
         if (lane < NW) wts[r * WT + lane] = w;
-        if (lane == 0) *(float2*)(cpart + r * OD + HD) = make_float2(m, l);
+        if (lane == 0) {
+            *(float2*)(cpart + r * OD + HD) = make_float2(m, l);
+            wts[r * WT + MAX_JOINED] = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        }
     }
     __syncthreads();
+    const int n_pre = common > 0 ? a.splits : 0;
+    const bool alone = CR == 1 && a.shares == 1 && n_pre == 0;           // nothing to join: the sum is the result
     for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += NW * 32) {
         const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -667,8 +692,15 @@ attn_kv8_kernel(const Args a) {
             const float4 p = *(const float4*)(part + ((size_t)w * ROWS + r) * OD + d);
             o.x = fmaf(p.x, e, o.x); o.y = fmaf(p.y, e, o.y); o.z = fmaf(p.z, e, o.z); o.w = fmaf(p.w, e, o.w);
         }
-        *(float4*)(cpart + r * OD + d) = o;
+        if (alone) {
+            const float inv = wts[r * WT + MAX_JOINED];
+            *(uint2*)(a.out + (packed0 + (row0 + r) / G) * (long long)(a.H * HD) + (long long)(kvh * G + (row0 + r) % G) * HD + d) =
+                make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        } else {
+            *(float4*)(cpart + r * OD + d) = o;
+        }
     }
+    if (alone) return;
     if (a.shares > 1) {                                      // (each thread stores what it has added up)
         for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += NW * 32) {
             const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
@@ -681,7 +713,6 @@ attn_kv8_kernel(const Args a) {
     if (CR > 1) cluster_sync_all();
     else __syncthreads();
     // this CTA's share of the rows' results: the cluster's sums in rank order, then the prefix's parts
-    const int n_pre = common > 0 ? a.splits : 0;
     for (int r = warp; r < rows; r += NW) {
         const int h = kvh * G + (row0 + r) % G;
         const float2* pre_ml = (const float2*)a.part_ml + ((long long)b * a.H + h) * a.splits;

@@ -250,6 +250,17 @@ def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context
     return mt, max(1, min(sms // ctas, pages // 4, 16))
 
 
+def sharing_pays(groups: list, eight: bool) -> bool:
+    """Whether a step's groups, (members, pages in common) each, are read faster by attention_shared than sequence by sequence, where
+    the common pages come out of the L2 for all but the first.  us, attention_shared / sequence by sequence, 24 heads over 8 KV
+    heads of 128, 100 keys behind a prefix of 1,024 / 2,048 / 4,096 / 8,192 tokens, 16-bit cache: 2 members 17/7, 19/9, 21/14, 27/22; 4
+    18/8, 19/13, 21/21, 27/38; 8 19/12, 20/20, 22/36, 28/66; 16 18/13, 19/21, 22/37, 28/67; 32 21/19, 23/33, 27/60, 32/115; 64 36/35,
+    38/66, 42/119, 50/226.  8-bit: 2 17/10, 19/13, 21/14, 25/17; 4 17/10, 19/14, 21/17, 26/26; 8 18/13, 20/16, 22/25, 27/40; 16 17/14,
+    19/22, 21/38, 26/69; 32 18/22, 20/38, 22/67, 27/128; 64 29/44, 31/73, 37/133, 46/252."""
+    base = 256 if eight else 768
+    return sum(members * (pages * PAGE - base) for members, pages in groups if pages * PAGE > base) >= 16384
+
+
 def shared_form(n_seqs: int, n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, eight: bool,
                 sm_count: int | None = None) -> tuple:
     """(tiles of 128 rows a CTA has, runs that a prefix's pages are cut into; warps of a CTA and CTAs of a cluster for the keys behind

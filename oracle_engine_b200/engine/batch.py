@@ -19,6 +19,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
+from ..csrc import ops_kv8
 from ..csrc.ops import SCAN_CHUNK
 
 
@@ -127,16 +128,17 @@ class SharedPrefixes:
         return self.n_groups, self.n_members, self.max_pages
 
 
-def shared_prefixes(marks: list, pad_seqs: int) -> SharedPrefixes | None:
+def shared_prefixes(marks: list, pad_seqs: int, eight: bool = False) -> SharedPrefixes | None:
     """marks: per sequence the cache's (mark, pages) or None (cache/kv_cache.py: fork).  Groups are sequences with the same mark,
-    two at least; None if there is no group.  The host numbers are rounded up to few different ones, so that a captured step
+    two at least; None if there is no group, or if reading the common pages apart is not worth it (ops_kv8.sharing_pays; eight: an
+    8-bit cache).  The host numbers are rounded up to few different ones, so that a captured step
     serves many."""
     groups: dict = {}
     for b, m in enumerate(marks):
         if m is not None:
             groups.setdefault(m, []).append(b)
     groups = {m: bs for m, bs in groups.items() if len(bs) > 1}
-    if not groups:
+    if not groups or not ops_kv8.sharing_pays([(len(bs), n) for (_, n), bs in groups.items()], eight):
         return None
     up = lambda n: 1 << max(0, n - 1).bit_length()                       # noqa: E731
     n_groups = up(len(groups))

@@ -175,7 +175,7 @@ class Stepper:
     def _prefixes(self, seqs, pad_seqs: int):
         """Which sequences of a step of single tokens begin with the same pages, or None."""
         marks = [self.cache.prefix[s.slot] for s in seqs]
-        return shared_prefixes(marks, pad_seqs) if any(m is not None for m in marks) else None
+        return shared_prefixes(marks, pad_seqs, self.rt.cache_codes is not None) if any(m is not None for m in marks) else None
 
     def _step_eager(self, seqs, starts, device_tokens=None, token_arrays=None):
         plan = build_plan(seqs, starts, token_arrays=token_arrays)

@@ -39,6 +39,17 @@ def rounded(monkeypatch):
     return use
 
 
+@pytest.fixture
+def always_share(monkeypatch):
+    """Steps read common pages apart however short they are."""
+    from oracle_engine_b200.csrc import ops_kv8
+    calls = []
+    inner = ops_kv8.attention_shared
+    monkeypatch.setattr(ops_kv8, "sharing_pays", lambda groups, eight: True)
+    monkeypatch.setattr(ops_kv8, "attention_shared", lambda *a, **kw: (calls.append(1), inner(*a, **kw)))
+    return calls
+
+
 def _logits(engine, slot, tokens, portions):
     """Logits of every token, the tokens taken in portions of these sizes (the last size again and again)."""
     from oracle_engine_b200 import SequenceStep
@@ -112,7 +123,7 @@ def test_chunks_and_layers_that_read_another_s_cache(tmp_path, kind):
 
 @pytest.mark.parametrize("dtype,kind", [("float32", None), ("bfloat16", None), ("bfloat16", "int8"), ("bfloat16", "fp8")])
 @pytest.mark.parametrize("graphs", [True, False])
-def test_forks_go_on_as_if_alone(model_dirs, plain_models, rounded, dtype, kind, graphs):
+def test_forks_go_on_as_if_alone(model_dirs, plain_models, rounded, always_share, dtype, kind, graphs):
     """Two bases, forks of each, a fork of a fork and a sequence on its own decode in one step; forks come and go."""
     from oracle_engine_b200 import SequenceStep
     if kind:
@@ -159,6 +170,7 @@ def test_forks_go_on_as_if_alone(model_dirs, plain_models, rounded, dtype, kind,
     eng.cache.check()
     eng.check_device_errors()
     assert all(g.pool.n_free == g.pool.n for g in eng.cache.groups)
+    assert bool(always_share) == (dtype == "bfloat16")
 
 
 def test_forks_of_recurrent_layers_take_their_state(tmp_path):
@@ -179,7 +191,7 @@ def test_forks_of_recurrent_layers_take_their_state(tmp_path):
 
 @pytest.mark.parametrize("dtype,kind", [("float32", None), ("bfloat16", None), ("bfloat16", "int8"), ("bfloat16", "fp8")])
 @pytest.mark.parametrize("portion", [None, 50])
-def test_generation_with_common_beginnings(model_dirs, plain_models, rounded, dtype, kind, portion):
+def test_generation_with_common_beginnings(model_dirs, plain_models, rounded, always_share, dtype, kind, portion):
     from oracle_engine_b200 import GenParams
     if kind:
         rounded(kind)

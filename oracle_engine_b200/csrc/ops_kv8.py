@@ -165,18 +165,31 @@ def many_pairs(n_seqs: int, n_kv_heads: int, sm_count: int | None = None) -> boo
     return n_seqs * n_kv_heads > 3 * (sm_count or ops.sm_count())
 
 
-def decode_form(n_seqs: int, n_kv_heads: int, context_class: int, sm_count: int | None = None) -> tuple:
+def decode_form(n_seqs: int, n_kv_heads: int, context_class: int, window: int = 0, sm_count: int | None = None) -> tuple:
     """(warps of a CTA, CTAs (a thread-block cluster) that share the keys of one (sequence, KV head), or CTAs that do so without being
-    a cluster) of a step of few rows."""
+    a cluster) of a step of few rows.
+
+    Short contexts: a CTA a pair, of twelve warps, which fill an SM's shared memory, while the pairs have an SM each, else of four.
+    Longer ones: CTAs of four warps, which leave room on their SMs for the products that overlap them; up to 8 of a cluster, and
+    for very long ones as many as fill the SMs twice and leave parts for another kernel.  ms a decode step of the 28-layer model with 24
+    heads over 8 KV heads of 128, int8:  1 sequence of 2,000 keys 12x1 1.83, 12x4 1.63, 12x8 1.58, 4x8 1.64; of 8,000 12x8 1.78,
+    12x1x18 2.39, 4x1x18 1.74; of 32,000 12x8 2.46, 12x1x18 2.74, 4x1x18 2.29, 4x1x36 2.05;  4 of 2,000 12x2 1.79, 12x4 2.47, 4x4
+    1.79, of 8,000 12x2 2.43, 4x4 2.40;  8 of 512 12x1 1.66, 4x1 1.77, of 2,000 12x1 2.10, 12x2 2.46, 4x2 2.03, 4x4 1.90, of 8,000 12x1
+    3.40, 12x2 3.15, 4x4 2.52;  16 of 2,000 12x1 2.39, 4x1 2.64, 4x2 2.32;  32 of 1,000 12x1 2.94, 4x1 2.78."""
     sms = sm_count or ops.sm_count()
     pairs = n_seqs * n_kv_heads
+    if window and abs(window) <= 1536:             # no more than the second class of contexts is seen
+        context_class = min(context_class, 1 if abs(window) > 768 else 0)
     if context_class >= 3 and pairs * 8 <= sms:
-        return 12, 1, sms // pairs
-    if context_class >= 2 and pairs * 16 <= sms:
-        return 12, 8, 1
-    for cr in (4, 2):
-        if context_class >= 1 and pairs * cr <= sms:
-            return 12, cr, 1
+        return 4, 1, 2 * sms // pairs
+    if context_class >= 1:
+        if pairs * 16 <= sms:
+            return 12, 8, 1
+        for cr in (8, 4):
+            if pairs * cr <= sms * (1 if cr == 8 else 2):
+                return 4, cr, 1
+        if context_class >= 2 and pairs <= sms:
+            return 4, 2, 1
     return (12 if pairs <= sms else 4), 1, 1
 
 
@@ -204,7 +217,7 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
         kv8_write(qkv, cos, sin, cache, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
     few = max(1, ctx.max_qlen) * (n_heads // n_kv_heads) <= FEW_ROWS
     if single or few:
-        warps, cluster, shares = form or decode_form(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0))
+        warps, cluster, shares = form or decode_form(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
         part = _parts(T * n_heads, shares, head_dim, out.device) if shares > 1 else None
         parts = _part_ptrs(part, T * n_heads, shares, head_dim)
         ops._check(_lib(head_dim).oe_attn_kv8(
@@ -252,26 +265,31 @@ def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context
 
 def sharing_pays(groups: list, eight: bool) -> bool:
     """Whether a step's groups, (members, pages in common) each, are read faster by attention_shared than sequence by sequence, where
-    the common pages come out of the L2 for all but the first.  us, attention_shared / sequence by sequence, 24 heads over 8 KV
-    heads of 128, 100 keys behind a prefix of 1,024 / 2,048 / 4,096 / 8,192 tokens, 16-bit cache: 2 members 17/7, 19/9, 21/14, 27/22; 4
-    18/8, 19/13, 21/21, 27/38; 8 19/12, 20/20, 22/36, 28/66; 16 18/13, 19/21, 22/37, 28/67; 32 21/19, 23/33, 27/60, 32/115; 64 36/35,
-    38/66, 42/119, 50/226.  8-bit: 2 17/10, 19/13, 21/14, 25/17; 4 17/10, 19/14, 21/17, 26/26; 8 18/13, 20/16, 22/25, 27/40; 16 17/14,
-    19/22, 21/38, 26/69; 32 18/22, 20/38, 22/67, 27/128; 64 29/44, 31/73, 37/133, 46/252."""
+    the common pages come out of the L2 for all but the first.  Measured with 24 heads over 8 KV heads of 128, 100 keys behind the prefix.
+    ms a decode step of 28 layers, shared / apart, prefix of 4,096 tokens: 16-bit cache, 8 members 2.53 / 2.49, 16 2.29 / 2.74, 32 2.98 /
+    3.89, 64 3.48 / 5.61; int8, 8 2.07 / 2.12, 16 2.23 / 2.79, 32 2.85 / 4.10, 64 3.23 / 6.01.  us of the attention alone, prefixes of
+    1,024 / 2,048 / 4,096 / 8,192, 16-bit: 2 members 17/7, 19/9, 21/14, 27/22; 8 19/12, 20/20, 22/36, 28/66; 16 18/13, 19/21, 22/37, 28/67;
+    32 21/19, 23/33, 27/60, 32/115; 64 36/35, 38/66, 42/119, 50/226; int8: 2 17/10, 19/13, 21/14, 25/17; 8 18/13, 20/16, 22/25, 27/40; 16
+    17/14, 19/22, 21/38, 26/69; 32 18/22, 20/38, 22/67, 27/128; 64 29/44, 31/73, 37/133, 46/252."""
     base = 256 if eight else 768
-    return sum(members * (pages * PAGE - base) for members, pages in groups if pages * PAGE > base) >= 16384
+    return sum(members * (pages * PAGE - base) for members, pages in groups if pages * PAGE > base) >= 32768
 
 
 def shared_form(n_seqs: int, n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, eight: bool,
                 sm_count: int | None = None) -> tuple:
     """(tiles of 128 rows a CTA has, runs that a prefix's pages are cut into; warps of a CTA and CTAs of a cluster for the keys behind
-    the prefixes)."""
+    the prefixes).  One tile, so that there are fewer parts to join, unless the tiles alone outnumber the SMs (us, 64 members of 32
+    heads behind 8,192 tokens in 8 bits: two tiles and 18 runs 54.0, one tile and 9 runs 53.1; behind 2,048 44.0 / 39.8).  As many runs as
+    give every SM a CTA (16 members of 24 heads behind 4,096, ms a decode step of 28 layers: 18 runs 2.23, 9 2.41, 4 2.66).  Own keys: CTAs
+    of all an SM has room for while the pairs have an SM each (12 / 4 warps: 8 members 2.07 / 2.10, 32 2.99 / 2.85, 64 3.60 / 3.23), no
+    clusters (8 members, two CTAs of 12 warps a pair: 2.61)."""
     sms = sm_count or ops.sm_count()
     tiles = -(-n_members // (TILE_ROWS // group))
     mt = 2 if tiles * n_kv_heads > sms else 1
     ctas = max(-(-tiles // mt), n_groups) * n_kv_heads          # (groups of equal size)
     pairs = n_seqs * n_kv_heads
     return (mt, max(1, min(max_pages, sms // ctas, MAX_SPLITS)),
-            (12 if eight else 6) if pairs <= sms else (4 if eight else 3), 2 if pairs * 2 <= sms else 1)
+            (12 if eight else 6) if pairs <= sms else (4 if eight else 3), 1)
 
 
 def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,

@@ -62,8 +62,10 @@ def test_split_and_cluster_rules():
     for n in (1, 2, 7, 64, 500):
         for kvh in (1, 2, 8):
             for cls in range(4):
-                warps, c, shares = ops_kv8.decode_form(n, kvh, cls, 148)
-                assert warps in (4, 12) and c in (1, 2, 4, 8) and shares >= 1 and (c == 1 or shares == 1) and (c == 1 or n * kvh * c <= 148)
+                warps, c, shares = ops_kv8.decode_form(n, kvh, cls, 0, 148)
+                assert warps in (4, 12) and c in (1, 2, 4, 8) and shares >= 1 and (c == 1 or shares == 1)
+                assert c * shares == 1 or n * kvh * c * shares * warps <= 12 * 148
+                assert ops_kv8.decode_form(n, kvh, cls, 100, 148)[1:] == (1, 1)
             for pages in (1, 5, 500):
                 for eight in (False, True):
                     mt, splits, warps, c = ops_kv8.shared_form(n, n, 1, 4, kvh, pages, eight, 148)

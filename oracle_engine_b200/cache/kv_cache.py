@@ -204,7 +204,7 @@ class KVCache:
                 lo_page = g.need.first_position(cur) // PAGE          # oldest key the first new query reads
             first_needed_page[g.index] = lo_page
             row = g.tables[slot]
-            releasable = int(((row[:lo_page] >= 0).sum())) if lo_page else 0
+            releasable = g.pool.sole(row[:lo_page][row[:lo_page] >= 0].tolist()) if lo_page else 0
             want = int((row[lo_page:need_hi] < 0).sum())
             if want > g.pool.n_free + releasable:
                 raise CacheFull(f"cache group {g.index} ({g.need.kind}) has {g.pool.n_free} free pages, "

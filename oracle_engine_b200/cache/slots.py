@@ -96,6 +96,10 @@ class PagePool:
     def holders(self, page: int) -> int:
         return (1 + self._more.get(page, 0)) if page in self._used else 0
 
+    def sole(self, pages: list) -> int:
+        """How many of these pages in use would be free if one holder released each."""
+        return len(pages) - sum(1 for p in pages if p in self._more) if self._more else len(pages)
+
     def _drop(self, page: int) -> bool:
         """True if the page keeps a holder."""
         more = self._more.get(page, 0)

@@ -95,6 +95,24 @@ def test_a_page_reserved_beyond_the_length_is_not_shared():
     assert c.groups[0].tables[base][1] != c.groups[0].tables[kid][1]
 
 
+def test_what_others_hold_is_not_counted_as_room():
+    """A window that moves on gives its pages back, but a page that another sequence holds too does not become free by that."""
+    c = KVCache([attention_cache_need(1, 8, 64)], 64 * 4, 64 * 4, allocate=False, n_slots=3)
+    base = c.alloc_slot()
+    grow(c, base, 128)
+    kid = c.fork(base)
+    other = c.alloc_slot()
+    grow(c, other, 128)                     # every page of the pool is in use
+    before = (c.groups[0].tables.copy(), c.groups[0].pool.n_free, c.version)
+    with pytest.raises(CacheFull):
+        grow(c, kid, 64)
+    assert (c.groups[0].tables == before[0]).all() and (c.groups[0].pool.n_free, c.version) == before[1:]
+    c.check()
+    c.free_slot(base)
+    grow(c, kid, 64)
+    c.check()
+
+
 def test_marks_of_forks_at_other_lengths():
     c = KVCache([FULL], 64 * 30, 64 * 10, allocate=False, n_slots=8)
     base = c.alloc_slot()

@@ -98,6 +98,7 @@ class Stepper:
         # (padded tokens, batch size, wanted rows; context class, what the parts choose by the lengths) -> graph
         self._token_graphs: dict[tuple, _DecodeGraph] = {}
         self._eager_buffers: dict[tuple, StepBuffers] = {}
+        self._last_prefixes = None         # the last step's common beginnings: what they were made from, and they
         self.launch_counter = None         # set by the bench to count kernel launches
 
     # ------------------------------------------------------------------ helpers
@@ -175,7 +176,12 @@ class Stepper:
     def _prefixes(self, seqs, pad_seqs: int):
         """Which sequences of a step of single tokens begin with the same pages, or None."""
         marks = [self.cache.prefix[s.slot] for s in seqs]
-        return shared_prefixes(marks, pad_seqs, self.rt.cache_codes is not None) if any(m is not None for m in marks) else None
+        if not any(marks):
+            return None
+        key = (pad_seqs, marks)
+        if self._last_prefixes is None or self._last_prefixes[0] != key:      # the same sequences one token further: as before
+            self._last_prefixes = (key, shared_prefixes(marks, pad_seqs, self.rt.cache_codes is not None))
+        return self._last_prefixes[1]
 
     def _step_eager(self, seqs, starts, device_tokens=None, token_arrays=None):
         plan = build_plan(seqs, starts, token_arrays=token_arrays)

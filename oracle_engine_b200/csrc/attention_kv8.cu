@@ -600,8 +600,15 @@ attn_kv8_kernel(const Args a) {
                 for (int c = 0; c < HD / 32; c++) {
                     uint32_t f[2][4];                       // dims c * 32 + gid * 4 + {0, 1} and + {2, 3}
                     if (EIGHT) {
-                        const uint32_t w0 = *(const uint32_t*)(vr + c * 32), w1 = *(const uint32_t*)(vr + L::V_ROW + c * 32);
-                        const uint32_t w2 = *(const uint32_t*)(vr + 8 * L::V_ROW + c * 32), w3 = *(const uint32_t*)(vr + 9 * L::V_ROW + c * 32);
+                        uint32_t w0 = *(const uint32_t*)(vr + c * 32), w1 = *(const uint32_t*)(vr + L::V_ROW + c * 32);
+                        uint32_t w2 = *(const uint32_t*)(vr + 8 * L::V_ROW + c * 32), w3 = *(const uint32_t*)(vr + 9 * L::V_ROW + c * 32);
+                        if (KIND == OE_KV_E4M3 && mask) {      // (as below; every int8 code is a number)
+                            const int key = k0 + kk * 16 + tig * 2;
+                            if (key < key_lo || key > key_hi) w0 = 0u;
+                            if (key + 1 < key_lo || key + 1 > key_hi) w1 = 0u;
+                            if (key + 8 < key_lo || key + 8 > key_hi) w2 = 0u;
+                            if (key + 9 < key_lo || key + 9 > key_hi) w3 = 0u;
+                        }
                         constexpr uint32_t LOWER = KIND == OE_KV_INT8 ? 0x5410u : 0x5140u, UPPER = KIND == OE_KV_INT8 ? 0x7632u : 0x7362u;
                         const uint32_t x0 = kv8_prmt(w0, w1, LOWER), x1 = kv8_prmt(w0, w1, UPPER);
                         const uint32_t y0 = kv8_prmt(w2, w3, LOWER), y1 = kv8_prmt(w2, w3, UPPER);

@@ -258,14 +258,15 @@ __device__ __forceinline__ uint32_t rest_bf16(float lo, float hi, uint32_t h) {
 }
 
 // A page's codes to the swizzled 16-bit tile, by four warps.  A lane takes 16 codes at a time; the lanes of the second sub-tile store their
-// two pieces in the other order, so that 8 lanes fill 8 different bank groups.
-template <int KIND>
-__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* tile, int t) {
+// two pieces in the other order, so that 8 lanes fill 8 different bank groups.  SOME: keys from `keys` on become zeros.
+template <int KIND, bool SOME>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* tile, int t, int keys) {
     constexpr int PER_ROW = HD / 16;
 #pragma unroll
     for (int u = t; u < BN * PER_ROW; u += 128) {
         const int key = u / PER_ROW, g = u % PER_ROW;
-        const uint4 w = *(const uint4*)(raw + u * 16);
+        uint4 w = *(const uint4*)(raw + u * 16);
+        if (SOME && key >= keys) w = make_uint4(0u, 0u, 0u, 0u);
         const uint32_t in[4] = {kv8_word<KIND>(w.x), kv8_word<KIND>(w.y), kv8_word<KIND>(w.z), kv8_word<KIND>(w.w)};
         uint4 o[2];
         o[0] = make_uint4(kv8_pair<KIND>(in[0], 0), kv8_pair<KIND>(in[0], 2), kv8_pair<KIND>(in[1], 0), kv8_pair<KIND>(in[1], 2));
@@ -536,7 +537,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                     fence_async();                         // the slot's scales were written by threads before
                     long long kr = row_of(i, 0), vr = row_of(i, 1);
                     ctl->sc[c].mapped = kr >= 0;
-                    if (kr < 0) { kr = (long long)kvh * BN; vr = kr + (long long)a.KVH * BN; }      // any codes are numbers
+                    if (kr < 0) { kr = (long long)kvh * BN; vr = kr + (long long)a.KVH * BN; }      // (any rows: none of them counts)
                     mbar_expect_tx(&ctl->raw_full[s], 2 * RAW);
                     bulk_load(raw_s + s * 2 * RAW, a.codes + kr * HD, RAW, &ctl->raw_full[s]);
                     bulk_load(raw_s + s * 2 * RAW + RAW, a.codes + vr * HD, RAW, &ctl->raw_full[s]);
@@ -672,7 +673,15 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
             const int s = i % STAGES, rs = i % RAW_STAGES;
             if (!warp_wait(&ctl->raw_full[rs], (uint32_t)(i / RAW_STAGES) & 1u, ctl, 12)) break;
             if (!warp_wait(&empty[s], ((uint32_t)(i / STAGES) & 1u) ^ 1u, ctl, 13)) break;
-            convert_tile<KIND>(raw_s + (rs * 2 + values) * RAW, (values ? v_s : k_s) + s * T_BYTES, t);
+            // a value behind the last token may hold e4m3 codes that are no numbers, and a weight of 0 times that is not 0
+            int keys = BN;
+            if (KIND == OE_KV_E4M3 && values) {
+                if (*(volatile int*)&ctl->sc[i % SC_SLOTS].mapped == 0) keys = 0;
+                else if (!PREFIX) keys = start + count - (j_lo + i) * BN;
+            }
+            uint8_t* to = (values ? v_s : k_s) + s * T_BYTES;
+            if (KIND == OE_KV_E4M3 && keys < BN) convert_tile<KIND, true>(raw_s + (rs * 2 + values) * RAW, to, t, keys);
+            else convert_tile<KIND, false>(raw_s + (rs * 2 + values) * RAW, to, t, BN);
             fence_async();
             __syncwarp();
             if (lane == 0) { mbar_arrive(&full[s]); mbar_arrive(&ctl->raw_empty[rs]); }
@@ -851,14 +860,15 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     }
 }
 
-// Rows' parts joined, in their order: a warp per row.
+// Rows' parts joined, in their order: a warp per row.  The step's padding rows, from token *n_real on, have no parts.
 __global__ void __launch_bounds__(256)
-join_parts_kernel(bf16* out, const float* part_o, const float* part_ml, long long rows, int n) {
+join_parts_kernel(bf16* out, const float* part_o, const float* part_ml, const int* n_real, int H, long long rows, int n) {
     pdl_launch_dependents();
+    const long long real = (long long)*n_real * H;
     pdl_wait();
     const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (r >= rows) return;
+    if (r >= min(rows, real)) return;
     constexpr int PER = HD / 32;
     const float2* ml = (const float2*)part_ml + r * n;
     float m = -INFINITY;
@@ -934,11 +944,13 @@ bool operands_ok(const Args& a, const void* cache) {
 
 extern "C" {
 
-// out [rows, HD] from each row's n parts: part_o [rows, n, HD] and part_ml [rows, n, 2].
-int oe_join_parts(bf16* out, const float* part_o, const float* part_ml, long long rows, int n, cudaStream_t st) {
+// out [n_tokens * H, HD] from each row's n parts: part_o [n_tokens * H, n, HD] and part_ml [n_tokens * H, n, 2].  n_real (on the
+// device): how many of the tokens are real; the rows of the others are left as they are.
+int oe_join_parts(bf16* out, const float* part_o, const float* part_ml, const int* n_real, int n_tokens, int H, int n, cudaStream_t st) {
+    const long long rows = (long long)n_tokens * H;
     if (rows <= 0) return 0;
     if (n < 1 || (rows + 7) / 8 > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
-    return oe_launch(join_parts_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, out, part_o, part_ml, rows, n);
+    return oe_launch(join_parts_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, out, part_o, part_ml, n_real, H, rows, n);
 }
 
 // Attention of the step's tokens over the 8-bit cache (kind OE_KV_INT8 or OE_KV_E4M3), which has their rows already.  mt: tiles of 128
@@ -965,7 +977,7 @@ int oe_attn_rows(int kind, bf16* out, const bf16* q, long long q_stride, const f
     if (kind == OE_KV_INT8) rc = launch_tiles<OE_KV_INT8, false>(mt, none, a, grid, st);
     else if (kind == OE_KV_E4M3) rc = launch_tiles<OE_KV_E4M3, false>(mt, none, a, grid, st);
     if (rc || splits == 1) return rc;
-    return oe_join_parts(out, part_o, part_ml, (long long)n_tokens * H, splits, st);
+    return oe_join_parts(out, part_o, part_ml, cu_q + n_seqs, n_tokens, H, splits, st);
 }
 
 // The parts of the groups' prefixes (see oe_attn_kv8_prefix) into part_o [B * H, splits, HD] and part_ml [B * H, splits, 2].

@@ -50,7 +50,7 @@ def _rows_lib(head_dim: int):
         P, I, F, L = c_void_p, c_int, c_float, c_longlong
         lib.oe_attn_rows.argtypes = [I, P, P, L, P, P, P, P, L, P, I, P, P, P, I, I, I, I, I, I, F, I, I, P, P, P]
         lib.oe_attn_rows_prefix.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, F, P, P, P, I, I, I, I, P, P, I, P]
-        lib.oe_join_parts.argtypes = [P, P, P, L, I, P]
+        lib.oe_join_parts.argtypes = [P, P, P, P, I, I, I, P]
         lib.oe_join_parts.restype = c_int
         lib.oe_attn_rows_error.argtypes = []
         lib.oe_attn_rows.restype = lib.oe_attn_rows_prefix.restype = lib.oe_attn_rows_error.restype = c_int
@@ -227,7 +227,8 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
             warps, cluster, int(many_pairs(ctx.n_seqs, n_kv_heads)), None, 0, None, None, shares, *parts, int(ahead), ops._stream()),
             what, {"warps": warps, "cluster": cluster, "shares": shares})
         if shares > 1:
-            ops._check(_rows_lib(head_dim).oe_join_parts(out.data_ptr(), *parts, T * n_heads, shares, ops._stream()), "join_parts")
+            ops._check(_rows_lib(head_dim).oe_join_parts(
+                out.data_ptr(), *parts, ctx.cu_q.data_ptr() + 4 * ctx.n_seqs, T, n_heads, shares, ops._stream()), "join_parts")
         return
     mt, splits = form or prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
     part = _parts(T * n_heads, splits, head_dim, out.device) if splits > 1 else None

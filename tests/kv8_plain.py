@@ -133,6 +133,25 @@ class Step:
             first=torch.tensor(ends, **i32), pages=torch.tensor(pages or [0], **i32),
             seq_pages=torch.tensor([p[1] if p is not None else 0 for p in self.prefixes], **i32))
 
+    def pad(self, n):
+        """n padding tokens, each a sequence without tokens, behind a step of single tokens, or behind the last sequence of others."""
+        more = lambda t, v, k=n: torch.cat([t, torch.full((k,), v, dtype=t.dtype, device=t.device)])    # noqa: E731
+        c = self.ctx
+        self.qkv = torch.cat([self.qkv, torch.full((n, self.qkv.shape[1]), math.nan, dtype=self.qkv.dtype, device="cuda")])
+        c.n_tokens += n
+        c.tok_seq, c.tok_pos = more(c.tok_seq, -1), more(c.tok_pos, 0)
+        if c.all_decode:
+            c.n_seqs += n
+            c.cu_q, c.seq_start, c.seq_qlen = more(c.cu_q, int(c.cu_q[-1])), more(c.seq_start, 0), more(c.seq_qlen, 0)
+            self.tables = torch.cat([self.tables, torch.full((n, self.tables.shape[1]), -1, dtype=torch.int32, device="cuda")])
+            self.prefix.seq_pages = more(self.prefix.seq_pages, 0)
+
+    def spoil_codes(self):
+        """Codes of rows that no token has yet become e4m3's codes that are no number."""
+        codes = self.cache[0].view(torch.uint8)
+        dead = ~self.live[:, None, None, :].expand(codes.shape[:4])
+        codes[dead.to(codes.device)] = 0x7f
+
     # ---------------------------------------------------------------------------------------------- what has to come out
     def truth(self):
         """(out, tolerance) [T, H hd] float64, and the cache as it has to be afterwards (codes and scales, or rows)."""

@@ -155,6 +155,72 @@ def test_undefined_rows_show_only_where_they_are_seen(dtype):
     close(got[1, 2 * 64:], want[1, 2 * 64:], tol[1, 2 * 64:])
 
 
+@pytest.mark.parametrize("starts,qlens,window,forms", [
+    ([100, 0, 63, 700], [1] * 4, 0, [(4, 1, 1), (12, 2, 1), (4, 1, 5)]), ([100, 200, 65], [1] * 3, 40, [None]),
+    ([30, 0], [2, 1], 0, [None]), ([0, 70, 300], [90, 3, 33], 0, [(1, 1), (2, 1), (2, 3)]), ([300], [100], 50, [None, (2, 2)])])
+def test_codes_behind_the_last_token_that_are_no_numbers(starts, qlens, window, forms):
+    for form in forms:
+        s = Step(starts, qlens, 6, 2, 64, torch.float8_e4m3fn, seed=19, window=window)
+        s.spoil_codes()
+        want, tol, cache = s.truth()
+        close(s.out(form=form), want, tol)
+        s.check_cache(cache)
+
+
+@pytest.mark.parametrize("qlens", [[1], [60]])
+def test_a_page_that_is_not_there_has_no_codes(qlens):
+    """Whatever the cache's first page holds."""
+    got = []
+    for spoilt in (False, True):
+        s = Step([200], qlens, 4, 2, 64, torch.float8_e4m3fn, seed=21)
+        assert 0 not in s.tables_list[0]
+        s.tables[0, 1] = -1
+        if spoilt:
+            s.spoil_codes()
+        got.append(s.out())
+    assert torch.equal(*got) and torch.isfinite(got[0].float()).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", [(1, 1), (2, 1), (1, 3), (2, 4), (2, 16)])
+@pytest.mark.parametrize("H,KVH,hd,window", [(6, 2, 128, 0), (10, 2, 64, 0), (4, 4, 64, 100), (6, 2, 64, -128)])
+def test_forms_of_prompts(H, KVH, hd, window, form, dtype):
+    s = Step([0, 600, 129, 64], [300, 70, 1, 129], H, KVH, hd, dtype, seed=21, window=window, peaked=2.0, pad_seqs=1)
+    want, tol, cache = s.truth()
+    close(s.out(form=form), want, tol)
+    s.check_cache(cache)
+
+
+@pytest.mark.parametrize("starts,qlens,form", [([70, 0, 900], [1] * 3, (4, 1, 1)), ([70, 0, 900], [1] * 3, (12, 4, 1)),
+                                               ([70, 0, 900], [1] * 3, (4, 1, 7)), ([0, 100], [80, 50], (2, 1)), ([0, 100], [80, 50], (1, 3))])
+def test_padding_rows_are_left_alone(starts, qlens, form):
+    s = Step(starts, qlens, 6, 2, 64, torch.int8, seed=22)
+    want, tol, cache = s.truth()
+    n = s.qkv.shape[0]
+    s.pad(5)
+    got = s.out(form=form)
+    close(got[:n], want, tol)
+    assert (got[n:] == 7.0).all()
+    s.check_cache(cache)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window", [0, 60])
+@pytest.mark.parametrize("form", [(2, 1), (1, 2)])
+def test_undefined_keys_and_values_of_a_prompt(dtype, window, form):
+    """Tokens before an undefined one, and those whose window it has left, do not see it."""
+    for which, value in ((1, math.inf), (2, math.nan)):
+        s = Step([40], [200], 4, 1, 64, dtype, seed=23, window=window)
+        sees = torch.zeros(200, dtype=torch.bool)
+        for at in (77, 150):
+            s.qkv[at, 4 * 64 + (which - 1) * 64 + 5] = value
+            sees[at:at + window if window else None] = True
+        want, tol, _ = s.truth()
+        got = s.out(form=form).cpu()
+        assert torch.isnan(got[sees]).all()
+        close(got[~sees], want[~sees], tol[~sees])
+
+
 def test_strided_rows_no_rotation_another_stream_and_a_graph():
     s = Step([70, 0, 200], [1, 1, 1], 6, 2, 64, torch.int8, seed=13, rotate=False, stride_pad=24)
     want, tol, cache = s.truth()

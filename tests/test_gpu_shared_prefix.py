@@ -64,6 +64,45 @@ def test_without_groups_and_with_bounds(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tiles,splits,wide,cluster", [(1, 1, True, 1), (2, 1, False, 1), (2, 3, True, 2), (1, 7, False, 4), (2, 148, True, 8)])
+@pytest.mark.parametrize("H,KVH,hd", [(6, 2, 64), (24, 8, 128)])
+def test_forms(H, KVH, hd, tiles, splits, wide, cluster, dtype):
+    n = 60
+    s = Step([320 + i for i in range(n)] + [100, 0], [1] * (n + 2), H, KVH, hd, dtype, seed=11, peaked=2.0, prefixes=[(0, 5)] * n + [None] * 2)
+    want, tol, cache = s.truth()
+    warps = (12 if wide else 4) if dtype != torch.bfloat16 else (6 if wide else 3)
+    close(s.shared_out(form=(tiles, splits, warps, cluster)), want, tol)
+    s.check_cache(cache)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_padding_rows_and_codes_that_are_no_numbers(dtype):
+    s = Step([192, 200, 255, 80], [1] * 4, 6, 2, 64, dtype, seed=12, prefixes=[(0, 3)] * 3 + [None])
+    if dtype == torch.float8_e4m3fn:
+        s.spoil_codes()
+    want, tol, cache = s.truth()
+    s.pad(4)
+    got = s.shared_out()
+    close(got[:4], want, tol)
+    assert (got[4:] == 7.0).all()
+    s.check_cache(cache)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_common_page_that_is_not_there(dtype):
+    """It has no keys, whatever the cache's first page holds: as if read sequence by sequence."""
+    got = []
+    for spoilt in (False, True):
+        s = Step([192, 200, 255], [1] * 3, 6, 2, 64, dtype, seed=13, prefixes=[(0, 3)] * 3)
+        assert all(0 not in t for t in s.tables_list)
+        s.tables[:, 1] = -1
+        if spoilt and dtype == torch.float8_e4m3fn:
+            s.spoil_codes()
+        got.append(s.shared_out(form=(1, 2, 6 if dtype == torch.bfloat16 else 12, 1)))
+    assert torch.equal(*got) and torch.isfinite(got[0].float()).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_queries_only(dtype):
     s = Step([128, 140], [1, 1], 8, 4, 64, dtype, seed=7, prefixes=[(0, 2)] * 2, has_kv=False)
     want, tol, cache = s.truth()

@@ -23,6 +23,7 @@ from .ops import PAGE, KernelError
 HEAD_DIMS = (64, 128)
 MAX_SPLITS = 148     # of a prefix; with a cluster's CTAs at most MAX_JOINED of attention_kv8.cu
 FEW_ROWS = 16        # rows of a tile of attention_kv8.cu
+MAX_RUNS = 16        # that a tile's pages are cut into
 TILE_ROWS = 128      # rows (a token's or member's heads of one KV head) of a tile of attention_rows.cu; must equal its BM
 CODE_TYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 _KINDS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
@@ -230,7 +231,8 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
             ops._check(_rows_lib(head_dim).oe_join_parts(
                 out.data_ptr(), *parts, ctx.cu_q.data_ptr() + 4 * ctx.n_seqs, T, n_heads, shares, ops._stream()), "join_parts")
         return
-    mt, splits = form or prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
+    mt, splits = form or prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window),
+                                     max_qlen=ctx.max_qlen)
     part = _parts(T * n_heads, splits, head_dim, out.device) if splits > 1 else None
     ops._check(_rows_lib(head_dim).oe_attn_rows(
         kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(), codes.shape[0],
@@ -252,16 +254,29 @@ def _part_ptrs(part, rows: int, splits: int, head_dim: int) -> tuple:
     return part.data_ptr(), part.data_ptr() + 4 * rows * splits * head_dim
 
 
-def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context_class: int, window: int, sm_count: int | None = None) -> tuple:
-    """(tiles of 128 rows a CTA has, runs that a tile's pages are cut into) of a step of prompts."""
-    sms = sm_count or ops.sm_count()
-    tiles = n_tokens // (TILE_ROWS // group) + n_seqs
-    mt = 2 if tiles > 1 else 1
-    ctas = -(-tiles // mt) * n_kv_heads
-    pages = (12, 24, 64, 128)[context_class]
+def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context_class: int, window: int, sm_count: int | None = None,
+                max_qlen: int | None = None) -> tuple:
+    """(tiles of 128 rows a CTA has, runs that a tile's pages are cut into) of a step of prompts: those of the lowest estimate.
+
+    A CTA takes about 8 us to start and end, and 1.1 us a page with one tile, 1.4 with two; CTAs beyond one an SM queue; a page run
+    more costs its parts' traffic, and the kernel that joins them 3 us.  How long the contexts are is known by class only.  us with
+    32 heads over 8 KV heads of 128 in int8, (tiles, runs):  64 tokens (1,1) 12, (1,3) 15, (2,1) 14, (2,3) 18; 300 17, 27, 20, 23; 600
+    23, 48, 27, 41; 2,048 (1,1) 102, (2,1) 74, (2,2) 126; 4 of 500 44, 37, 72; 64 of 30 41, 46, 86; 192 tokens behind 12,000 (1,1)
+    221, (1,3) 87, (2,4) 89, (2,6) 68, (2,12) 81; 512 behind 4,000 (1,1) 90, (2,1) 113, (2,2) 78, (2,4) 85; 32 behind 12,000 (1,8) 40,
+    (1,16) 30, (2,16) 33, (1,24) 40; 4 of 64 behind 8,000 (1,2) 86, (2,3) 81, (2,4) 67, (2,8) 76."""
+    sms, pages, best = sm_count or ops.sm_count(), (6, 18, 44, 128)[context_class], None
     if window:
         pages = min(pages, abs(window) // PAGE + 2)
-    return mt, max(1, min(sms // ctas, pages // 4, 16))
+    for mt in (1, 2):
+        tokens = TILE_ROWS // group * mt                       # of a CTA
+        ctas = min(n_seqs * -(-(max_qlen or n_tokens) // tokens), n_tokens // tokens + n_seqs) * n_kv_heads
+        for runs in {1, max(1, min(sms // ctas, pages // 4, MAX_RUNS))}:
+            us = max(1.0, ctas * runs / sms) * (8 + pages / runs * (1.1 if mt == 1 else 1.4))
+            if runs > 1:
+                us += 3 + runs * n_tokens * group * n_kv_heads * 2.5e-4
+            if best is None or us < best[0]:
+                best = us, mt, runs
+    return best[1:]
 
 
 def sharing_pays(groups: list, eight: bool) -> bool:

@@ -5,8 +5,8 @@
 // A row is a (token, query head of the group) pair.  A CTA has MT tiles of 128 rows of one KV head and a run of cache pages (64 keys
 // each); the tiles share every page's K and V.  Per page and tile:
 //   S = Q K^T      tcgen05.mma M=128 N=64 K=HD, float32 in tensor memory (two buffers);
-//   softmax        128 threads, one row each: the row's 64 scores from tensor memory, times the keys' scales, mask, maximum and sum in
-//                  float32, P back into the buffer's columns;
+//   softmax        128 threads, one row each, or of a single tile 256, half a row's keys each: the scores from tensor memory, times
+//                  the keys' scales, mask, maximum and sum in float32, P back into the buffer's columns;
 //   O += P V       tcgen05.mma M=128 N=HD K=64, P from tensor memory, O float32 in tensor memory for the whole run.
 // A row's reference maximum moves only when its maximum has grown by more than 2^7 since it was set; O and the sum are rescaled
 // then, before the page's P V is issued, and the factor cancels in O / l.
@@ -17,8 +17,16 @@
 // then below 2^-33 of a row's largest weight).  R grows for the whole CTA at once, with the rescaling of O.
 // bfloat16: K and V as they are (TMA); queries and weights are sums of two bfloat16, a second product each.
 // Roles (warps): 0 asks for the pages, 1 issues the products, 2 prepares the scales, 4-11 turn codes into float16 (8-bit forms),
-// the last 4 MT load and turn the queries, then do the softmax and store.
+// the last 8 load and turn the queries, then do the softmax and store.
 // Few tiles: the pages are cut into `splits` runs, whose parts (O, m, l) are joined by the kernel that runs next.
+// Measured (us; 8 KV heads of 128, int8):  a page takes a CTA 0.98 with one tile and 1.38 with two, besides 10 to 13 to start and end.  No
+// unit is full then (two tiles: issue slots 56 %, exponentials and tensor cores 39 % each); the time is the chain that a page's
+// scores, weights and products are, with two buffers of scores, and the waits between its warps: leaving out the exponentials, the scales'
+// loads, half of either product or half of the conversion's stores changes it by 3 % at most.  One tile, whose chain nothing else
+// hides: two threads a row 0.98, one 1.06; two tiles: 1.52 and 1.38.  Two CTAs of one tile an SM: 2,048 tokens in 90 instead of 74.  A
+// warp for each tile's products: 1.44 instead of 1.38.  A prompt of 2,048 tokens with 24 heads takes 68 (379 TFLOP/s of causal work),
+// 192 tokens with 32 heads behind 12,005 of e4m3 73 (518 TFLOP/s), joined from 6 runs; 64 members with 32 heads behind
+// 8,192 common tokens 50 with the kernel of their own keys (177 TFLOP/s).
 // Every wait on an mbarrier is bounded in time; one that runs out raises an error flag, every role leaves its loop, copies in
 // flight get a fixed time, and tensor memory is freed.
 #include <cuda.h>
@@ -58,6 +66,7 @@ struct Ctl {
     uint32_t tmem_base;
     int abort_flag;
     float up[2 * BM];                            // what a row of queries was divided by
+    float swap[2][BM];                           // what the two threads of a row tell each other
 };
 
 template <int KIND, int MT>
@@ -69,7 +78,13 @@ struct Shape {
     static constexpr int BYTES = CTL_AT + (int)sizeof(Ctl);
     static constexpr int CONVERT = EIGHT ? 8 : 0;                      // warps: four for keys, four for values
     static constexpr int FIRST = 4 + CONVERT;                          // the first softmax warp
-    static constexpr int THREADS = (FIRST + 4 * MT) * 32;
+    static constexpr int SPLIT = MT == 1 ? 2 : 1;                      // softmax threads of a row
+    static constexpr int KEYS = BN / SPLIT;                            // that each has of a page
+    static constexpr int SOFTMAX = 4 * MT * SPLIT;                     // warps
+    static constexpr int THREADS = (FIRST + SOFTMAX) * 32;
+    // 8-bit forms: the launch gives each thread of the five warpgroups 96 registers, 480 for a lane of each; the softmax's need more
+    static constexpr int SOFTMAX_REGISTERS = 144, CONVERT_REGISTERS = 56, OTHER_REGISTERS = 80;
+    static constexpr int ALL_REGISTERS = OTHER_REGISTERS + 2 * CONVERT_REGISTERS + SOFTMAX / 4 * SOFTMAX_REGISTERS;
     static constexpr uint32_t S_COLS = MT * 2 * BN, O_COLS = MT * HD;
     static constexpr uint32_t COLS = S_COLS + O_COLS <= 128 ? 128 : S_COLS + O_COLS <= 256 ? 256 : 512;
     static constexpr float HEADROOM = EIGHT ? 8.f : 0.f;
@@ -141,6 +156,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, Ctl* c
 }
 // All lanes of the warp wait and take the same decision.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Ctl* ctl, int code) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctl, code));
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -278,14 +294,14 @@ __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* tile, 
     }
 }
 
-// A row's weights of a page: P into tensor memory, their sum.  GONE: some scores are -infinity, whose weights are zero whatever the
-// values' scales are.
-template <bool EIGHT, bool GONE>
-__device__ __forceinline__ float page_weights(const float (&s)[BN], const float* vscale, float scale, float neg_m, uint32_t p_addr) {
+// A row's weights of a page, or of the half that the thread has: P into tensor memory, their sum.  GONE: some scores are -infinity,
+// whose weights are zero whatever the values' scales are.
+template <bool EIGHT, bool GONE, int KEYS>
+__device__ __forceinline__ float page_weights(const float (&s)[KEYS], const float* vscale, float scale, float neg_m, uint32_t p_addr) {
     const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(neg_m, neg_m);
     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int k0 = 0; k0 < BN; k0 += 16) {
+    for (int k0 = 0; k0 < KEYS; k0 += 16) {
         uint32_t w[8], rest[8];
 #pragma unroll
         for (int k = 0; k < 16; k += 4) {
@@ -314,6 +330,14 @@ __device__ __forceinline__ float page_weights(const float (&s)[BN], const float*
     }
     const float2 all = add2(sum[0], sum[1]);
     return all.x + all.y;
+}
+// Two warps' decision: true for all 64 threads if it is true for one.
+__device__ __forceinline__ bool either(int barrier, bool mine) {
+    uint32_t all;
+    __syncwarp();
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((uint32_t)mine), "r"(barrier) : "memory");
+    return all != 0;
 }
 
 // PREFIX false: the tiles are those of one sequence's tokens, keys up to each row's position.  PREFIX true: the rows are those of all
@@ -383,18 +407,18 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     }
     const int* trow = a.tables + (size_t)b * a.max_pages;
     if (threadIdx.x == 0) {
-        mbar_init(&ctl->q_full, Z::CONVERT + MT * 4);
+        mbar_init(&ctl->q_full, Z::CONVERT + Z::SOFTMAX);
         for (int s = 0; s < RAW_STAGES; s++) { mbar_init(&ctl->raw_full[s], 1); mbar_init(&ctl->raw_empty[s], 8); }
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&ctl->k_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->k_empty[s], 1);
             mbar_init(&ctl->v_full[s], EIGHT ? 4 : 1); mbar_init(&ctl->v_empty[s], 1);
         }
         for (int s = 0; s < SC_SLOTS; s++) {
-            mbar_init(&ctl->sc_full[s], 1); mbar_init(&ctl->sc_ready[s], 1); mbar_init(&ctl->sc_empty[s], MT * 4);
+            mbar_init(&ctl->sc_full[s], 1); mbar_init(&ctl->sc_ready[s], 1); mbar_init(&ctl->sc_empty[s], Z::SOFTMAX);
         }
         for (int t = 0; t < MT; t++) {
             mbar_init(&ctl->s_full[t][0], 1); mbar_init(&ctl->s_full[t][1], 1);
-            mbar_init(&ctl->p_ready[t][0], 4); mbar_init(&ctl->p_ready[t][1], 4);
+            mbar_init(&ctl->p_ready[t][0], 4 * Z::SPLIT); mbar_init(&ctl->p_ready[t][1], 4 * Z::SPLIT);
             mbar_init(&ctl->pv_done[t], 1); mbar_init(&ctl->o_done[t], 1);
         }
         ctl->abort_flag = 0;
@@ -416,8 +440,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     // The queries, turned, by all warps from 4 on: HD / 16 lanes have a row, 8 dimensions of its lower half and the 8 that they are
     // turned with each.  Several rows' pieces are asked for before the first is used: the start of a CTA is these loads.
     if (warp >= 4) {
-        constexpr int PER = HD / 16, AT_ONCE = 32 / PER, WARPS = Z::CONVERT + 4 * MT, GROUPS = MT * BM / AT_ONCE;
-        constexpr int ROUND = EIGHT && MT == 2 ? 2 : GROUPS / WARPS >= 4 ? 4 : (GROUPS + WARPS - 1) / WARPS;     // (two: what 96 registers hold)
+        constexpr int PER = HD / 16, AT_ONCE = 32 / PER, WARPS = Z::CONVERT + Z::SOFTMAX, GROUPS = MT * BM / AT_ONCE;
+        constexpr int NEEDED = (GROUPS + WARPS - 1) / WARPS, MOST = Z::THREADS > 384 ? 2 : 4, ROUND = NEEDED < MOST ? NEEDED : MOST;     // (what the registers hold)
         const int d = lane % PER * 8;
         // where the rows are, of all rounds
         constexpr int ALL = (GROUPS + WARPS - 1) / WARPS;
@@ -516,10 +540,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->q_full);
     }
-    // 8-bit forms: the launch gives every thread of the 3 + MT warpgroups 96 registers (two tiles) or 128 (one), 480 or 512 for a lane of
-    // each; the softmax needs more of them than the others: 80 + 56 + 56 + 2 * 144 = 480, 80 + 56 + 56 + 200 < 512
-    constexpr int SOFTMAX_REGISTERS = MT == 2 ? 144 : 200;
-    if (EIGHT && warp < 4) fewer_registers<80>();
+    if (EIGHT && warp < 4) fewer_registers<Z::OTHER_REGISTERS>();
     if (warp == 0) {
         // ---------------- the pages ----------------
         if (lane == 0) {
@@ -665,7 +686,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         }
     } else if (EIGHT && warp >= 4 && warp < Z::FIRST) {
         // ---------------- codes to 16-bit tiles: four warps the keys', four the values' ----------------
-        fewer_registers<56>();
+        fewer_registers<Z::CONVERT_REGISTERS>();
         const int t = threadIdx.x & 127;
         const bool values = warp >= 8;
         uint64_t *full = values ? ctl->v_full : ctl->k_full, *empty = values ? ctl->v_empty : ctl->k_empty;
@@ -687,12 +708,13 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
             if (lane == 0) { mbar_arrive(&full[s]); mbar_arrive(&ctl->raw_empty[rs]); }
         }
     } else if (warp >= Z::FIRST) {
-        // ---------------- queries, softmax, output: one row a thread ----------------
-        if (EIGHT) more_registers<SOFTMAX_REGISTERS>();
-        const int tile = (warp - Z::FIRST) / 4, quarter = warp & 3;
+        // ---------------- softmax, output: one row a thread, or two threads a row ----------------
+        if (EIGHT) more_registers<Z::SOFTMAX_REGISTERS>();
+        constexpr int SPLIT = Z::SPLIT, KEYS = Z::KEYS;
+        const int tile = (warp - Z::FIRST) / (4 * SPLIT), half = SPLIT == 2 ? (warp - Z::FIRST) / 4 & 1 : 0, quarter = warp & 3, pair = 1 + tile * 4 + quarter;
         const int r = quarter * 32 + lane;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t s_addr = lane_addr + (uint32_t)(tile * 2 * BN), o_addr = lane_addr + Z::S_COLS + (uint32_t)(tile * HD);
+        const uint32_t s_addr = lane_addr + (uint32_t)(tile * 2 * BN), o_addr = lane_addr + Z::S_COLS + (uint32_t)(tile * HD + half * (HD / SPLIT));
         const int tok = t0 + tile * tpt + r / G, head = kvh * G + r % G;
         const bool valid = r < tpt * G && tok < count;
         int pos = 0, low = 0;
@@ -719,18 +741,26 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
             scale *= ctl->up[tile * BM + r];
         }
         float m_run = -INFINITY, l_run = 0.f, ref = 1.f;
-        for (int i = 0; i < nb && ok; i++) {
+        float* tell = &ctl->swap[half][r];                 // (two threads a row: one tile)
+        const float* told = &ctl->swap[half ^ 1][r];
+        // (a wait that runs out is told to the warp with the other half of the rows, so that neither waits for the other)
+        for (int i = 0; i < nb; i++) {
             const int c = i % SC_SLOTS;
             const Scales* sc = &ctl->sc[c];
-            if (EIGHT) ok = mbar_wait(&ctl->sc_ready[c], (uint32_t)(i / SC_SLOTS) & 1u, ctl, 15);
-            if (ok) ok = mbar_wait(&ctl->s_full[tile][i & 1], (uint32_t)(i >> 1) & 1u, ctl, 7);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            const uint32_t sc_parity = (uint32_t)(i / SC_SLOTS) & 1u, s_parity = (uint32_t)(i >> 1) & 1u;
+            const bool scales = !EIGHT || mbar_try_wait(&ctl->sc_ready[c], sc_parity), scores = mbar_try_wait(&ctl->s_full[tile][i & 1], s_parity);
+            if (!__all_sync(0xffffffffu, scales && scores)) {
+                if (ok && !scales) ok = mbar_wait(&ctl->sc_ready[c], sc_parity, ctl, 15);
+                if (ok && !scores) ok = mbar_wait(&ctl->s_full[tile][i & 1], s_parity, ctl, 7);
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            if (SPLIT == 1 && !ok) break;
             fence_after();
-            float s[BN];
+            float s[KEYS];
 #pragma unroll
-            for (int c0 = 0; c0 < BN; c0 += 16) tmem_ld16_nowait(s_addr + (uint32_t)((i & 1) * BN + c0), &s[c0]);
+            for (int c0 = 0; c0 < KEYS; c0 += 16) tmem_ld16_nowait(s_addr + (uint32_t)((i & 1) * BN + half * KEYS + c0), &s[c0]);
             tmem_ld_wait();
-            const int key0 = (j_lo + i) * BN;
+            const int key0 = (j_lo + i) * BN + half * KEYS;
             bool mapped;
             float grown = 1.f;
             if (EIGHT) {
@@ -738,8 +768,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 grown = sc->grown;
                 ref = sc->ref;
 #pragma unroll
-                for (int k = 0; k < BN; k += 4) {
-                    const float4 f = *(const float4*)&sc->k[k];
+                for (int k = 0; k < KEYS; k += 4) {
+                    const float4 f = *(const float4*)&sc->k[half * KEYS + k];
                     const float2 x = mul2(make_float2(s[k], s[k + 1]), make_float2(f.x, f.y));
                     const float2 y = mul2(make_float2(s[k + 2], s[k + 3]), make_float2(f.z, f.w));
                     s[k] = x.x; s[k + 1] = x.y; s[k + 2] = y.x; s[k + 3] = y.y;
@@ -749,45 +779,57 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 mapped = (unsigned)page < (unsigned long long)a.n_pages;
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            // a page wholly before a row's position, inside its window and of the cache needs no mask; the decision is the warp's, and
+            // keys wholly before a row's position, inside its window and of the cache need no mask; the decision is the warp's, and
             // rows without a token, whose results nobody stores, take no part in it
-            const bool masked = __any_sync(0xffffffffu, !mapped || (!PREFIX && valid && !(key0 + BN - 1 <= pos && key0 >= low)));
+            const bool masked = __any_sync(0xffffffffu, !mapped || (!PREFIX && valid && !(key0 + KEYS - 1 <= pos && key0 >= low)));
             if (masked) {
-                const int hi = !mapped ? -1 : PREFIX ? BN - 1 : min(pos - key0, BN - 1), lo = PREFIX ? 0 : max(low - key0, 0);
+                const int hi = !mapped ? -1 : PREFIX ? KEYS - 1 : min(pos - key0, KEYS - 1), lo = PREFIX ? 0 : max(low - key0, 0);
                 const unsigned span = hi >= lo ? (unsigned)(hi - lo) : 0u;
                 const bool some = hi >= lo;
 #pragma unroll
-                for (int k = 0; k < BN; k++) s[k] = some && (unsigned)(k - lo) <= span ? s[k] : -INFINITY;
+                for (int k = 0; k < KEYS; k++) s[k] = some && (unsigned)(k - lo) <= span ? s[k] : -INFINITY;
             }
 #pragma unroll
-            for (int k = 0; k < BN; k += 2) mx4[k / 2 & 3] = max3(mx4[k / 2 & 3], s[k], s[k + 1]);
-            const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale);
-            if (i == 0) {
-                m_run = m_new;
-            } else if (__any_sync(0xffffffffu, grown != 1.f || (valid && m_new > m_run + RESCALE_STEP))) {
-                // P_{i-1} V_{i-1} must have been added to O before O is rescaled (S_i is complete, hence P_{i-2} V_{i-2} too)
-                ok = mbar_wait(&ctl->pv_done[tile], (uint32_t)(i - 1) & 1u, ctl, 8);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            for (int k = 0; k < KEYS; k += 2) mx4[k / 2 & 3] = max3(mx4[k / 2 & 3], s[k], s[k + 1]);
+            float m_new = fmaxf(m_run, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale);
+            // Both halves of the scores have been read behind this: P may take their place.
+            bool move = !ok || i == 0 || grown != 1.f || (valid && m_new > m_run + RESCALE_STEP);
+            if (SPLIT == 2) {
+                fence_before();
+                move = either(pair, move);
                 fence_after();
-                const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new)), beta = alpha * grown;
+            } else {
+                move = __any_sync(0xffffffffu, move);
+            }
+            if (move) {
+                // P_{i-1} V_{i-1} must have been added to O before O is rescaled (S_i is complete, hence P_{i-2} V_{i-2} too)
+                if (ok && i > 0) ok = mbar_wait(&ctl->pv_done[tile], (uint32_t)(i - 1) & 1u, ctl, 8);
+                if (SPLIT == 2) *tell = m_new;
+                ok = SPLIT == 2 ? !either(pair, !ok) : __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                fence_after();
+                if (SPLIT == 2) m_new = fmaxf(m_new, *told);
+                if (i > 0) {
+                    const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new)), beta = alpha * grown;
 #pragma unroll
-                for (int c0 = 0; c0 < HD; c0 += 16) {
-                    float ob[16];
-                    uint32_t ow[16];
-                    tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
-                    tmem_ld_wait();
+                    for (int c0 = 0; c0 < HD / SPLIT; c0 += 16) {
+                        float ob[16];
+                        uint32_t ow[16];
+                        tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int d = 0; d < 16; d++) ow[d] = __float_as_uint(ob[d] * beta);
-                    tmem_st16(o_addr + (uint32_t)c0, ow);
+                        for (int d = 0; d < 16; d++) ow[d] = __float_as_uint(ob[d] * beta);
+                        tmem_st16(o_addr + (uint32_t)c0, ow);
+                    }
+                    tmem_st_wait();
+                    l_run *= alpha;
                 }
-                tmem_st_wait();
-                l_run *= alpha;
                 m_run = m_new;
             }
             const float neg_m = (m_run == -INFINITY ? 0.f : -m_run) + Z::HEADROOM;
-            const uint32_t p_addr = s_addr + (uint32_t)((i & 1) * BN);
-            const float* vs = EIGHT ? sc->v : nullptr;
-            l_run += EIGHT && masked ? page_weights<EIGHT, true>(s, vs, scale, neg_m, p_addr) : page_weights<EIGHT, false>(s, vs, scale, neg_m, p_addr);
+            const uint32_t p_addr = s_addr + (uint32_t)((i & 1) * BN + half * (KEYS / 2));
+            const float* vs = EIGHT ? sc->v + half * KEYS : nullptr;
+            l_run += EIGHT && masked ? page_weights<EIGHT, true, KEYS>(s, vs, scale, neg_m, p_addr) : page_weights<EIGHT, false, KEYS>(s, vs, scale, neg_m, p_addr);
             tmem_st_wait();
             fence_before();
             __syncwarp();
@@ -804,6 +846,13 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 if (lane == 0) mbar_arrive(&ctl->sc_empty[c]);
             }
         }
+        if (SPLIT == 2 && nb > 0) {
+            // (m is told in the last page's round at the latest, which the barrier of that page's P, or of this, has behind it)
+            either(pair, false);
+            *tell = l_run;
+            if (either(pair, !ok)) ok = false;
+            l_run = half ? *told + l_run : l_run + *told;
+        }
         if (ok) {
             if (nb > 0) {
                 ok = mbar_wait(&ctl->o_done[tile], 0, ctl, 16);
@@ -811,30 +860,32 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 fence_after();
             }
             if (ok && nb > 0) {
-                // 32 columns of the warp's rows at a time go through the tile of its queries, which nothing reads any more, so that a row's
-                // values are stored side by side
+                // COLS columns of the warp's rows at a time go through the tile of its queries, which nothing reads any more, so that a
+                // row's values are stored side by side: LANES lanes have a row
+                constexpr int COLS = SPLIT == 2 ? HD / 4 : 32, LANES = COLS / 4, ROWS = 32 / LANES;
+                auto place = [](int rl, int c) { return LANES == 8 ? c ^ (rl & 7) : c ^ (rl >> 1 & 3); };      // (16 bytes: no two of 8 lanes in a bank)
                 const bool parts = PREFIX || a.splits > 1;
                 const float f = parts ? ref : l_run > 0.f ? ref / l_run : l_run == 0.f ? 0.f : l_run;
-                uint8_t* stage = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES + quarter * (32 * 128);
-                const long long mine = parts ? (part * a.splits + split) * HD : row * (long long)(a.H * HD) + (long long)head * HD;
+                uint8_t* stage = q_s + tile * (EIGHT ? 1 : 2) * Q_BYTES + (half * 4 + quarter) * (32 * COLS * 4);
+                const long long mine = (parts ? (part * a.splits + split) * HD : row * (long long)(a.H * HD) + (long long)head * HD) + half * (HD / SPLIT);
                 const uint32_t there = __ballot_sync(0xffffffffu, valid);
-                long long to[8];                            // of the rows whose values this lane stores
+                long long to[LANES];                        // of the rows whose values this lane stores
 #pragma unroll
-                for (int k = 0; k < 8; k++) to[k] = __shfl_sync(0xffffffffu, mine, k * 4 + lane / 8) + lane % 8 * 4;
+                for (int k = 0; k < LANES; k++) to[k] = __shfl_sync(0xffffffffu, mine, k * ROWS + lane / LANES) + lane % LANES * 4;
 #pragma unroll 1
-                for (int c0 = 0; c0 < HD; c0 += 32) {
-                    float ob[32];
-                    tmem_ld16_nowait(o_addr + (uint32_t)c0, ob);
-                    tmem_ld16_nowait(o_addr + (uint32_t)(c0 + 16), ob + 16);
+                for (int c0 = 0; c0 < HD / SPLIT; c0 += COLS) {
+                    float ob[COLS];
+#pragma unroll
+                    for (int c = 0; c < COLS; c += 16) tmem_ld16_nowait(o_addr + (uint32_t)(c0 + c), ob + c);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        *(float4*)(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(ob[4 * c] * f, ob[4 * c + 1] * f, ob[4 * c + 2] * f, ob[4 * c + 3] * f);
+                    for (int c = 0; c < COLS / 4; c++)
+                        *(float4*)(stage + lane * (COLS * 4) + (place(lane, c) << 4)) = make_float4(ob[4 * c] * f, ob[4 * c + 1] * f, ob[4 * c + 2] * f, ob[4 * c + 3] * f);
                     __syncwarp();
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const int rl = k * 4 + lane / 8, c = lane % 8;
-                        const float4 x = *(const float4*)(stage + rl * 128 + ((c ^ (rl & 7)) << 4));
+                    for (int k = 0; k < LANES; k++) {
+                        const int rl = k * ROWS + lane / LANES, c = lane % LANES;
+                        const float4 x = *(const float4*)(stage + rl * (COLS * 4) + (place(rl, c) << 4));
                         if (there >> rl & 1u) {
                             if (parts) *(float4*)(a.part_o + to[k] + c0) = x;
                             else *(uint2*)(a.out + to[k] + c0) = make_uint2(pack16<false>(x.x, x.y), pack16<false>(x.z, x.w));
@@ -843,7 +894,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                     __syncwarp();
                 }
             }
-            if (ok && valid && (PREFIX || a.splits > 1)) *(float2*)(a.part_ml + (part * a.splits + split) * 2) = make_float2(m_run, l_run);
+            if (ok && valid && half == 0 && (PREFIX || a.splits > 1)) *(float2*)(a.part_ml + (part * a.splits + split) * 2) = make_float2(m_run, l_run);
         }
         fence_before();
     }
@@ -860,7 +911,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     }
 }
 
-// Rows' parts joined, in their order: a warp per row.  The step's padding rows, from token *n_real on, have no parts.
+// Rows' parts joined, in their order: a warp per row.  The step's padding rows, from token *n_real on, have no parts.  Its time is that
+// of starting a kernel and of two dependent loads: 3 us for 24 to 6,000 rows of 6 to 36 parts, which are in the L2.
 __global__ void __launch_bounds__(256)
 join_parts_kernel(bf16* out, const float* part_o, const float* part_ml, const int* n_real, int H, long long rows, int n) {
     pdl_launch_dependents();
@@ -926,6 +978,12 @@ int launch(const CUtensorMap& map, const Args& a, dim3 grid, cudaStream_t st) {
     if (set.first()) {
         const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<KIND, PREFIX, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
+        if (Z::EIGHT) {                                    // the warpgroups' shares have to fit what the launch gives
+            cudaFuncAttributes f;
+            const cudaError_t g = cudaFuncGetAttributes(&f, attn_rows_kernel<KIND, PREFIX, MT>);
+            if (g != cudaSuccess) return (int)g;
+            if (f.numRegs * (Z::THREADS / 128) < Z::ALL_REGISTERS) return OE_ERR_UNSUPPORTED;
+        }
         set.done();
     }
     return oe_launch(attn_rows_kernel<KIND, PREFIX, MT>, grid, dim3(Z::THREADS), smem, st, map, a);

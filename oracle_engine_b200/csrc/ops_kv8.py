@@ -258,12 +258,12 @@ def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context
                 max_qlen: int | None = None) -> tuple:
     """(tiles of 128 rows a CTA has, runs that a tile's pages are cut into) of a step of prompts: those of the lowest estimate.
 
-    A CTA takes about 8 us to start and end, and 1.1 us a page with one tile, 1.4 with two; CTAs beyond one an SM queue; a page run
-    more costs its parts' traffic, and the kernel that joins them 3 us.  How long the contexts are is known by class only.  us with
-    32 heads over 8 KV heads of 128 in int8, (tiles, runs):  64 tokens (1,1) 12, (1,3) 15, (2,1) 14, (2,3) 18; 300 17, 27, 20, 23; 600
-    23, 48, 27, 41; 2,048 (1,1) 102, (2,1) 74, (2,2) 126; 4 of 500 44, 37, 72; 64 of 30 41, 46, 86; 192 tokens behind 12,000 (1,1)
-    221, (1,3) 87, (2,4) 89, (2,6) 68, (2,12) 81; 512 behind 4,000 (1,1) 90, (2,1) 113, (2,2) 78, (2,4) 85; 32 behind 12,000 (1,8) 40,
-    (1,16) 30, (2,16) 33, (1,24) 40; 4 of 64 behind 8,000 (1,2) 86, (2,3) 81, (2,4) 67, (2,8) 76."""
+    A CTA takes about 10 us to start and end and 1.0 us a page with one tile, 13 and 1.4 with two; CTAs beyond one an SM queue; runs
+    cost their parts' traffic, and the kernel that joins them 3 us.  How long the contexts are is known by class only.  us with 32
+    heads over 8 KV heads of 128 in int8, (tiles, runs):  64 tokens (1,1) 11, (1,3) 15, (2,1) 14, (2,3) 18; 300 16, 26, 20, 23; 600 22, 48,
+    27, 41; 2,048 (1,1) 95, (2,1) 74, (2,2) 126; 4 of 500 42, 38, 73; 64 of 30 38, 47, 88; 192 tokens behind 12,000 (1,1) 201, (1,3) 81,
+    (2,4) 89, (2,6) 68, (2,12) 81; 512 behind 4,000 (1,1) 82, (2,1) 113, (2,2) 78, (2,4) 85; 32 behind 12,000 (1,8) 37, (1,16) 29, (2,16) 33,
+    (1,24) 38; 4 of 64 behind 8,000 (1,2) 80, (2,3) 81, (2,4) 67, (2,8) 76; 4 of 192 behind 2,000 (1,1) 85, (2,1) 65, (2,2) 80."""
     sms, pages, best = sm_count or ops.sm_count(), (6, 18, 44, 128)[context_class], None
     if window:
         pages = min(pages, abs(window) // PAGE + 2)
@@ -271,7 +271,8 @@ def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context
         tokens = TILE_ROWS // group * mt                       # of a CTA
         ctas = min(n_seqs * -(-(max_qlen or n_tokens) // tokens), n_tokens // tokens + n_seqs) * n_kv_heads
         for runs in {1, max(1, min(sms // ctas, pages // 4, MAX_RUNS))}:
-            us = max(1.0, ctas * runs / sms) * (8 + pages / runs * (1.1 if mt == 1 else 1.4))
+            full = ctas * runs / sms                            # (the CTAs that queue end together less well)
+            us = (full + 0.3 if full > 1 else 1.0) * (10 + pages / runs if mt == 1 else 13 + 1.4 * pages / runs)
             if runs > 1:
                 us += 3 + runs * n_tokens * group * n_kv_heads * 2.5e-4
             if best is None or us < best[0]:

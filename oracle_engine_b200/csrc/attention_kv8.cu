@@ -816,51 +816,47 @@ int launch_rows(int warps, const Args& a, long long rows, int n_seqs, cudaStream
 
 extern "C" {
 
-// Keys and values of n_tokens tokens (rows of `stride` bfloat16: H query heads, KVH keys, KVH values) into the 8-bit cache.
-int oe_kv8_write(int kind, const bf16* qkv, long long stride, const float* cos_tab, const float* sin_tab, void* codes, float* scales,
-                 long long n_pages, const int* tables, int max_pages, const int* tok_seq, const int* tok_pos, int n_tokens, int H,
-                 int KVH, cudaStream_t st) {
-    if (n_tokens <= 0) return 0;
-    if (stride % 8 || ((uintptr_t)qkv & 15) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15)) return OE_ERR_UNSUPPORTED;
-    const long long blocks = ((long long)n_tokens * 2 * KVH * (HD / 16) + 255) / 256;
-    if (blocks > 0x00ffffffLL || ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15)) return OE_ERR_UNSUPPORTED;   // (lanes are counted in 32 bits)
-    if (kind == OE_KV_INT8)
-        return oe_launch(kv8_write_kernel<OE_KV_INT8>, dim3((unsigned)blocks), dim3(256), 0, st, qkv, stride, cos_tab, sin_tab,
-                         (uint8_t*)codes, scales, n_pages, tables, max_pages, tok_seq, tok_pos, n_tokens, H, KVH);
-    if (kind == OE_KV_E4M3)
-        return oe_launch(kv8_write_kernel<OE_KV_E4M3>, dim3((unsigned)blocks), dim3(256), 0, st, qkv, stride, cos_tab, sin_tab,
-                         (uint8_t*)codes, scales, n_pages, tables, max_pages, tok_seq, tok_pos, n_tokens, H, KVH);
-    return OE_ERR_UNSUPPORTED;
+// Keys and values of n_tokens tokens into the 8-bit cache.
+int oe_kv8_write(const Kv8Call* call) {
+    const Kv8Call& c = *call;
+    if (c.bytes != (int)sizeof(Kv8Call)) return OE_ERR_UNSUPPORTED;
+    if (c.n_tokens <= 0) return 0;
+    if (c.stride % 8 || ((uintptr_t)c.qkv & 15) || ((uintptr_t)c.cache & 15) || ((uintptr_t)c.scales & 15)) return OE_ERR_UNSUPPORTED;
+    const long long blocks = ((long long)c.n_tokens * 2 * c.KVH * (HD / 16) + 255) / 256;
+    if (blocks > 0x00ffffffLL || ((uintptr_t)c.cos_tab & 15) || ((uintptr_t)c.sin_tab & 15)) return OE_ERR_UNSUPPORTED;   // (lanes are counted in 32 bits)
+    if (c.kind != OE_KV_INT8 && c.kind != OE_KV_E4M3) return OE_ERR_UNSUPPORTED;
+    return oe_launch(c.kind == OE_KV_INT8 ? kv8_write_kernel<OE_KV_INT8> : kv8_write_kernel<OE_KV_E4M3>, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.qkv,
+                     c.stride, c.cos_tab, c.sin_tab, (uint8_t*)c.cache, c.scales, c.n_pages, c.tables, c.max_pages, c.tok_seq, c.tok_pos,
+                     c.n_tokens, c.H, c.KVH);
 }
 
 // Attention of the step's tokens over their sequences' caches (kind: OE_KV_*).  write != 0: every sequence brings one token, whose
 // key and value this kernel writes.  With seq_pages the pages before a sequence's own are left out and the parts that
-// oe_attn_rows_prefix left are added.  shares > 1: as many CTAs share a tile's keys and leave their parts in own_o [T * H, shares, HD]
-// and own_ml [T * H, shares, 2] (oe_join_parts).
-int oe_attn_kv8(int kind, bf16* out, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, void* cache,
-                float* scales, int write, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
-                const int* seq_qlen, int n_seqs, int max_qlen, int H, int KVH, int window, float scale, int warps, int cluster,
-                int ordered, const int* seq_pages, int splits, const float* part_o, const float* part_ml, int shares, float* own_o, float* own_ml, int ahead,
-                cudaStream_t st) {
-    if (n_seqs <= 0 || max_qlen <= 0) return 0;
-    if (H % KVH || q_stride % 8 || ((uintptr_t)q & 15) || ((uintptr_t)cache & 15) || ((uintptr_t)scales & 15) ||
-        ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15) || ((uintptr_t)out & 15)) return OE_ERR_UNSUPPORTED;
-    if (cluster < 1 || cluster > 8 || (cluster & (cluster - 1)) || (write && max_qlen != 1)) return OE_ERR_UNSUPPORTED;
-    if (seq_pages != nullptr && (window != 0 || max_qlen != 1 || splits < 1 || splits + cluster > MAX_JOINED || part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
-    if (shares < 1 || (shares > 1 && (cluster != 1 || seq_pages != nullptr || own_o == nullptr || own_ml == nullptr))) return OE_ERR_UNSUPPORTED;
+// oe_attn_rows_prefix left (`splits` a row) are added.  shares > 1: as many CTAs share a tile's keys and leave their parts (oe_join_parts).
+int oe_attn_kv8(const Kv8Call* call) {
+    const Kv8Call& c = *call;
+    if (c.bytes != (int)sizeof(Kv8Call)) return OE_ERR_UNSUPPORTED;
+    if (c.n_seqs <= 0 || c.max_qlen <= 0) return 0;
+    if (c.KVH <= 0 || c.H % c.KVH || c.stride % 8 || ((uintptr_t)c.qkv & 15) || ((uintptr_t)c.cache & 15) || ((uintptr_t)c.scales & 15) ||
+        ((uintptr_t)c.cos_tab & 15) || ((uintptr_t)c.sin_tab & 15) || ((uintptr_t)c.out & 15)) return OE_ERR_UNSUPPORTED;
+    if (c.cluster < 1 || c.cluster > 8 || (c.cluster & (c.cluster - 1)) || (c.write && c.max_qlen != 1)) return OE_ERR_UNSUPPORTED;
+    const bool no_parts = c.part_o == nullptr || c.part_ml == nullptr;
+    if (c.seq_pages != nullptr && (c.window != 0 || c.max_qlen != 1 || c.splits < 1 || c.splits + c.cluster > MAX_JOINED || no_parts)) return OE_ERR_UNSUPPORTED;
+    if (c.shares < 1 || (c.shares > 1 && (c.cluster != 1 || c.seq_pages != nullptr || no_parts))) return OE_ERR_UNSUPPORTED;
     Args a = {};
-    a.out = out; a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab;
-    a.cache = cache; a.scales = scales;
-    if (write) { a.cache_w = cache; a.scales_w = scales; }
-    a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start; a.seq_qlen = seq_qlen;
-    a.H = H; a.KVH = KVH; a.window = window; a.scale_log2 = scale * LOG2E; a.cluster = cluster;
-    a.seq_pages = seq_pages; a.splits = splits; a.part_o = part_o; a.part_ml = part_ml; a.ahead = ahead;
-    a.shares = shares; a.own_o = own_o; a.own_ml = own_ml;
-    a.ordered = ordered && window == 0 && n_seqs > 1 && n_seqs <= MAX_ORDERED ? n_seqs : 0;
-    const long long rows = (long long)max_qlen * (H / KVH);
-    if (kind == OE_KV_BF16) return launch_rows<OE_KV_BF16>(warps, a, rows, n_seqs, st);
-    if (kind == OE_KV_INT8) return launch_rows<OE_KV_INT8>(warps, a, rows, n_seqs, st);
-    if (kind == OE_KV_E4M3) return launch_rows<OE_KV_E4M3>(warps, a, rows, n_seqs, st);
+    a.out = c.out; a.q = c.qkv; a.q_stride = c.stride; a.cos_tab = c.cos_tab; a.sin_tab = c.sin_tab;
+    a.cache = c.cache; a.scales = c.scales;
+    if (c.write) { a.cache_w = c.cache; a.scales_w = c.scales; }
+    a.n_pages = c.n_pages; a.tables = c.tables; a.max_pages = c.max_pages; a.cu_q = c.cu_q; a.seq_start = c.seq_start; a.seq_qlen = c.seq_qlen;
+    a.H = c.H; a.KVH = c.KVH; a.window = c.window; a.scale_log2 = c.scale * LOG2E; a.cluster = c.cluster;
+    a.seq_pages = c.seq_pages; a.splits = c.splits; a.ahead = c.ahead; a.shares = c.shares;
+    if (c.seq_pages != nullptr) { a.part_o = c.part_o; a.part_ml = c.part_ml; }
+    else { a.own_o = c.part_o; a.own_ml = c.part_ml; }
+    a.ordered = c.ordered && c.window == 0 && c.n_seqs > 1 && c.n_seqs <= MAX_ORDERED ? c.n_seqs : 0;
+    const long long rows = (long long)c.max_qlen * (c.H / c.KVH);
+    if (c.kind == OE_KV_BF16) return launch_rows<OE_KV_BF16>(c.warps, a, rows, c.n_seqs, c.stream);
+    if (c.kind == OE_KV_INT8) return launch_rows<OE_KV_INT8>(c.warps, a, rows, c.n_seqs, c.stream);
+    if (c.kind == OE_KV_E4M3) return launch_rows<OE_KV_E4M3>(c.warps, a, rows, c.n_seqs, c.stream);
     return OE_ERR_UNSUPPORTED;
 }
 

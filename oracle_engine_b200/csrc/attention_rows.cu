@@ -993,6 +993,14 @@ int launch_tiles(int mt, const CUtensorMap& map, const Args& a, dim3 grid, cudaS
     return mt == 1 ? launch<KIND, PREFIX, 1>(map, a, grid, st) : launch<KIND, PREFIX, 2>(map, a, grid, st);
 }
 
+Args arguments(const Kv8Call& c) {
+    Args a = {};
+    a.out = c.out; a.q = c.qkv; a.q_stride = c.stride; a.cos_tab = c.cos_tab; a.sin_tab = c.sin_tab; a.codes = (const uint8_t*)c.cache;
+    a.scales = c.scales; a.n_pages = c.n_pages; a.tables = c.tables; a.max_pages = c.max_pages; a.cu_q = c.cu_q; a.seq_start = c.seq_start;
+    a.seq_qlen = c.seq_qlen; a.H = c.H; a.KVH = c.KVH; a.window = c.window; a.scale_log2 = c.scale * LOG2E; a.ahead = c.ahead;
+    a.members = c.members; a.first = c.first; a.pages = c.pages; a.splits = c.splits; a.part_o = c.part_o; a.part_ml = c.part_ml;
+    return a;
+}
 bool operands_ok(const Args& a, const void* cache) {
     return a.KVH > 0 && a.H % a.KVH == 0 && a.H / a.KVH <= BM && a.q_stride % 8 == 0 && !((uintptr_t)a.q & 15) && !((uintptr_t)cache & 15) &&
            !((uintptr_t)a.scales & 15) && !((uintptr_t)a.cos_tab & 15) && !((uintptr_t)a.sin_tab & 15) && a.splits >= 1 && a.n_pages >= 1;
@@ -1002,76 +1010,69 @@ bool operands_ok(const Args& a, const void* cache) {
 
 extern "C" {
 
-// out [n_tokens * H, HD] from each row's n parts: part_o [n_tokens * H, n, HD] and part_ml [n_tokens * H, n, 2].  n_real (on the
-// device): how many of the tokens are real; the rows of the others are left as they are.
-int oe_join_parts(bf16* out, const float* part_o, const float* part_ml, const int* n_real, int n_tokens, int H, int n, cudaStream_t st) {
-    const long long rows = (long long)n_tokens * H;
+// out from each row's parts, as many as `shares`, or else `splits`, says.  cu_q[n_seqs] of the tokens are real; the rows of the others are
+// left as they are.
+int oe_join_parts(const Kv8Call* call) {
+    const Kv8Call& c = *call;
+    if (c.bytes != (int)sizeof(Kv8Call)) return OE_ERR_UNSUPPORTED;
+    const long long rows = (long long)c.n_tokens * c.H;
     if (rows <= 0) return 0;
+    const int n = c.shares > 1 ? c.shares : c.splits;
     if (n < 1 || (rows + 7) / 8 > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
-    return oe_launch(join_parts_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, out, part_o, part_ml, n_real, H, rows, n);
+    return oe_launch(join_parts_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, c.stream, c.out, (const float*)c.part_o, (const float*)c.part_ml,
+                     c.cu_q + c.n_seqs, c.H, rows, n);
 }
 
 // Attention of the step's tokens over the 8-bit cache (kind OE_KV_INT8 or OE_KV_E4M3), which has their rows already.  mt: tiles of 128
-// rows a CTA has (1 or 2); splits > 1: the pages of a tile are cut into as many runs, whose parts go through part_o
-// [T * H, splits, HD] and part_ml [T * H, splits, 2].
-int oe_attn_rows(int kind, bf16* out, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, const void* cache,
-                 const float* scales, long long n_pages, const int* tables, int max_pages, const int* cu_q, const int* seq_start,
-                 const int* seq_qlen, int n_seqs, int n_tokens, int max_qlen, int H, int KVH, int window, float scale, int mt, int splits,
-                 float* part_o, float* part_ml, cudaStream_t st) {
-    if (n_seqs <= 0 || max_qlen <= 0) return 0;
-    Args a = {};
-    a.out = out; a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.codes = (const uint8_t*)cache;
-    a.scales = scales; a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start;
-    a.seq_qlen = seq_qlen; a.H = H; a.KVH = KVH; a.window = window; a.scale_log2 = scale * LOG2E;
-    a.splits = splits; a.part_o = part_o; a.part_ml = part_ml;
-    if (!operands_ok(a, cache) || ((uintptr_t)out & 15) || (mt != 1 && mt != 2)) return OE_ERR_UNSUPPORTED;
-    if (splits > 1 && (part_o == nullptr || part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
-    const int tpt = BM / (H / KVH) * mt;
-    const long long tiles = ((long long)max_qlen + tpt - 1) / tpt, x = (long long)KVH * splits;
-    if (tiles > 65535 || n_seqs > 65535 || x > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)x, n_seqs, (unsigned)tiles);
+// rows a CTA has (1 or 2); splits > 1: the pages of a tile are cut into as many runs, whose parts are joined.
+int oe_attn_rows(const Kv8Call* call) {
+    const Kv8Call& c = *call;
+    if (c.bytes != (int)sizeof(Kv8Call)) return OE_ERR_UNSUPPORTED;
+    if (c.n_seqs <= 0 || c.max_qlen <= 0) return 0;
+    const Args a = arguments(c);
+    if (!operands_ok(a, c.cache) || ((uintptr_t)c.out & 15) || (c.mt != 1 && c.mt != 2)) return OE_ERR_UNSUPPORTED;
+    if (c.splits > 1 && (c.part_o == nullptr || c.part_ml == nullptr)) return OE_ERR_UNSUPPORTED;
+    const int tpt = BM / (c.H / c.KVH) * c.mt;
+    const long long tiles = ((long long)c.max_qlen + tpt - 1) / tpt, x = (long long)c.KVH * c.splits;
+    if (tiles > 65535 || c.n_seqs > 65535 || x > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)x, c.n_seqs, (unsigned)tiles);
     const CUtensorMap none = {};
     int rc = OE_ERR_UNSUPPORTED;
-    if (kind == OE_KV_INT8) rc = launch_tiles<OE_KV_INT8, false>(mt, none, a, grid, st);
-    else if (kind == OE_KV_E4M3) rc = launch_tiles<OE_KV_E4M3, false>(mt, none, a, grid, st);
-    if (rc || splits == 1) return rc;
-    return oe_join_parts(out, part_o, part_ml, cu_q + n_seqs, n_tokens, H, splits, st);
+    if (c.kind == OE_KV_INT8) rc = launch_tiles<OE_KV_INT8, false>(c.mt, none, a, grid, c.stream);
+    else if (c.kind == OE_KV_E4M3) rc = launch_tiles<OE_KV_E4M3, false>(c.mt, none, a, grid, c.stream);
+    if (rc || c.splits == 1) return rc;
+    return oe_join_parts(call);
 }
 
-// The parts of the groups' prefixes (see oe_attn_kv8_prefix) into part_o [B * H, splits, HD] and part_ml [B * H, splits, 2].
-int oe_attn_rows_prefix(int kind, const bf16* q, long long q_stride, const float* cos_tab, const float* sin_tab, const void* cache,
-                        const float* scales, long long n_pages, const int* tables, int max_pages, const int* cu_q,
-                        const int* seq_start, int H, int KVH, float scale, const int* members, const int* first, const int* pages,
-                        int n_groups, int n_members, int mt, int splits, float* part_o, float* part_ml, int ahead, cudaStream_t st) {
-    if (n_groups <= 0 || n_members <= 0) return 0;
-    Args a = {};
-    a.q = q; a.q_stride = q_stride; a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.codes = (const uint8_t*)cache; a.scales = scales;
-    a.n_pages = n_pages; a.tables = tables; a.max_pages = max_pages; a.cu_q = cu_q; a.seq_start = seq_start; a.H = H; a.KVH = KVH;
-    a.scale_log2 = scale * LOG2E; a.members = members; a.first = first; a.pages = pages; a.splits = splits;
-    a.part_o = part_o; a.part_ml = part_ml; a.ahead = ahead;
-    if (!operands_ok(a, cache) || (mt != 1 && mt != 2) || part_o == nullptr || part_ml == nullptr) return OE_ERR_UNSUPPORTED;
-    const int tpt = BM / (H / KVH) * mt;
-    const long long tiles = ((long long)n_members + tpt - 1) / tpt, x = (long long)KVH * splits;
-    if (tiles > 65535 || n_groups > 65535 || x > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)x, n_groups, (unsigned)tiles);
+// The parts of the groups' prefixes, `splits` a row (oe_attn_kv8 with seq_pages adds them).
+int oe_attn_rows_prefix(const Kv8Call* call) {
+    const Kv8Call& c = *call;
+    if (c.bytes != (int)sizeof(Kv8Call)) return OE_ERR_UNSUPPORTED;
+    if (c.n_groups <= 0 || c.n_members <= 0) return 0;
+    const Args a = arguments(c);
+    if (!operands_ok(a, c.cache) || (c.mt != 1 && c.mt != 2) || c.part_o == nullptr || c.part_ml == nullptr) return OE_ERR_UNSUPPORTED;
+    const int tpt = BM / (c.H / c.KVH) * c.mt;
+    const long long tiles = ((long long)c.n_members + tpt - 1) / tpt, x = (long long)c.KVH * c.splits;
+    if (tiles > 65535 || c.n_groups > 65535 || x > 0x7fffffffLL) return OE_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)x, c.n_groups, (unsigned)tiles);
     CUtensorMap map = {};
-    if (kind == OE_KV_BF16) {
+    if (c.kind == OE_KV_BF16) {
         // the cache entry as rows of HD: [pages * 2 * KVH * 64][HD]; a box is 64 rows x 64 dims
-        if (n_pages * 2 * KVH * BN > 0x7fffffffLL - BN) return OE_ERR_UNSUPPORTED;
+        if (c.n_pages * 2 * c.KVH * BN > 0x7fffffffLL - BN) return OE_ERR_UNSUPPORTED;
         int rc = get_encode();
         if (rc) return rc;
-        cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)n_pages * 2 * KVH * BN};
+        cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)c.n_pages * 2 * c.KVH * BN};
         cuuint64_t strides[1] = {(cuuint64_t)HD * 2};
         cuuint32_t box[2] = {64, (cuuint32_t)BN};
         cuuint32_t es[2] = {1, 1};
-        CUresult r = g_encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, es,
+        CUresult r = g_encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.cache, dims, strides, box, es,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return 2000 + (int)r;
-        return launch_tiles<OE_KV_BF16, true>(mt, map, a, grid, st);
+        return launch_tiles<OE_KV_BF16, true>(c.mt, map, a, grid, c.stream);
     }
-    if (kind == OE_KV_INT8) return launch_tiles<OE_KV_INT8, true>(mt, map, a, grid, st);
-    if (kind == OE_KV_E4M3) return launch_tiles<OE_KV_E4M3, true>(mt, map, a, grid, st);
+    if (c.kind == OE_KV_INT8) return launch_tiles<OE_KV_INT8, true>(c.mt, map, a, grid, c.stream);
+    if (c.kind == OE_KV_E4M3) return launch_tiles<OE_KV_E4M3, true>(c.mt, map, a, grid, c.stream);
     return OE_ERR_UNSUPPORTED;
 }
 

@@ -30,6 +30,26 @@ struct Kv8Devices {
 #define OE_KV_INT8 1
 #define OE_KV_E4M3 2
 
+// What an entry point of these kernels is told, as the host packs it (one argument to convert instead of thirty); a field that an entry
+// point does not use is 0.
+struct Kv8Call {
+    __nv_bfloat16* out;            // [n_tokens, H*HD]
+    const __nv_bfloat16* qkv;      // [n_tokens, (H + 2 KVH) HD], or queries only; rows of `stride`
+    long long stride;
+    const float *cos_tab, *sin_tab;
+    void* cache;                   // a cache entry's codes, or its bfloat16 rows
+    float* scales;
+    long long n_pages;
+    const int *tables, *cu_q, *seq_start, *seq_qlen, *tok_seq, *tok_pos;
+    const int *members, *first, *pages, *seq_pages;     // of prefixes
+    float *part_o, *part_ml;       // [n_tokens * H, parts, HD], [n_tokens * H, parts, 2]; parts: shares, or splits
+    cudaStream_t stream;
+    int bytes;                     // of this struct
+    int kind, write, max_pages, n_seqs, n_tokens, max_qlen, H, KVH, window, warps, cluster, ordered, shares, mt, splits, n_groups, n_members, ahead;
+    float scale;
+};
+static_assert(sizeof(Kv8Call) == 21 * 8 + 20 * 4, "as the host packs it");
+
 // a * c - b * s rounded once to bfloat16.  Two float32 operations are within 2^-23 of the magnitudes they add; only a sum that near to the
 // border between two bfloat16 is taken apart: the two products into a float32 and its error each, the sum likewise, and what is left
 // over beside a float32 sum on the border settles it.

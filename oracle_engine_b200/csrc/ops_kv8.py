@@ -12,7 +12,8 @@ step, where the projections do; the kernel then asks for those rows while the ke
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_int
 
 import torch
 
@@ -26,8 +27,12 @@ FEW_ROWS = 16        # rows of a tile of attention_kv8.cu
 MAX_RUNS = 16        # that a tile's pages are cut into
 TILE_ROWS = 128      # rows (a token's or member's heads of one KV head) of a tile of attention_rows.cu; must equal its BM
 CODE_TYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _KINDS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
 _libs: dict = {}
+
+
+_CALL = struct.Struct("<21q19if")        # Kv8Call of kv8.cuh
 
 
 def _lib(head_dim: int):
@@ -36,9 +41,7 @@ def _lib(head_dim: int):
         if head_dim not in HEAD_DIMS:
             raise KernelError(f"the 8-bit cache's kernels take heads of {HEAD_DIMS}, not {head_dim}")
         lib = _build.load("attention_kv8", {"OE_HD": head_dim})
-        P, I, F, L = c_void_p, c_int, c_float, c_longlong
-        lib.oe_kv8_write.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, I, P]
-        lib.oe_attn_kv8.argtypes = [I, P, P, L, P, P, P, P, I, L, P, I, P, P, P, I, I, I, I, I, F, I, I, I, P, I, P, P, I, P, P, I, P]
+        lib.oe_kv8_write.argtypes = lib.oe_attn_kv8.argtypes = [c_char_p]
         lib.oe_kv8_write.restype = lib.oe_attn_kv8.restype = c_int
         _libs[head_dim] = lib
     return lib
@@ -48,15 +51,39 @@ def _rows_lib(head_dim: int):
     lib = _libs.get(("rows", head_dim))
     if lib is None:
         lib = _build.load("attention_rows", {"OE_HD": head_dim})
-        P, I, F, L = c_void_p, c_int, c_float, c_longlong
-        lib.oe_attn_rows.argtypes = [I, P, P, L, P, P, P, P, L, P, I, P, P, P, I, I, I, I, I, I, F, I, I, P, P, P]
-        lib.oe_attn_rows_prefix.argtypes = [I, P, L, P, P, P, P, L, P, I, P, P, I, I, F, P, P, P, I, I, I, I, P, P, I, P]
-        lib.oe_join_parts.argtypes = [P, P, P, P, I, I, I, P]
-        lib.oe_join_parts.restype = c_int
+        lib.oe_attn_rows.argtypes = lib.oe_attn_rows_prefix.argtypes = lib.oe_join_parts.argtypes = [c_char_p]
         lib.oe_attn_rows_error.argtypes = []
-        lib.oe_attn_rows.restype = lib.oe_attn_rows_prefix.restype = lib.oe_attn_rows_error.restype = c_int
+        lib.oe_attn_rows.restype = lib.oe_attn_rows_prefix.restype = lib.oe_join_parts.restype = lib.oe_attn_rows_error.restype = c_int
         _libs[("rows", head_dim)] = lib
     return lib
+
+
+def _packed(out, qkv, cos, sin, rows, scales, tables, ctx, part, part_rows: int, parts: int, head_dim: int, dev: int, kind: int, write: int,
+            max_qlen: int, n_heads: int, n_kv_heads: int, window: int, scale: float, ahead: bool, warps: int = 0, cluster: int = 0, ordered: int = 0,
+            shares: int = 1, mt: int = 0, splits: int = 1, prefix=None) -> bytes:
+    """The argument of an attention's entry points; part: room for `parts` parts of `part_rows` rows, or None."""
+    T, max_pages, n_pages = qkv.shape[0], tables.shape[1], rows.shape[0]
+    part_o = 0 if part is None else part.data_ptr()
+    if prefix is None:
+        lists, n_groups, n_members = (0, 0, 0, 0), 0, 0
+    else:
+        lists = (prefix.members.data_ptr(), prefix.first.data_ptr(), prefix.pages.data_ptr(), prefix.seq_pages.data_ptr())
+        n_groups, n_members = prefix.n_groups, prefix.n_members
+    return _CALL.pack(
+        out.data_ptr(), qkv.data_ptr(), qkv.stride(0), 0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(),
+        rows.data_ptr(), 0 if scales is None else scales.data_ptr(), n_pages, tables.data_ptr(), ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
+        ctx.seq_qlen.data_ptr(), 0, 0, *lists,
+        part_o, part_o + 4 * part_rows * parts * head_dim if part_o else 0, _stream(dev),
+        _CALL.size, kind, write, max_pages, ctx.n_seqs, T, max_qlen, n_heads, n_kv_heads, window, warps, cluster, ordered, shares, mt, splits,
+        n_groups, n_members, ahead, scale)
+
+
+def _stream(dev: int) -> int:
+    return ops._raw_stream(dev) if ops._raw_stream is not None else ops._stream()
+
+
+def _sms(dev: int) -> int:
+    return ops._sms.get(dev) or ops.sm_count()
 
 
 def device_error() -> int:
@@ -81,9 +108,9 @@ def _cache_args(what: str, cache, n_kv_heads: int, head_dim: int, allow_16: bool
     if scales is None and not allow_16:
         raise KernelError(f"{what}: codes and scales expected")
     shape = rows.shape
-    if len(shape) != 5 or shape[1] != 2 or shape[2] != n_kv_heads or shape[3] != PAGE or shape[4] != head_dim or not rows.is_contiguous():
+    if shape[1:] != (2, n_kv_heads, PAGE, head_dim) or not rows.is_contiguous():
         raise KernelError(f"{what}: cache entry must be contiguous [pages, 2, KVH, PAGE, head_dim]")
-    if scales is not None and (scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.shape != shape[:4]):
+    if scales is not None and (scales.dtype is not _F32 or not scales.is_contiguous() or scales.shape != shape[:4]):
         raise KernelError(f"{what}: scales must be contiguous float32 [pages, 2, KVH, PAGE]")
     return kind, rows, scales
 
@@ -95,27 +122,26 @@ def _check_heads(what: str, n_heads: int, n_kv_heads: int, head_dim: int) -> Non
 
 
 def _check_rows(what: str, qkv, cos, sin, width: int, head_dim: int) -> None:
-    if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or qkv.stride(0) % 8 or \
-            qkv.data_ptr() % 16:
+    shape, stride = qkv.shape, qkv.stride()
+    if qkv.dtype is not _BF16 or len(shape) != 2 or shape[1] != width or stride[1] != 1 or stride[0] % 8 or qkv.data_ptr() % 16:
         raise KernelError(f"{what}: qkv must be bfloat16 [T, {width}] with rows of multiples of 16 bytes")
     if cos is None and sin is None:
         return
     for t in (cos, sin):
-        if t is None or t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] != head_dim // 2 or not t.is_contiguous() or \
-                t.data_ptr() % 16:
+        if t is None or t.dtype is not _F32 or t.dim() != 2 or t.shape[1] != head_dim // 2 or not t.is_contiguous() or t.data_ptr() % 16:
             raise KernelError(f"{what}: cos/sin must be contiguous float32 [max_pos, head_dim/2]")
-    if cos.shape[0] != sin.shape[0]:
+    if cos.shape != sin.shape:
         raise KernelError(f"{what}: cos and sin must have equally many rows")
 
 
-def _check_ints(what: str, **tensors) -> None:
-    for name, t in tensors.items():
-        if t.dtype is not torch.int32 or not t.is_contiguous():
+def _check_ints(what: str, names: tuple, tensors: tuple) -> None:
+    for t, name in zip(tensors, names):
+        if t.dtype is not _I32 or not t.is_contiguous():
             raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
 
 
-def _here(what: str, *tensors) -> None:
-    """Every tensor is on the current device, whose stream the kernel is launched on."""
+def _here(what: str, *tensors) -> int:
+    """The current device, on whose stream the kernel is launched; every tensor is on it."""
     if tensors[0].get_device() < 0:
         ops._dev(*tensors)
     dev = torch._C._cuda_getDevice()
@@ -123,22 +149,20 @@ def _here(what: str, *tensors) -> None:
         if t is not None and t.get_device() != dev:
             ops._dev(t)
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+    return dev
 
 
 def _check_step(what: str, out, qkv, cos, tables, ctx, n_heads: int, head_dim: int) -> None:
     n, longest = ctx.n_seqs, getattr(ctx, "max_kvlen", 0)
-    _check_ints(what, tables=tables, cu_q=ctx.cu_q, seq_start=ctx.seq_start, seq_qlen=ctx.seq_qlen)
-    if out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != qkv.shape[0] or out.shape[1] != n_heads * head_dim or \
-            not out.is_contiguous() or out.data_ptr() % 16:
+    cu_q, start, qlen = ctx.cu_q, ctx.seq_start, ctx.seq_qlen
+    _check_ints(what, ("tables", "cu_q", "seq_start", "seq_qlen"), (tables, cu_q, start, qlen))
+    if out.dtype is not _BF16 or out.shape != (qkv.shape[0], n_heads * head_dim) or not out.is_contiguous() or out.data_ptr() % 16:
         raise KernelError(f"{what}: out must be contiguous bfloat16 [T, {n_heads * head_dim}]")
-    if tables.dim() != 2 or tables.shape[0] < n or ctx.cu_q.numel() <= n or ctx.seq_start.numel() < n or ctx.seq_qlen.numel() < n:
+    table = tables.shape
+    if len(table) != 2 or table[0] < n or cu_q.numel() <= n or start.numel() < n or qlen.numel() < n:
         raise KernelError(f"{what}: the step's tables are shorter than its {n} sequences")
-    if longest > tables.shape[1] * PAGE or cos is not None and longest > cos.shape[0]:
+    if longest > table[1] * PAGE or cos is not None and longest > cos.shape[0]:
         raise KernelError(f"{what}: a sequence of {longest} tokens is longer than its page table or the position tables")
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
@@ -148,17 +172,18 @@ def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv
     what = "kv8_write"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
-    _here(what, qkv, cos, sin, codes, scales, tables, tok_seq, tok_pos)
+    dev = _here(what, qkv, cos, sin, codes, scales, tables, tok_seq, tok_pos)
     _check_rows(what, qkv, cos, sin, (n_heads + 2 * n_kv_heads) * head_dim, head_dim)
-    _check_ints(what, tables=tables, tok_seq=tok_seq, tok_pos=tok_pos)
+    _check_ints(what, ("tables", "tok_seq", "tok_pos"), (tables, tok_seq, tok_pos))
     T = qkv.shape[0]
     if tables.dim() != 2 or tok_seq.numel() < T or tok_pos.numel() < T:
         raise KernelError(f"{what}: fewer places than the {T} tokens")
     if T == 0:
         return
-    ops._check(_lib(head_dim).oe_kv8_write(
-        kind, qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(), codes.shape[0],
-        tables.data_ptr(), tables.shape[1], tok_seq.data_ptr(), tok_pos.data_ptr(), T, n_heads, n_kv_heads, ops._stream()), what)
+    ops._check(_lib(head_dim).oe_kv8_write(_CALL.pack(
+        0, qkv.data_ptr(), qkv.stride(0), 0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), codes.data_ptr(),
+        scales.data_ptr(), codes.shape[0], tables.data_ptr(), 0, 0, 0, tok_seq.data_ptr(), tok_pos.data_ptr(), 0, 0, 0, 0, 0, 0, _stream(dev),
+        _CALL.size, kind, 1, tables.shape[1], 0, T, 0, n_heads, n_kv_heads, 0, 0, 0, 0, 1, 0, 1, 0, 0, 0, 0.0)), what)
 
 
 def many_pairs(n_seqs: int, n_kv_heads: int, sm_count: int | None = None) -> bool:
@@ -207,38 +232,30 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
     what = "attention_kv8"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
-    _here(what, out, qkv, cos, sin, codes, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen)
+    dev = _here(what, out, qkv, cos, sin, codes, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen)
     _check_rows(what, qkv, cos, sin, (n_heads + (2 * n_kv_heads if has_kv else 0)) * head_dim, head_dim)
     _check_step(what, out, qkv, cos, tables, ctx, n_heads, head_dim)
-    T = qkv.shape[0]
-    if T == 0 or ctx.n_seqs == 0:
+    T, n_seqs, sms, window = qkv.shape[0], ctx.n_seqs, _sms(dev), int(window)
+    if T == 0 or n_seqs == 0:
         return
-    single = bool(ctx.all_decode) and T == ctx.n_seqs
+    single = bool(ctx.all_decode) and T == n_seqs
     if has_kv and not single:
         kv8_write(qkv, cos, sin, cache, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
-    few = max(1, ctx.max_qlen) * (n_heads // n_kv_heads) <= FEW_ROWS
-    if single or few:
-        warps, cluster, shares = form or decode_form(ctx.n_seqs, n_kv_heads, getattr(ctx, "context_class", 0), int(window))
+    group, context_class, max_qlen = n_heads // n_kv_heads, getattr(ctx, "context_class", 0), 1 if single else max(1, ctx.max_qlen)
+    if single or max_qlen * group <= FEW_ROWS:
+        warps, cluster, shares = form or decode_form(n_seqs, n_kv_heads, context_class, window, sms)
         part = _parts(T * n_heads, shares, head_dim, out.device) if shares > 1 else None
-        parts = _part_ptrs(part, T * n_heads, shares, head_dim)
-        ops._check(_lib(head_dim).oe_attn_kv8(
-            kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(),
-            int(has_kv and single), codes.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(),
-            ctx.seq_qlen.data_ptr(), ctx.n_seqs, 1 if single else max(1, ctx.max_qlen), n_heads, n_kv_heads, int(window), float(scale),
-            warps, cluster, int(many_pairs(ctx.n_seqs, n_kv_heads)), None, 0, None, None, shares, *parts, int(ahead), ops._stream()),
-            what, {"warps": warps, "cluster": cluster, "shares": shares})
+        call = _packed(out, qkv, cos, sin, codes, scales, tables, ctx, part, T * n_heads, shares, head_dim, dev, kind, has_kv and single, max_qlen,
+                       n_heads, n_kv_heads, window, scale, ahead, warps, cluster, many_pairs(n_seqs, n_kv_heads, sms), shares)
+        ops._check(_lib(head_dim).oe_attn_kv8(call), what, {"warps": warps, "cluster": cluster, "shares": shares})
         if shares > 1:
-            ops._check(_rows_lib(head_dim).oe_join_parts(
-                out.data_ptr(), *parts, ctx.cu_q.data_ptr() + 4 * ctx.n_seqs, T, n_heads, shares, ops._stream()), "join_parts")
+            ops._check(_rows_lib(head_dim).oe_join_parts(call), "join_parts")
         return
-    mt, splits = form or prompt_form(T, ctx.n_seqs, n_heads // n_kv_heads, n_kv_heads, getattr(ctx, "context_class", 0), int(window),
-                                     max_qlen=ctx.max_qlen)
+    mt, splits = form or prompt_form(T, n_seqs, group, n_kv_heads, context_class, window, sms, ctx.max_qlen)
     part = _parts(T * n_heads, splits, head_dim, out.device) if splits > 1 else None
-    ops._check(_rows_lib(head_dim).oe_attn_rows(
-        kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), codes.data_ptr(), scales.data_ptr(), codes.shape[0],
-        tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr(), ctx.seq_qlen.data_ptr(), ctx.n_seqs, T,
-        ctx.max_qlen, n_heads, n_kv_heads, int(window), float(scale), mt, splits, *_part_ptrs(part, T * n_heads, splits, head_dim),
-        ops._stream()), what, {"tiles": mt, "splits": splits})
+    call = _packed(out, qkv, cos, sin, codes, scales, tables, ctx, part, T * n_heads, splits, head_dim, dev, kind, 0, max_qlen, n_heads, n_kv_heads,
+                   window, scale, ahead, mt=mt, splits=splits)
+    ops._check(_rows_lib(head_dim).oe_attn_rows(call), what, {"tiles": mt, "splits": splits})
     if splits > 1:
         ops.LAUNCHES[0] += 1
 
@@ -246,12 +263,6 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
 def _parts(rows: int, splits: int, head_dim: int, device):
     """Room for the parts of `rows` rows: their sums, then maxima and sums of weights."""
     return torch.empty(rows * splits * (head_dim + 2), dtype=torch.float32, device=device)
-
-
-def _part_ptrs(part, rows: int, splits: int, head_dim: int) -> tuple:
-    if part is None:
-        return None, None
-    return part.data_ptr(), part.data_ptr() + 4 * rows * splits * head_dim
 
 
 def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context_class: int, window: int, sm_count: int | None = None,
@@ -324,30 +335,24 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     _check_heads(what, n_heads, n_kv_heads, head_dim)
     kind, rows, scales = _cache_args(what, cache, n_kv_heads, head_dim, True)
     lists = (prefix.members, prefix.first, prefix.pages, prefix.seq_pages)
-    _here(what, out, qkv, cos, sin, rows, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen, *lists)
+    dev = _here(what, out, qkv, cos, sin, rows, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen, *lists)
     _check_rows(what, qkv, cos, sin, (n_heads + (2 * n_kv_heads if has_kv else 0)) * head_dim, head_dim)
     _check_step(what, out, qkv, cos, tables, ctx, n_heads, head_dim)
-    B = ctx.n_seqs
+    B, n_groups, n_members, sms = ctx.n_seqs, prefix.n_groups, prefix.n_members, _sms(dev)
     if not ctx.all_decode or qkv.shape[0] != B:
         raise KernelError(f"{what}: one token a sequence expected")
-    _check_ints(what, members=prefix.members, first=prefix.first, pages=prefix.pages, seq_pages=prefix.seq_pages)
-    for t, n, least in zip(lists, ("members", "first", "pages", "seq_pages"), (prefix.n_members, prefix.n_groups + 1, prefix.n_groups, B)):
+    names = ("members", "first", "pages", "seq_pages")
+    _check_ints(what, names, lists)
+    for t, n, least in zip(lists, names, (n_members, n_groups + 1, n_groups, B)):
         if t.numel() < least:
             raise KernelError(f"{what}: {n} holds {t.numel()} numbers, {least} are needed")
     if B == 0:
         return
-    step = (rows.shape[0], tables.data_ptr(), tables.shape[1], ctx.cu_q.data_ptr(), ctx.seq_start.data_ptr())
     mt, splits, warps, cluster = form or shared_form(
-        B, max(1, prefix.n_members), max(1, prefix.n_groups), n_heads // n_kv_heads, n_kv_heads, max(1, prefix.max_pages), scales is not None)
+        B, max(1, n_members), max(1, n_groups), n_heads // n_kv_heads, n_kv_heads, max(1, prefix.max_pages), scales is not None, sms)
     part = _parts(B * n_heads, splits, head_dim, out.device)
-    parts = _part_ptrs(part, B * n_heads, splits, head_dim)
-    if prefix.n_groups > 0 and prefix.n_members > 0:
-        ops._check(_rows_lib(head_dim).oe_attn_rows_prefix(
-            kind, qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), *step, n_heads, n_kv_heads,
-            float(scale), prefix.members.data_ptr(), prefix.first.data_ptr(), prefix.pages.data_ptr(), prefix.n_groups,
-            prefix.n_members, mt, splits, *parts, int(ahead), ops._stream()), "attention_shared_prefix", {"tiles": mt, "splits": splits})
-    ops._check(_lib(head_dim).oe_attn_kv8(
-        kind, out.data_ptr(), qkv.data_ptr(), qkv.stride(0), _ptr(cos), _ptr(sin), rows.data_ptr(), _ptr(scales), int(has_kv),
-        *step, ctx.seq_qlen.data_ptr(), B, 1, n_heads, n_kv_heads, 0, float(scale), warps, cluster,
-        int(many_pairs(B, n_kv_heads)), prefix.seq_pages.data_ptr(), splits,
-        *parts, 1, None, None, int(ahead), ops._stream()), what)
+    call = _packed(out, qkv, cos, sin, rows, scales, tables, ctx, part, B * n_heads, splits, head_dim, dev, kind, has_kv, 1, n_heads, n_kv_heads, 0,
+                   scale, ahead, warps, cluster, many_pairs(B, n_kv_heads, sms), 1, mt, splits, prefix)
+    if n_groups > 0 and n_members > 0:
+        ops._check(_rows_lib(head_dim).oe_attn_rows_prefix(call), "attention_shared_prefix", {"tiles": mt, "splits": splits})
+    ops._check(_lib(head_dim).oe_attn_kv8(call), what)

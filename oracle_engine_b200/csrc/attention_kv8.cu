@@ -44,10 +44,12 @@ constexpr int MAX_JOINED = 160;                  // parts that a result is joine
 constexpr float LOG2E = 1.4426950408889634f;
 
 // ------------------------------------------------------------------------------------------------ the write
-// keys and values of a step's tokens into the 8-bit cache.  HD / 16 lanes have a row: 8 dimensions of its lower half and the 8 that
-// they are turned with, so that a row's lanes read 16 bytes each of both halves and only its maximum crosses lanes.
-// Measured (B200): 10,235 tokens of 24 heads over 8 KV heads of 128 in int8, 46 MB, 21 us: 2.2 TB/s, bound by the loads' latency and by the
-// instructions of the exact roundings; one token 1.8 us, 64 tokens 3.6: the start of a kernel and two rounds of loads.
+// Keys and values of a step's tokens into the 8-bit cache.  HD / 16 lanes have a token's key and value of one KV head: 8 dimensions of
+// the lower half and the 8 that they are turned with, so that a row's lanes read 16 bytes each of both halves and only its maximum
+// crosses lanes.  Both rows are asked for at once and share the look-ups of the token's place.
+// Measured (B200): 10,235 tokens of 24 heads over 8 KV heads of 128 in int8, 46 MB, 16 us: 2.8 TB/s (a lane group a row: 21 us), bound by the
+// loads' latency, at 32 warps an SM, and by the instructions of the exact roundings; one token 1.9 us, 64 tokens 3.8: the start of a
+// kernel and two rounds of loads.
 template <int KIND>
 __global__ void __launch_bounds__(256)
 kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ cos_tab, const float* __restrict__ sin_tab,
@@ -56,16 +58,15 @@ kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ co
     constexpr int LANES = HD / 16;
     pdl_launch_dependents();
     pdl_wait();
-    const unsigned item = blockIdx.x * 256u + threadIdx.x, r = item / LANES;       // a row: (token, K or V, KV head)
-    const int i = (int)(item % LANES) * 8;
-    const unsigned per_token = 2u * KVH, t = r / per_token, which_head = r - t * per_token;
-    const int which = which_head >= (unsigned)KVH, kvh = (int)which_head - (which ? KVH : 0);
-    // (two rounds of loads: the row and the token's place, then the page's number and the angle)
+    const unsigned item = blockIdx.x * 256u + threadIdx.x, r = item / LANES, t = r / (unsigned)KVH;       // (token, KV head)
+    const int i = (int)(item % LANES) * 8, kvh = (int)(r - t * (unsigned)KVH);
+    // (two rounds of loads: the rows and the token's place, then the page's number and the angle)
     const bool here = t < (unsigned)n_tokens;
-    const bf16* row = qkv + (long long)(here ? t : 0) * stride + (long long)(H + which * KVH + kvh) * HD;
-    const uint4 x0 = *(const uint4*)(row + i), x1 = *(const uint4*)(row + i + HD / 2);
+    const bf16* row = qkv + (long long)(here ? t : 0) * stride + (long long)(H + kvh) * HD + i;
+    const uint4 k0 = *(const uint4*)row, k1 = *(const uint4*)(row + HD / 2);
+    const uint4 v0 = *(const uint4*)(row + KVH * HD), v1 = *(const uint4*)(row + KVH * HD + HD / 2);
     const int b = here ? tok_seq[t] : -1, pos = here ? max(tok_pos[t], 0) : 0;
-    const bool turns = which == 0 && cos_tab != nullptr && b >= 0;
+    const bool turns = cos_tab != nullptr && b >= 0;
     float cs[8], sn[8];
     if (turns) {
 #pragma unroll
@@ -76,22 +77,27 @@ kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ co
     }
     const int page = b >= 0 && pos / OE_PAGE < max_pages ? tables[(long long)b * max_pages + pos / OE_PAGE] : -1;
     const bool ok = page >= 0 && page < n_pages;
-    uint32_t lo[4] = {x0.x, x0.y, x0.z, x0.w}, hi[4] = {x1.x, x1.y, x1.z, x1.w};      // dimensions i .. i + 7, and those they are turned with
+    const long long at = ((long long)page * 2 * KVH + kvh) * OE_PAGE + pos % OE_PAGE;
+    auto quantise = [&](const uint32_t (&lo)[4], const uint32_t (&hi)[4], long long to) {      // dimensions i .. i + 7, and those they are turned with
+        uint32_t w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) most = kv8_most(most, w[j]);
+        most = kv8_most(most);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float scale;
+        const float by = kv8_row<KIND>(most, w, &scale);
+        if (!ok) return;
+        *(uint2*)(codes + to * HD + i) = make_uint2(kv8_codes4<KIND>(by, w[0], w[1]), kv8_codes4<KIND>(by, w[2], w[3]));
+        *(uint2*)(codes + to * HD + i + HD / 2) = make_uint2(kv8_codes4<KIND>(by, w[4], w[5]), kv8_codes4<KIND>(by, w[6], w[7]));
+        if (i == 0) scales[to] = scale;
+    };
+    const uint32_t vl[4] = {v0.x, v0.y, v0.z, v0.w}, vh[4] = {v1.x, v1.y, v1.z, v1.w};
+    quantise(vl, vh, at + (long long)KVH * OE_PAGE);       // (the value first: it needs no angle)
+    uint32_t lo[4] = {k0.x, k0.y, k0.z, k0.w}, hi[4] = {k1.x, k1.y, k1.z, k1.w};
     if (turns) kv8_turn<8>(lo, hi, cs, sn);
-    uint32_t w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    uint32_t most = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) most = kv8_most(most, w[j]);
-    most = kv8_most(most);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (!ok) return;
-    float scale;
-    const float by = kv8_row<KIND>(most, w, &scale);
-    const long long at = (((long long)page * 2 + which) * KVH + kvh) * OE_PAGE + pos % OE_PAGE;
-    *(uint2*)(codes + at * HD + i) = make_uint2(kv8_codes4<KIND>(by, w[0], w[1]), kv8_codes4<KIND>(by, w[2], w[3]));
-    *(uint2*)(codes + at * HD + i + HD / 2) = make_uint2(kv8_codes4<KIND>(by, w[4], w[5]), kv8_codes4<KIND>(by, w[6], w[7]));
-    if (i == 0) scales[at] = scale;
+    quantise(lo, hi, at);
 }
 
 // ------------------------------------------------------------------------------------------------ the attention
@@ -822,7 +828,7 @@ int oe_kv8_write(const Kv8Call* call) {
     if (c.bytes != (int)sizeof(Kv8Call)) return OE_ERR_UNSUPPORTED;
     if (c.n_tokens <= 0) return 0;
     if (c.stride % 8 || ((uintptr_t)c.qkv & 15) || ((uintptr_t)c.cache & 15) || ((uintptr_t)c.scales & 15)) return OE_ERR_UNSUPPORTED;
-    const long long blocks = ((long long)c.n_tokens * 2 * c.KVH * (HD / 16) + 255) / 256;
+    const long long blocks = ((long long)c.n_tokens * c.KVH * (HD / 16) + 255) / 256;
     if (blocks > 0x00ffffffLL || ((uintptr_t)c.cos_tab & 15) || ((uintptr_t)c.sin_tab & 15)) return OE_ERR_UNSUPPORTED;   // (lanes are counted in 32 bits)
     if (c.kind != OE_KV_INT8 && c.kind != OE_KV_E4M3) return OE_ERR_UNSUPPORTED;
     return oe_launch(c.kind == OE_KV_INT8 ? kv8_write_kernel<OE_KV_INT8> : kv8_write_kernel<OE_KV_E4M3>, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.qkv,

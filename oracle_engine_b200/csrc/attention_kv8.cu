@@ -54,7 +54,7 @@ template <int KIND>
 __global__ void __launch_bounds__(256)
 kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ cos_tab, const float* __restrict__ sin_tab,
                  uint8_t* codes, float* scales, long long n_pages, const int* __restrict__ tables, int max_pages,
-                 const int* __restrict__ tok_seq, const int* __restrict__ tok_pos, int n_tokens, int H, int KVH) {
+                 const int* __restrict__ tok_seq, const int* __restrict__ tok_pos, int n_tokens, int H, int KVH, int n_positions, int n_tables) {
     constexpr int LANES = HD / 16;
     pdl_launch_dependents();
     pdl_wait();
@@ -65,8 +65,9 @@ kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ co
     const bf16* row = qkv + (long long)(here ? t : 0) * stride + (long long)(H + kvh) * HD + i;
     const uint4 k0 = *(const uint4*)row, k1 = *(const uint4*)(row + HD / 2);
     const uint4 v0 = *(const uint4*)(row + KVH * HD), v1 = *(const uint4*)(row + KVH * HD + HD / 2);
-    const int b = here ? tok_seq[t] : -1, pos = here ? max(tok_pos[t], 0) : 0;
-    const bool turns = cos_tab != nullptr && b >= 0;
+    const int b = here ? tok_seq[t] : -1, pos = here ? tok_pos[t] : 0;
+    const bool placed = b >= 0 && b < n_tables && pos >= 0 && pos < n_positions;
+    const bool turns = cos_tab != nullptr && placed;
     float cs[8], sn[8];
     if (turns) {
 #pragma unroll
@@ -75,7 +76,7 @@ kv8_write_kernel(const bf16* qkv, long long stride, const float* __restrict__ co
             *(float4*)&sn[j] = *(const float4*)(sin_tab + (long long)pos * (HD / 2) + i + j);
         }
     }
-    const int page = b >= 0 && pos / OE_PAGE < max_pages ? tables[(long long)b * max_pages + pos / OE_PAGE] : -1;
+    const int page = placed && pos / OE_PAGE < max_pages ? tables[(long long)b * max_pages + pos / OE_PAGE] : -1;
     const bool ok = page >= 0 && page < n_pages;
     const long long at = ((long long)page * 2 * KVH + kvh) * OE_PAGE + pos % OE_PAGE;
     auto quantise = [&](const uint32_t (&lo)[4], const uint32_t (&hi)[4], long long to) {      // dimensions i .. i + 7, and those they are turned with
@@ -833,7 +834,7 @@ int oe_kv8_write(const Kv8Call* call) {
     if (c.kind != OE_KV_INT8 && c.kind != OE_KV_E4M3) return OE_ERR_UNSUPPORTED;
     return oe_launch(c.kind == OE_KV_INT8 ? kv8_write_kernel<OE_KV_INT8> : kv8_write_kernel<OE_KV_E4M3>, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.qkv,
                      c.stride, c.cos_tab, c.sin_tab, (uint8_t*)c.cache, c.scales, c.n_pages, c.tables, c.max_pages, c.tok_seq, c.tok_pos,
-                     c.n_tokens, c.H, c.KVH);
+                     c.n_tokens, c.H, c.KVH, c.n_positions, c.n_tables);
 }
 
 // Attention of the step's tokens over their sequences' caches (kind: OE_KV_*).  write != 0: every sequence brings one token, whose

@@ -24,8 +24,8 @@
 // scores, weights and products are, with two buffers of scores, and the waits between its warps: leaving out the exponentials, the scales'
 // loads, half of either product or half of the conversion's stores changes it by 3 % at most.  One tile, whose chain nothing else
 // hides: two threads a row 0.98, one 1.06; two tiles: 1.52 and 1.38.  Two CTAs of one tile an SM: 2,048 tokens in 90 instead of 74.  A
-// warp for each tile's products: 1.44 instead of 1.38.  A prompt of 2,048 tokens with 24 heads takes 68 (379 TFLOP/s of causal work),
-// 192 tokens with 32 heads behind 12,005 of e4m3 73 (518 TFLOP/s), joined from 6 runs; 64 members with 32 heads behind
+// warp for each tile's products: 1.44 instead of 1.38.  A prompt of 2,048 tokens with 24 heads takes 66 (390 TFLOP/s of causal
+// work), 192 tokens with 32 heads behind 12,005 of e4m3 73 (518 TFLOP/s), joined from 6 runs, both with the cache write; 64 members with 32 heads behind
 // 8,192 common tokens 50 with the kernel of their own keys (177 TFLOP/s).
 // Every wait on an mbarrier is bounded in time; one that runs out raises an error flag, every role leaves its loop, copies in
 // flight get a fixed time, and tensor memory is freed.

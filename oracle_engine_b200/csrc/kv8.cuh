@@ -46,9 +46,10 @@ struct Kv8Call {
     cudaStream_t stream;
     int bytes;                     // of this struct
     int kind, write, max_pages, n_seqs, n_tokens, max_qlen, H, KVH, window, warps, cluster, ordered, shares, mt, splits, n_groups, n_members, ahead;
+    int n_positions, n_tables;     // that the angles and the page tables are there for (the write's bounds)
     float scale;
 };
-static_assert(sizeof(Kv8Call) == 21 * 8 + 20 * 4, "as the host packs it");
+static_assert(sizeof(Kv8Call) == 21 * 8 + 22 * 4, "as the host packs it");
 
 // a * c - b * s rounded once to bfloat16.  Two float32 operations are within 2^-23 of the magnitudes they add; only a sum that near to the
 // border between two bfloat16 is taken apart: the two products into a float32 and its error each, the sum likewise, and what is left

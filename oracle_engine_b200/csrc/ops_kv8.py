@@ -32,7 +32,7 @@ _KINDS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
 _libs: dict = {}
 
 
-_CALL = struct.Struct("<21q19if")        # Kv8Call of kv8.cuh
+_CALL = struct.Struct("<21q21if")        # Kv8Call of kv8.cuh
 
 
 def _lib(head_dim: int):
@@ -75,7 +75,7 @@ def _packed(out, qkv, cos, sin, rows, scales, tables, ctx, part, part_rows: int,
         ctx.seq_qlen.data_ptr(), 0, 0, *lists,
         part_o, part_o + 4 * part_rows * parts * head_dim if part_o else 0, _stream(dev),
         _CALL.size, kind, write, max_pages, ctx.n_seqs, T, max_qlen, n_heads, n_kv_heads, window, warps, cluster, ordered, shares, mt, splits,
-        n_groups, n_members, ahead, scale)
+        n_groups, n_members, ahead, 0, 0, scale)
 
 
 def _stream(dev: int) -> int:
@@ -167,8 +167,8 @@ def _check_step(what: str, out, qkv, cos, tables, ctx, n_heads: int, head_dim: i
 
 def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
     """Keys (turned at each token's position; cos/sin float32 [max_pos, hd/2] or None) and values of the step's tokens into the
-    8-bit cache.  qkv [T, (H + 2 KVH) hd] is left as it is; tok_seq < 0: a padding row; a page outside the cache: nothing is
-    written."""
+    8-bit cache.  qkv [T, (H + 2 KVH) hd] is left as it is; tok_seq < 0: a padding row; a sequence without a table, a
+    position without an angle or a page outside the cache: nothing is written."""
     what = "kv8_write"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
@@ -183,7 +183,8 @@ def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv
     ops._check(_lib(head_dim).oe_kv8_write(_CALL.pack(
         0, qkv.data_ptr(), qkv.stride(0), 0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), codes.data_ptr(),
         scales.data_ptr(), codes.shape[0], tables.data_ptr(), 0, 0, 0, tok_seq.data_ptr(), tok_pos.data_ptr(), 0, 0, 0, 0, 0, 0, _stream(dev),
-        _CALL.size, kind, 1, tables.shape[1], 0, T, 0, n_heads, n_kv_heads, 0, 0, 0, 0, 1, 0, 1, 0, 0, 0, 0.0)), what)
+        _CALL.size, kind, 1, tables.shape[1], 0, T, 0, n_heads, n_kv_heads, 0, 0, 0, 0, 1, 0, 1, 0, 0, 0,
+        2 ** 31 - 1 if cos is None else cos.shape[0], tables.shape[0], 0.0)), what)
 
 
 def many_pairs(n_seqs: int, n_kv_heads: int, sm_count: int | None = None) -> bool:

@@ -68,6 +68,17 @@ def test_write_leaves_padding_and_unmapped_pages_alone():
     assert torch.equal(codes, s.cache[0]) and torch.equal(scales.nan_to_num(-1), s.cache[1].nan_to_num(-1))
 
 
+def test_write_leaves_places_that_are_not_there_alone():
+    """A sequence behind the page tables, a position behind the angles or before the first: the other tokens are written."""
+    from oracle_engine_b200.csrc import ops_kv8
+    s = Step([0], [6], 4, 2, 64, torch.int8, seed=3)
+    s.ctx.tok_seq[1], s.ctx.tok_pos[2], s.ctx.tok_pos[3] = 1, 1000, -5
+    ops_kv8.kv8_write(s.qkv, s.cos, s.sin, s.cache, s.tables, s.ctx.tok_seq, s.ctx.tok_pos, 4, 2, 64)
+    page = s.tables_list[0][0]
+    written = ~torch.isnan(s.cache[1]).cpu()
+    assert written[page, :, :, [0, 4, 5]].all() and written.sum() == 3 * 2 * 2
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("H,KVH,hd", HEADS)
 @pytest.mark.parametrize("window", [0, 1, 50, 64, -64, -100])

@@ -174,17 +174,22 @@ def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
     dev = _here(what, qkv, cos, sin, codes, scales, tables, tok_seq, tok_pos)
     _check_rows(what, qkv, cos, sin, (n_heads + 2 * n_kv_heads) * head_dim, head_dim)
+    _write(what, dev, kind, qkv, cos, sin, codes, scales, tables, tok_seq, tok_pos, n_heads, n_kv_heads, head_dim)
+
+
+def _write(what: str, dev: int, kind: int, qkv, cos, sin, codes, scales, tables, tok_seq, tok_pos, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+    """kv8_write of rows and a cache that have been checked."""
     _check_ints(what, ("tables", "tok_seq", "tok_pos"), (tables, tok_seq, tok_pos))
-    T = qkv.shape[0]
-    if tables.dim() != 2 or tok_seq.numel() < T or tok_pos.numel() < T:
+    T, table = qkv.shape[0], tables.shape
+    if len(table) != 2 or tok_seq.numel() < T or tok_pos.numel() < T:
         raise KernelError(f"{what}: fewer places than the {T} tokens")
     if T == 0:
         return
     ops._check(_lib(head_dim).oe_kv8_write(_CALL.pack(
         0, qkv.data_ptr(), qkv.stride(0), 0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), codes.data_ptr(),
         scales.data_ptr(), codes.shape[0], tables.data_ptr(), 0, 0, 0, tok_seq.data_ptr(), tok_pos.data_ptr(), 0, 0, 0, 0, 0, 0, _stream(dev),
-        _CALL.size, kind, 1, tables.shape[1], 0, T, 0, n_heads, n_kv_heads, 0, 0, 0, 0, 1, 0, 1, 0, 0, 0,
-        2 ** 31 - 1 if cos is None else cos.shape[0], tables.shape[0], 0.0)), what)
+        _CALL.size, kind, 1, table[1], 0, T, 0, n_heads, n_kv_heads, 0, 0, 0, 0, 1, 0, 1, 0, 0, 0,
+        2 ** 31 - 1 if cos is None else cos.shape[0], table[0], 0.0)), "kv8_write")
 
 
 def many_pairs(n_seqs: int, n_kv_heads: int, sm_count: int | None = None) -> bool:
@@ -241,7 +246,8 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
         return
     single = bool(ctx.all_decode) and T == n_seqs
     if has_kv and not single:
-        kv8_write(qkv, cos, sin, cache, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
+        _here(what, out, ctx.tok_seq, ctx.tok_pos)
+        _write(what, dev, kind, qkv, cos, sin, codes, scales, tables, ctx.tok_seq, ctx.tok_pos, n_heads, n_kv_heads, head_dim)
     group, context_class, max_qlen = n_heads // n_kv_heads, getattr(ctx, "context_class", 0), 1 if single else max(1, ctx.max_qlen)
     if single or max_qlen * group <= FEW_ROWS:
         warps, cluster, shares = form or decode_form(n_seqs, n_kv_heads, context_class, window, sms)

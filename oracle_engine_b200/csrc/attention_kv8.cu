@@ -122,6 +122,8 @@ struct Args {
     float scale_log2;
     int cluster;               // CTAs that share a tile of rows
     int ahead;                 // rows of earlier tokens may be read before the wait
+    int late;                  // the kernel before this one is that of the prefixes, which lets this one start when what it waits for is
+                               // done: only its parts have to be waited for
     int ordered;               // n: blockIdx.z counts the n sequences by their lengths, the longest first
     // sequences that begin with the same pages: what attention_rows.cu has left of those pages
     const int* seq_pages;      // [B] pages of the sequence's prefix (0: none); null: no prefixes
@@ -245,7 +247,7 @@ struct NewToken {
         const bf16* src = row + (size_t)(a.H + (lane & 1) * a.KVH + kvh) * HD + d;
         uint32_t lo[PP], hi[PP], most = 0;
 #pragma unroll
-        for (int j = 0; j < PP; j++) { lo[j] = *(const uint32_t*)(src + 2 * j); hi[j] = *(const uint32_t*)(src + HD / 2 + 2 * j); }
+        for (int j = 0; j < PP; j++) { lo[j] = __ldcg((const uint32_t*)(src + 2 * j)); hi[j] = __ldcg((const uint32_t*)(src + HD / 2 + 2 * j)); }
         if (!(lane & 1) && a.cos_tab != nullptr) {
             float cs[2 * PP], sn[2 * PP];
 #pragma unroll
@@ -355,8 +357,8 @@ attn_kv8_kernel(const Args a) {
     const bool own_kv = a.cache_w != nullptr;
     // where the caller says so, keys and values of earlier steps are asked for before the wait: only the new token's q, k and v
     // come from the kernel before this one
-    const bool ahead = a.ahead && own_kv;
-    if (!ahead) pdl_wait();
+    const bool ahead = a.ahead && own_kv && !a.late;
+    if (!ahead && !a.late) pdl_wait();
     // The queries of the rows nt * 8 + gid, 4 dimensions that lie together a k-step, and their angles: asked for before the tiles where
     // the kernel before this one has been waited for, since a score needs both.
     uint2 qw[NT][KS];
@@ -367,7 +369,7 @@ attn_kv8_kernel(const Args a) {
             const int r = nt * 8 + gid, rr = row0 + (r < rows ? r : 0);
             const bf16* src = a.q + (packed0 + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * HD + tig * 4;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) qw[nt][ks] = r < rows ? *(const uint2*)(src + ks * 16) : make_uint2(0u, 0u);
+            for (int ks = 0; ks < KS; ks++) qw[nt][ks] = r < rows ? __ldcg((const uint2*)(src + ks * 16)) : make_uint2(0u, 0u);
             if (a.cos_tab != nullptr) {
                 const size_t at = (size_t)(start + rr / G) * (HD / 2) + tig * 4;
 #pragma unroll
@@ -702,6 +704,7 @@ attn_kv8_kernel(const Args a) {
         }
     }
     __syncthreads();
+    if (a.late) pdl_wait();
     const int n_pre = common > 0 ? a.splits : 0;
     const bool alone = CR == 1 && a.shares == 1 && n_pre == 0;           // nothing to join: the sum is the result
     for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += NW * 32) {
@@ -839,7 +842,7 @@ int oe_kv8_write(const Kv8Call* call) {
 
 // Attention of the step's tokens over their sequences' caches (kind: OE_KV_*).  write != 0: every sequence brings one token, whose
 // key and value this kernel writes.  With seq_pages the pages before a sequence's own are left out and the parts that
-// oe_attn_rows_prefix left (`splits` a row) are added.  shares > 1: as many CTAs share a tile's keys and leave their parts (oe_join_parts).
+// oe_attn_rows_prefix, launched right before with the same argument, left (`splits` a row) are added.  shares > 1: as many CTAs share a tile's keys and leave their parts (oe_join_parts).
 int oe_attn_kv8(const Kv8Call* call) {
     const Kv8Call& c = *call;
     if (c.bytes != (int)sizeof(Kv8Call)) return OE_ERR_UNSUPPORTED;
@@ -857,6 +860,7 @@ int oe_attn_kv8(const Kv8Call* call) {
     a.n_pages = c.n_pages; a.tables = c.tables; a.max_pages = c.max_pages; a.cu_q = c.cu_q; a.seq_start = c.seq_start; a.seq_qlen = c.seq_qlen;
     a.H = c.H; a.KVH = c.KVH; a.window = c.window; a.scale_log2 = c.scale * LOG2E; a.cluster = c.cluster;
     a.seq_pages = c.seq_pages; a.splits = c.splits; a.ahead = c.ahead; a.shares = c.shares;
+    a.late = c.seq_pages != nullptr && c.n_groups > 0 && c.n_members > 0;
     if (c.seq_pages != nullptr) { a.part_o = c.part_o; a.part_ml = c.part_ml; }
     else { a.own_o = c.part_o; a.own_ml = c.part_ml; }
     a.ordered = c.ordered && c.window == 0 && c.n_seqs > 1 && c.n_seqs <= MAX_ORDERED ? c.n_seqs : 0;

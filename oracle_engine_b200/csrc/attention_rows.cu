@@ -378,8 +378,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         t0 = ((int)gridDim.z - 1 - (int)blockIdx.z) * MT * tpt;     // the heaviest tiles first
     }
     if (t0 >= count) {
-        pdl_launch_dependents();
         pdl_wait();
+        pdl_launch_dependents();
         return;
     }
     int any = 0;                                           // the most pages a tile has
@@ -432,10 +432,12 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     __syncthreads();
     fence_after();
     const uint32_t tmem_base = *(volatile uint32_t*)&ctl->tmem_base;
-    pdl_launch_dependents();
-    // prefixes: where the caller says so, the pages are asked for before the wait; the queries come from the kernel before
+    // prefixes: where the caller says so, the pages are asked for before the wait; the queries come from the kernel before.  The kernel
+    // of the own keys may start when that one is done: it waits for this one only where it needs the parts
+    if (!PREFIX) pdl_launch_dependents();
     const bool ahead = PREFIX && a.ahead;
     if (!ahead || warp >= 4) pdl_wait();
+    if (PREFIX && warp >= 4) pdl_launch_dependents();
 
     // The queries, turned, by all warps from 4 on: HD / 16 lanes have a row, 8 dimensions of its lower half and the 8 that they are
     // turned with each.  Several rows' pieces are asked for before the first is used: the start of a CTA is these loads.

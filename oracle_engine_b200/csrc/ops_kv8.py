@@ -300,31 +300,34 @@ def prompt_form(n_tokens: int, n_seqs: int, group: int, n_kv_heads: int, context
 
 def sharing_pays(groups: list, eight: bool) -> bool:
     """Whether a step's groups, (members, pages in common) each, are read faster by attention_shared than sequence by sequence, where
-    the common pages come out of the L2 for all but the first.  Measured with 24 heads over 8 KV heads of 128, 100 keys behind the prefix.
-    ms a decode step of 28 layers, shared / apart, prefix of 4,096 tokens: 16-bit cache, 8 members 2.53 / 2.49, 16 2.29 / 2.74, 32 2.98 /
-    3.89, 64 3.48 / 5.61; int8, 8 2.07 / 2.12, 16 2.23 / 2.79, 32 2.85 / 4.10, 64 3.23 / 6.01.  us of the attention alone, prefixes of
-    1,024 / 2,048 / 4,096 / 8,192, 16-bit: 2 members 17/7, 19/9, 21/14, 27/22; 8 19/12, 20/20, 22/36, 28/66; 16 18/13, 19/21, 22/37, 28/67;
-    32 21/19, 23/33, 27/60, 32/115; 64 36/35, 38/66, 42/119, 50/226; int8: 2 17/10, 19/13, 21/14, 25/17; 8 18/13, 20/16, 22/25, 27/40; 16
-    17/14, 19/22, 21/38, 26/69; 32 18/22, 20/38, 22/67, 27/128; 64 29/44, 31/73, 37/133, 46/252."""
-    base = 256 if eight else 768
-    return sum(members * (pages * PAGE - base) for members, pages in groups if pages * PAGE > base) >= 32768
+    the common pages come out of the L2 for all but the first.  Measured with 24 heads over 8 KV heads of 128, 100 keys behind the prefix: ms
+    a decode step of 28 layers, shared / apart, prefixes of 1,024, 2,048, 4,096, 8,192 tokens.  16-bit cache: 2 members 2.21/1.56,
+    2.28/1.61, 2.42/1.74, 2.65/1.96; 4 2.22/1.63, 2.30/1.74, 2.44/1.97, 2.64/2.41; 8 2.03/1.77, 2.13/2.00, 2.27/2.46, 2.47/3.29; 16 2.00/2.04,
+    2.06/2.27, 2.17/2.71, 2.37/3.56; 32 2.73/2.62, 2.78/3.01, 2.83/3.79.  int8: 2 1.73/1.62, 1.79/1.68, 1.92/1.73, 2.12/1.85; 4 1.77/1.67,
+    1.83/1.78, 1.93/2.01, 2.14/2.45; 8 1.86/1.78, 1.91/1.89, 2.02/2.12, 2.22/2.56; 16 2.00/2.08, 2.06/2.32, 2.17/2.76, 2.37/3.61; 32
+    2.69/2.75, 2.72/3.19, 2.77/4.05."""
+    less, base = (1, 256) if eight else (3, 768)
+    return sum((members - less) * (pages * PAGE - base) for members, pages in groups if members > less and pages * PAGE > base) >= 11500
 
 
 def shared_form(n_seqs: int, n_members: int, n_groups: int, group: int, n_kv_heads: int, max_pages: int, eight: bool,
                 sm_count: int | None = None) -> tuple:
     """(tiles of 128 rows a CTA has, runs that a prefix's pages are cut into; warps of a CTA and CTAs of a cluster for the keys behind
     the prefixes).  One tile, so that there are fewer parts to join, unless the tiles alone outnumber the SMs (us, 64 members of 32
-    heads behind 8,192 tokens in 8 bits: two tiles and 18 runs 54.0, one tile and 9 runs 53.1; behind 2,048 44.0 / 39.8).  As many runs as
-    give every SM a CTA (16 members of 24 heads behind 4,096, ms a decode step of 28 layers: 18 runs 2.23, 9 2.41, 4 2.66).  Own keys: CTAs
-    of all an SM has room for while the pairs have an SM each (12 / 4 warps: 8 members 2.07 / 2.10, 32 2.99 / 2.85, 64 3.60 / 3.23), no
-    clusters (8 members, two CTAs of 12 warps a pair: 2.61)."""
+    heads behind 8,192 tokens in 8 bits: two tiles and 18 runs 54.0, one tile and 9 runs 53.1; behind 2,048 44.0 / 39.8).  The two kernels
+    run beside each other: as many runs as give half of the SMs a CTA while the own keys' CTAs fit the other half, else as many as
+    give every SM one (us, 24 heads, runs of half / of all SMs: 8 members behind 2,048 tokens 14.8 / 21.4, in 8 bits 14.2 / 21.3; 16 behind
+    4,096 21.7 / 25.6, 18.1 / 23.7; 32 in 8 bits 30.9 / 28.1).  Own keys: CTAs of all an SM has room for while they have an SM each, no clusters
+    (8 members, 9 runs, 6 / 3 warps 14.8 / 15.9; 16 24.9 / 21.7)."""
     sms = sm_count or ops.sm_count()
     tiles = -(-n_members // (TILE_ROWS // group))
     mt = 2 if tiles * n_kv_heads > sms else 1
     ctas = max(-(-tiles // mt), n_groups) * n_kv_heads          # (groups of equal size)
-    pairs = n_seqs * n_kv_heads
-    return (mt, max(1, min(max_pages, sms // ctas, MAX_SPLITS)),
-            (12 if eight else 6) if pairs <= sms else (4 if eight else 3), 1)
+    pairs, few = n_seqs * n_kv_heads, 4 if eight else 3
+    half = sms // 2
+    beside = pairs <= 3 * half and ctas <= half
+    warps = few if pairs > (half if beside else sms) else 12 if eight else 6
+    return mt, max(1, min(max_pages, (half if beside else sms) // ctas, MAX_SPLITS)), warps, 1
 
 
 def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,

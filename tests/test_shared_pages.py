@@ -215,7 +215,8 @@ def test_when_sharing_pays():
     assert not sharing_pays([], False) and not sharing_pays([(2, 1), (60, 1)], False)
     assert sharing_pays([(16, 64)], False) and sharing_pays([(64, 32)], False) and not sharing_pays([(16, 16)], False)
     assert sharing_pays([(64, 16)], True) and not sharing_pays([(2, 64)], True) and sharing_pays([(6, 64), (4, 64)], True)
-    assert shared_prefixes([(1, 3), (1, 3)], 2) is None and shared_prefixes([(1, 300), (1, 300)], 2) is not None
+    assert sharing_pays([(8, 64)], False) and not sharing_pays([(2, 300)], False) and not sharing_pays([(4, 128)], False)
+    assert shared_prefixes([(1, 3)] * 8, 8) is None and shared_prefixes([(1, 300)] * 8, 8) is not None
 
 
 def test_groups_of_a_step(monkeypatch):

@@ -103,6 +103,32 @@ def test_a_common_page_that_is_not_there(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ahead", [False, True])
+def test_tokens_one_after_the_other(dtype, ahead):
+    """Every call reads what the call before wrote, with nothing between them; with ahead, another kernel."""
+    n, H, KVH, hd = 40, 6, 2, 64
+    s = Step([150 + n, 128 + n, 191 + n, 40 + n], [1] * 4, H, KVH, hd, dtype, seed=14, prefixes=[(0, 2)] * 3 + [None])
+    first = [x - n for x in s.starts]
+    g = torch.Generator().manual_seed(1)
+    rows = torch.randn(n, *s.qkv.shape, generator=g).to(torch.bfloat16).cuda()
+    starts = torch.tensor([[x + i for x in first] for i in range(n)], dtype=torch.int32, device="cuda")
+    outs = []
+    torch.cuda.synchronize()
+    for i in range(n):
+        s.qkv, s.ctx.seq_start = rows[i].clone() if ahead else rows[i], starts[i]
+        outs.append(s.shared_out(ahead=ahead))
+    for i in range(n):
+        s.qkv, s.starts = rows[i], [x + i for x in first]
+        want, tol, cache = s.truth()
+        close(outs[i], want, tol)
+        if dtype == torch.bfloat16:
+            s.rows64 = cache
+        else:
+            s.codes64, s.scales64 = cache
+            s.rows64 = s.codes64 * s.scales64[..., None]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_queries_only(dtype):
     s = Step([128, 140], [1, 1], 8, 4, 64, dtype, seed=7, prefixes=[(0, 2)] * 2, has_kv=False)
     want, tol, cache = s.truth()

@@ -339,7 +339,7 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     prefix: n_groups and n_members (host numbers, or bounds for them: what first and members hold beyond the real ones are
     groups without members), max_pages (the most pages a group has in common), and int32 tensors members (sequences in the order of
     their groups), first [n_groups + 1] (where each group's members begin), pages [n_groups] (full pages that the group's
-    tables begin with), seq_pages [n_seqs] (those of the sequence's group, 0 for a sequence in none).
+    tables begin with, whose tokens are all earlier than the step's), seq_pages [n_seqs] (those of the sequence's group, 0 for a sequence in none).
     form: the kernels' form; None: by shared_form."""
     what = "attention_shared"
     _check_heads(what, n_heads, n_kv_heads, head_dim)

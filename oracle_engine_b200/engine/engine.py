@@ -175,8 +175,11 @@ class _Backend:
 
     def alloc_behind(self, prefix_slot, request_index, prompt, params):
         slot = self.e.fork(prefix_slot)
-        self.e.sampler.start_sequence(slot, params.seed + request_index, prompt, params)
+        self.take_prefix(slot, request_index, prompt, params)
         return slot
+
+    def take_prefix(self, prefix_slot, request_index, prompt, params):
+        self.e.sampler.start_sequence(prefix_slot, params.seed + request_index, prompt, params)
 
     def check(self):
         self.e.check_device_errors()

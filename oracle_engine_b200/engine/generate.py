@@ -47,6 +47,8 @@ class GenerationBackend:
     # A backend whose sequences can begin with another's cache has, for `share_prefix`:
     #   alloc_prefix() -> slot                                          an empty slot for the common tokens
     #   alloc_behind(prefix_slot, request_index, prompt, params) -> slot    as alloc, with the prefix slot's tokens in it
+    # and optionally, without which the prefix needs a slot beside those of the batch's requests:
+    #   take_prefix(prefix_slot, request_index, prompt, params)         the prefix's slot becomes that of a request behind it
 
     # A backend that can run one step ahead of the host sets `supports_lookahead` and has:
     #   sample_async(logits, slots, params) -> handle     sampling started, tokens not yet read
@@ -82,6 +84,29 @@ def common_prefixes(prompts: list, requests: list) -> list:
     return found
 
 
+def begin_behind_common(backend, prompts, batch, params, max_step_tokens, slots: dict, fed: dict) -> None:
+    """What requests of a batch have in common goes through the model; these requests get their slots behind it (`slots`, and in
+    `fed` how many tokens of their prompts that was)."""
+    take = getattr(backend, "take_prefix", None)
+    for members, n in common_prefixes(prompts, batch):
+        base = backend.alloc_prefix()
+        try:
+            common = prompts[members[0]][:n]
+            portion = max_step_tokens or n
+            for at in range(0, n, portion):
+                backend.step([SequenceStep(base, common[at:at + portion], [])])
+            for i in members if take is None else members[:-1]:
+                slots[i] = backend.alloc_behind(base, i, prompts[i], params)
+                fed[i] = n
+            if take is not None:                 # the last one goes on in the common tokens' own slot: the batch needs no more
+                i = members[-1]                  # slots than without common beginnings
+                take(base, i, prompts[i], params)
+                slots[i], fed[i], base = base, n, None
+        finally:
+            if base is not None:
+                backend.free(base)
+
+
 def run_generation(backend: GenerationBackend, prompts, params, batch_size: int | None = None,
                    stop_ids=(), on_token=None, max_step_tokens: int | None = None,
                    share_prefix: bool = False) -> list[GenerationResult]:
@@ -114,18 +139,7 @@ def run_generation(backend: GenerationBackend, prompts, params, batch_size: int 
         try:
             fed = {i: 0 for i in batch}            # prompt tokens given to the step function so far
             if share_prefix and params.n_predict > 0:
-                for members, n in common_prefixes(prompts, batch):
-                    base = backend.alloc_prefix()
-                    try:
-                        common = prompts[members[0]][:n]
-                        portion = max_step_tokens or n
-                        for at in range(0, n, portion):
-                            backend.step([SequenceStep(base, common[at:at + portion], [])])
-                        for i in members:
-                            slots[i] = backend.alloc_behind(base, i, prompts[i], params)
-                            fed[i] = n
-                    finally:
-                        backend.free(base)
+                begin_behind_common(backend, prompts, batch, params, max_step_tokens, slots, fed)
             for i in batch:
                 if i not in slots:
                     slots[i] = backend.alloc(i, prompts[i], params)

@@ -1,0 +1,37 @@
+"""Engines whose requests start behind what their prompts have in common."""
+import pytest
+
+import helpers
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("params", [dict(temperature=0.0), dict(temperature=0.8, top_k=30, repeat_penalty=1.2, seed=5)])
+def test_as_many_slots_as_requests(model_dirs, params):
+    """Tokens, random draws among them, are those of the batch without common beginnings."""
+    from oracle_engine_b200 import GenParams
+    from oracle_engine_b200.engine.engine import Engine
+    eng = Engine.from_pretrained(model_dirs["E"], dtype="float32", max_tokens=2048, n_slots=4)
+    common = helpers.random_tokens(150, 389, 1)
+    prompts = [common + helpers.random_tokens(3 + 20 * i, 389, 2 + i) for i in range(4)]
+    p = GenParams(n_predict=6, ignore_eos=True, **params)
+    want = eng.generate(prompts, p)
+    for _ in range(2):
+        assert eng.generate(prompts, p, share_prefix=True) == want
+        eng.cache.check()
+    assert eng.cache.slots.n_free == 4
+
+
+def test_recurrent_layers_in_the_common_tokens_own_slot(tmp_path):
+    import fuvipel_models as fm
+    from oracle_engine_b200 import GenParams
+    from oracle_engine_b200.engine.engine import Engine
+    eng = Engine.from_pretrained(fm.write(tmp_path, *fm.ALL["F1"]), dtype="float32", max_tokens=1024, n_slots=3)
+    common = helpers.random_tokens(64, 300, 6)
+    prompts = [common + helpers.random_tokens(4 + i, 300, 7 + i) for i in range(3)]
+    p = GenParams.greedy(5, ignore_eos=True)
+    alone = [eng.generate([q], p)[0] for q in prompts]
+    shared = eng.generate(prompts, p, share_prefix=True)
+    cut = [eng.generate([q], p, max_step_tokens=64)[0] for q in prompts]
+    assert shared in (alone, cut)
+    eng.cache.check()

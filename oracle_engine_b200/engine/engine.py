@@ -140,8 +140,8 @@ class Engine:
         of a token while the step after it is already running).  max_step_tokens: the most
         prompt tokens a step takes; longer prompts go through in portions (bounds the memory
         of a step's activations; None: every prompt whole).  share_prefix: whole pages of 64 tokens with which prompts of a batch
-        begin alike go through the model once, are kept once, and are read once a step for all of these requests (the results
-        may round differently).  Raises RuntimeError if a kernel
+        begin alike go through the model once and are kept once, those that only some of the prompts share among them; a step may read
+        what a group of requests has in common once for all of them (the results may round differently).  Raises RuntimeError if a kernel
         reported an error during a batch (the tokens of that batch are then not returned)."""
         params = params or GenParams()
         backend = _Backend(self)
@@ -177,6 +177,9 @@ class _Backend:
         slot = self.e.fork(prefix_slot)
         self.take_prefix(slot, request_index, prompt, params)
         return slot
+
+    def fork_prefix(self, prefix_slot):
+        return self.e.fork(prefix_slot)
 
     def take_prefix(self, prefix_slot, request_index, prompt, params):
         self.e.sampler.start_sequence(prefix_slot, params.seed + request_index, prompt, params)

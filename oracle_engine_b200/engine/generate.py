@@ -47,8 +47,11 @@ class GenerationBackend:
     # A backend whose sequences can begin with another's cache has, for `share_prefix`:
     #   alloc_prefix() -> slot                                          an empty slot for the common tokens
     #   alloc_behind(prefix_slot, request_index, prompt, params) -> slot    as alloc, with the prefix slot's tokens in it
-    # and optionally, without which the prefix needs a slot beside those of the batch's requests:
-    #   take_prefix(prefix_slot, request_index, prompt, params)         the prefix's slot becomes that of a request behind it
+    # and optionally
+    #   take_prefix(prefix_slot, request_index, prompt, params)         the prefix's slot becomes that of a request behind it; without
+    #                                                                   it prefixes need slots beside those of the batch's requests
+    #   fork_prefix(prefix_slot) -> slot                                another prefix that goes on behind this one; without it only
+    #                                                                   what all requests with the same first page share is shared
 
     # A backend that can run one step ahead of the host sets `supports_lookahead` and has:
     #   sample_async(logits, slots, params) -> handle     sampling started, tokens not yet read
@@ -58,13 +61,14 @@ class GenerationBackend:
     supports_lookahead = False
 
 
-def common_prefixes(prompts: list, requests: list) -> list:
-    """[(requests, tokens)] of the requests whose prompts begin alike: those with the same first page, two at least, and how many
-    tokens all of them have in common, in whole pages, at least one token of every prompt left."""
+def common_prefixes(prompts: list, requests: list, held: int = 0) -> list:
+    """[(requests, tokens)] of the requests whose prompts begin alike: those with the same page behind the first `held` tokens, which
+    all of them have in common, two at least, and how many tokens all of them have in common, in whole pages, at least one token of
+    every prompt left."""
     groups: dict = {}
     for i in requests:
-        if len(prompts[i]) > PAGE:
-            groups.setdefault(tuple(prompts[i][:PAGE]), []).append(i)
+        if len(prompts[i]) > held + PAGE:
+            groups.setdefault(tuple(prompts[i][held:held + PAGE]), []).append(i)
     found = []
     for members in groups.values():
         if len(members) < 2:
@@ -72,7 +76,7 @@ def common_prefixes(prompts: list, requests: list) -> list:
         base = prompts[members[0]]
         n = min(len(prompts[i]) for i in members) - 1
         for i in members[1:]:
-            p, lo, hi = prompts[i], 0, n
+            p, lo, hi = prompts[i], held, n
             while lo < hi:                               # the largest k <= n with equal first k tokens
                 mid = (lo + hi + 1) // 2
                 if p[lo:mid] == base[lo:mid]:
@@ -84,27 +88,68 @@ def common_prefixes(prompts: list, requests: list) -> list:
     return found
 
 
+def run_portions(backend, parts: list, max_step_tokens) -> None:
+    """(slot, tokens) pairs through the model in as few steps as may be, no logits wanted."""
+    seqs, room = [], max_step_tokens
+    for slot, tokens in parts:
+        at = 0
+        while at < len(tokens):
+            n = len(tokens) - at if room is None else min(len(tokens) - at, room)
+            seqs.append(SequenceStep(slot, tokens[at:at + n], []))
+            at += n
+            if room is not None:
+                room -= n
+                if room == 0:
+                    backend.step(seqs)
+                    seqs, room = [], max_step_tokens
+    if seqs:
+        backend.step(seqs)
+
+
 def begin_behind_common(backend, prompts, batch, params, max_step_tokens, slots: dict, fed: dict) -> None:
     """What requests of a batch have in common goes through the model; these requests get their slots behind it (`slots`, and in
-    `fed` how many tokens of their prompts that was)."""
-    take = getattr(backend, "take_prefix", None)
-    for members, n in common_prefixes(prompts, batch):
-        base = backend.alloc_prefix()
-        try:
-            common = prompts[members[0]][:n]
-            portion = max_step_tokens or n
-            for at in range(0, n, portion):
-                backend.step([SequenceStep(base, common[at:at + portion], [])])
-            for i in members if take is None else members[:-1]:
-                slots[i] = backend.alloc_behind(base, i, prompts[i], params)
-                fed[i] = n
-            if take is not None:                 # the last one goes on in the common tokens' own slot: the batch needs no more
-                i = members[-1]                  # slots than without common beginnings
-                take(base, i, prompts[i], params)
-                slots[i], fed[i], base = base, n, None
-        finally:
-            if base is not None:
-                backend.free(base)
+    `fed` how many tokens of their prompts that was).
+
+    The prompts' pages are a tree: behind what all requests of a group have in common some of them may have more in common.  A group's
+    common tokens lie in a slot of their own, its base; the groups of one depth go through the model together; then
+    every group within a group gets a base forked from that one's, and every other request its slot.  The last of these branches goes
+    on in the base itself, so that the batch needs no more slots than without common beginnings."""
+    take, fork = getattr(backend, "take_prefix", None), getattr(backend, "fork_prefix", None)
+    bases: list = []                                     # slots that are no request's
+    try:
+        level = []                                       # (base, requests, tokens it holds, tokens they have in common)
+        for members, n in common_prefixes(prompts, batch):
+            bases.append(backend.alloc_prefix())
+            level.append((bases[-1], members, 0, n))
+        while level:
+            run_portions(backend, [(base, prompts[members[0]][at:n]) for base, members, at, n in level], max_step_tokens)
+            deeper = []
+            for base, members, _, n in level:
+                inner = common_prefixes(prompts, members, n) if fork is not None else []
+                within = {i for group, _ in inner for i in group}
+                alone = [i for i in members if i not in within]
+                goes_on = inner.pop() if take is not None and not alone else None
+                for group, m in inner:
+                    bases.append(fork(base))
+                    deeper.append((bases[-1], group, n, m))
+                if goes_on is not None:
+                    deeper.append((base, goes_on[0], n, goes_on[1]))
+                    continue
+                for i in alone if take is None else alone[:-1]:
+                    slots[i] = backend.alloc_behind(base, i, prompts[i], params)
+                    fed[i] = n
+                if take is None:
+                    bases.remove(base)
+                    backend.free(base)
+                else:
+                    i = alone[-1]
+                    take(base, i, prompts[i], params)
+                    bases.remove(base)
+                    slots[i], fed[i] = base, n
+            level = deeper
+    finally:
+        for base in bases:
+            backend.free(base)
 
 
 def run_generation(backend: GenerationBackend, prompts, params, batch_size: int | None = None,
@@ -115,7 +160,7 @@ def run_generation(backend: GenerationBackend, prompts, params, batch_size: int 
     portion that does not end its prompt wants no logits; a request whose prompt is complete
     decodes one token per step in the same steps in which later requests still bring portions;
     a request that got no room in a step is left out of it.  The tokens are the same either way.
-    share_prefix: what prompts of a batch have in common (`common_prefixes`) goes through the model once, in steps of its own
+    share_prefix: what prompts of a batch have in common (`begin_behind_common`) goes through the model once, in steps of its own
     before the batch's first one, and the requests begin behind it."""
     params.validate()
     prompts = [list(p) for p in prompts]

@@ -87,3 +87,83 @@ def test_slots_go_back_when_a_request_cannot_start(fails):
     with pytest.raises(RuntimeError if fails else IndexError):
         run_generation(b, [common + [i] for i in range(4)], GenParams.greedy(1), share_prefix=True)
     assert sorted(b.free_slots) == list(range(4 if fails else 3))
+
+
+class Tree(Plain):
+    def fork_prefix(self, base):
+        assert self.owner[base] == "prefix"
+        slot = self.alloc_prefix()
+        self._note(slot, self.held[base])
+        return slot
+
+
+def _tree(prompts, portion=None):
+    n = len(prompts)
+    b = Tree([[5, 6]] * n, n_slots=n, max_seq_len=10000)
+    got = run_generation(b, prompts, GenParams.greedy(2), max_step_tokens=portion, share_prefix=True)
+    assert [g.tokens for g in got] == [[5, 6]] * n
+    mine, prefix = b.fed()
+    assert sorted(b.free_slots) == list(range(n))
+    for i, p in enumerate(prompts):
+        own = mine[i][:-1]                       # (the last one is its first token)
+        assert own and own == p[len(p) - len(own):]
+    if portion is not None:
+        assert all(sum(len(t) for t in st) <= portion for st in prefix)
+    return {i: len(p) - len(mine[i]) + 1 for i, p in enumerate(prompts)}, prefix
+
+
+@pytest.mark.parametrize("portion", [None, 100])
+def test_one_request_that_shares_little_does_not_take_it_from_the_others(portion):
+    long = list(range(1000))
+    prompts = [long + [2000 + i] for i in range(5)] + [long[:64] + [1]]
+    shared, prefix = _tree(prompts, portion)
+    assert shared == {0: 960, 1: 960, 2: 960, 3: 960, 4: 960, 5: 64}
+    assert sum(len(t) for st in prefix for t in st) == 960
+
+
+def test_two_documents_behind_one_text():
+    text, docs = list(range(128)), [list(range(1000, 1320)), list(range(2000, 2200))]
+    prompts = [text + docs[i % 2] + [i] for i in range(6)]
+    shared, prefix = _tree(prompts)
+    assert shared == {i: 448 if i % 2 == 0 else 320 for i in range(6)}
+    # the text in one step, what the documents' requests have in common in one more
+    assert [sorted(len(t) for t in st) for st in prefix] == [[128], [192, 320]]
+
+
+def test_every_prompt_goes_on_from_the_one_before():
+    talk = list(range(64 * 6))
+    shared, prefix = _tree([talk[:64 * k] + [9000 + k] for k in range(1, 7)])
+    assert shared == {0: 64, 1: 128, 2: 192, 3: 256, 4: 320, 5: 320}
+    assert sum(len(t) for st in prefix for t in st) == 320
+
+
+def test_prompts_of_random_trees():
+    import random
+    r = random.Random(9)
+    for _ in range(60):
+        stems = [[r.randint(0, 3) for _ in range(r.randint(0, 3) * 64 + r.randint(0, 40))] for _ in range(3)]
+        prompts = []
+        for _ in range(r.randint(1, 9)):
+            p = []
+            for _ in range(r.randint(1, 3)):
+                p = p + r.choice(stems)
+            prompts.append(p + [r.randint(0, 3) for _ in range(r.randint(1, 5))])
+        shared, prefix = _tree(prompts, r.choice([None, 30, 64, 1000]))
+        # every page that two prompts have in common, a token of each left, is computed once
+        pages = {}
+        for p in prompts:
+            for k in range(64, len(p), 64):
+                pages.setdefault(tuple(p[:k]), []).append(1)
+        assert sum(len(t) for st in prefix for t in st) == 64 * sum(1 for c in pages.values() if len(c) > 1)
+        for i, p in enumerate(prompts):
+            assert shared[i] == max([k for k in range(64, len(p), 64) if len(pages[tuple(p[:k])]) > 1], default=0)
+
+
+def test_a_deep_group_that_cannot_be_held_gives_its_slots_back():
+    a, b = list(range(100, 300)), list(range(1000, 1300))
+    prompts = [a + [1], a + [2], a[:64] + b + [3], a[:64] + b + [4]]
+    for n in (1, 2, 3):
+        be = Tree([[5]] * 4, n_slots=n, max_seq_len=1000)
+        with pytest.raises(IndexError):
+            run_generation(be, prompts, GenParams.greedy(1), share_prefix=True)
+        assert sorted(be.free_slots) == list(range(n))

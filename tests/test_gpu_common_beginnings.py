@@ -35,3 +35,19 @@ def test_recurrent_layers_in_the_common_tokens_own_slot(tmp_path):
     cut = [eng.generate([q], p, max_step_tokens=64)[0] for q in prompts]
     assert shared in (alone, cut)
     eng.cache.check()
+
+
+def test_groups_within_a_group(model_dirs):
+    """Prompts that are a tree of pages: some have more in common than all of them have."""
+    from oracle_engine_b200 import GenParams
+    from oracle_engine_b200.engine.engine import Engine
+    eng = Engine.from_pretrained(model_dirs["E"], dtype="float32", max_tokens=4096, n_slots=8)
+    text, docs = helpers.random_tokens(70, 389, 1), [helpers.random_tokens(n, 389, n) for n in (130, 200)]
+    prompts = [text[:64] + docs[i % 2] + helpers.random_tokens(3 + i, 389, 20 + i) for i in range(6)]
+    prompts += [text + [3], helpers.random_tokens(100, 389, 40)]
+    p = GenParams.greedy(5, ignore_eos=True)
+    want = eng.generate(prompts, p)
+    for portion in (None, 100):
+        assert eng.generate(prompts, p, share_prefix=True, max_step_tokens=portion) == want
+        eng.cache.check()
+    assert eng.cache.slots.n_free == 8

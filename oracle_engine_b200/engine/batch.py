@@ -115,7 +115,7 @@ class SharedPrefixes:
     attention_shared): host numbers, and the integers on the host (`arrays`) or as tensors."""
     n_groups: int                   # a bound: groups beyond the real ones have no members
     n_members: int                  # a bound
-    max_pages: int                  # a bound
+    max_pages: int                  # a bound, as far as the attention's form depends on it (ops_kv8.MAX_SPLITS)
     arrays: tuple = ()              # numpy int32: members, first, pages, seq_pages
     members: torch.Tensor | None = None
     first: torch.Tensor | None = None
@@ -152,7 +152,8 @@ def shared_prefixes(marks: list, pad_seqs: int, eight: bool = False) -> SharedPr
         at += len(bs)
         first[g + 1] = at
     first[len(groups) + 1:] = at
-    return SharedPrefixes(n_groups, min(up(at), pad_seqs), up(int(pages.max())), (members, first, pages, seq_pages))
+    max_pages = min(up(int(pages.max())), up(ops_kv8.MAX_SPLITS))
+    return SharedPrefixes(n_groups, min(up(at), pad_seqs), max_pages, (members, first, pages, seq_pages))
 
 
 @dataclass

@@ -36,6 +36,9 @@ GRAPH_STEP_TOKENS = 256
 EARLY_LAUNCH_MAX_TOKENS = 512
 EARLY_LAUNCH_MAX_TOKENS_MIXTURE = GRAPH_STEP_TOKENS
 MAX_TOKEN_GRAPHS = 64
+# Decode steps whose sequences begin with the same pages are captured per shape of their groups too (SharedPrefixes.shape); groups come and
+# go, so only the shapes used last are kept.
+MAX_PREFIX_GRAPHS = 16
 MAX_GRAPH_WANTED_ROWS = 64
 _TOKEN_BUCKETS = (16, 32, 64, 128, 256)
 
@@ -94,7 +97,8 @@ class Stepper:
         self._state_views = [state.views(e) for e in range(self.n_entries)]
         self._stages = model.stages()
         self.use_graphs = bool(use_graphs and any(safe for safe, _, _ in self._stages))
-        self._graphs: dict[tuple, _DecodeGraph] = {}      # (padded batch size, long context) -> graph
+        self._graphs: dict[tuple, _DecodeGraph] = {}      # (padded batch size, context class) -> graph
+        self._prefix_graphs: dict[tuple, _DecodeGraph] = {}      # the same and the groups' shape -> graph, the one used last at the end
         # (padded tokens, batch size, wanted rows; context class, what the parts choose by the lengths) -> graph
         self._token_graphs: dict[tuple, _DecodeGraph] = {}
         self._eager_buffers: dict[tuple, StepBuffers] = {}
@@ -289,17 +293,25 @@ class Stepper:
         all_logits = self._run_graph(g, ctx)
         return all_logits[:n_want] if n_want else None
 
+    def _decode_graph(self, bucket: int, of_class: int, prefix) -> _DecodeGraph:
+        """One graph per padded batch size and context class: kernels chosen by the class stay right; and per shape of the
+        sequences' common pages, where there are any (MAX_PREFIX_GRAPHS of those at most)."""
+        graphs, key = (self._graphs, (bucket, of_class)) if prefix is None else (self._prefix_graphs, (bucket, of_class) + prefix.shape)
+        g = graphs.get(key) if prefix is None else graphs.pop(key, None)
+        if g is None:
+            if prefix is not None and len(graphs) >= MAX_PREFIX_GRAPHS:
+                if self.rt.device.type == "cuda":
+                    torch.cuda.synchronize(self.rt.device)          # the step before may still be under way
+                del graphs[next(iter(graphs))]
+            g = _DecodeGraph(bucket, StepBuffers(bucket, bucket, bucket, self._table_shapes(bucket), self.rt.device, prefix))
+        graphs[key] = g
+        return g
+
     def _step_graph(self, seqs, starts, tables_changed=True, device_tokens=None):
         B = len(seqs)
         bucket = _bucket(B)
-        # one graph per padded batch size and context class: kernels chosen by the class stay right; and per shape of the
-        # sequences' common pages, where there are any
         prefix = self._prefixes(seqs, bucket)
-        gkey = (bucket, context_class(max(starts) + 1)) + (() if prefix is None else prefix.shape)
-        g = self._graphs.get(gkey)
-        if g is None:
-            g = _DecodeGraph(bucket, StepBuffers(bucket, bucket, bucket, self._table_shapes(bucket), self.rt.device, prefix))
-            self._graphs[gkey] = g
+        g = self._decode_graph(bucket, context_class(max(starts) + 1), prefix)
         key = tuple(s.slot for s in seqs)
         if key == g.key and g.version == self.cache.version:
             # the same sequences one token further: only tokens and positions change

@@ -167,3 +167,31 @@ def test_a_deep_group_that_cannot_be_held_gives_its_slots_back():
         with pytest.raises(IndexError):
             run_generation(be, prompts, GenParams.greedy(1), share_prefix=True)
         assert sorted(be.free_slots) == list(range(n))
+
+
+def test_captured_steps_of_groups_that_come_and_go_are_bounded():
+    """Only the shapes used last keep a graph; steps without groups, and shapes in use, keep theirs."""
+    from types import SimpleNamespace
+
+    import torch
+
+    from oracle_engine_b200.engine import step
+    from oracle_engine_b200.engine.batch import shared_prefixes
+    st = object.__new__(step.Stepper)
+    st._graphs, st._prefix_graphs = {}, {}
+    st.cache, st.rt = SimpleNamespace(groups=[0], max_pages_per_seq=4), SimpleNamespace(device=torch.device("cpu"))
+    plain = st._decode_graph(64, 0, None)
+    often = shared_prefixes([(1, 300)] * 16, 64)
+    kept = st._decode_graph(64, 0, often)
+    made = set()
+    for bucket in (64, 96, 128):
+        for n in (16, 32, 60):
+            for pages in (64, 128, 1000):
+                p = shared_prefixes([(1, pages)] * n, bucket)
+                made.add((bucket, 3) + p.shape)
+                st._decode_graph(bucket, 3, p)
+                assert len(st._prefix_graphs) <= step.MAX_PREFIX_GRAPHS
+                assert st._decode_graph(64, 0, often) is kept
+    assert len(made) > step.MAX_PREFIX_GRAPHS and st._decode_graph(64, 0, None) is plain
+    last = st._decode_graph(128, 3, shared_prefixes([(1, 1000)] * 60, 128))
+    assert st._decode_graph(128, 3, shared_prefixes([(7, 400)] * 60, 128)) is last       # (no form distinguishes the two)

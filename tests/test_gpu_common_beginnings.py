@@ -51,3 +51,36 @@ def test_groups_within_a_group(model_dirs):
         assert eng.generate(prompts, p, share_prefix=True, max_step_tokens=portion) == want
         eng.cache.check()
     assert eng.cache.slots.n_free == 8
+
+
+def test_captured_steps_of_many_shapes(model_dirs, monkeypatch):
+    """More shapes of groups than graphs are kept for, each used until it is captured and replayed, and the first once more."""
+    import numpy as np
+
+    from oracle_engine_b200 import SequenceStep
+    from oracle_engine_b200.csrc import ops_kv8
+    from oracle_engine_b200.engine import step
+    from oracle_engine_b200.engine.engine import Engine
+    monkeypatch.setattr(ops_kv8, "sharing_pays", lambda *a: True)
+    monkeypatch.setattr(step, "MAX_PREFIX_GRAPHS", 3)
+    eng = Engine.from_pretrained(model_dirs["E"], dtype="bfloat16", max_tokens=8192)
+    alone = Engine.from_pretrained(model_dirs["E"], dtype="bfloat16", max_tokens=8192)
+    for n, pages in ((2, 1), (3, 1), (5, 2), (9, 1), (2, 5), (3, 1), (2, 1)):
+        common = helpers.random_tokens(64 * pages, 389, 7 + pages)
+        slots = []
+        for e in (eng, alone):
+            base = e.alloc()
+            e.step([SequenceStep(base, common, [])])
+            slots.append([e.fork(base) for _ in range(n)])
+            e.free(base)
+        alone.cache.prefix = [None] * alone.cache.n_slots
+        for k in range(4):
+            toks = helpers.random_tokens(n, 389, 100 * n + k)
+            got, want = (e.step([SequenceStep(s, [t], [0]) for s, t in zip(sl, toks)]).float().cpu().numpy().copy()
+                         for e, sl in zip((eng, alone), slots))
+            assert np.abs(got - want).max() < helpers.TOL["bfloat16"]
+        assert len(eng.stepper._prefix_graphs) <= 3 and not alone.stepper._prefix_graphs
+        for e, sl in zip((eng, alone), slots):
+            for s in sl:
+                e.free(s)
+    eng.check_device_errors()

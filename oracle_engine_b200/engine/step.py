@@ -102,6 +102,7 @@ class Stepper:
         # (padded tokens, batch size, wanted rows; context class, what the parts choose by the lengths) -> graph
         self._token_graphs: dict[tuple, _DecodeGraph] = {}
         self._eager_buffers: dict[tuple, StepBuffers] = {}
+        self._reads_common = model.reads_common_pages()
         self._last_prefixes = None         # the last step's common beginnings: what they were made from, and they
         self.launch_counter = None         # set by the bench to count kernel launches
 
@@ -178,7 +179,9 @@ class Stepper:
         return logits
 
     def _prefixes(self, seqs, pad_seqs: int):
-        """Which sequences of a step of single tokens begin with the same pages, or None."""
+        """Which sequences of a step of single tokens begin with the same pages, or None (also where no mixer reads them apart)."""
+        if not self._reads_common:
+            return None
         marks = [self.cache.prefix[s.slot] for s in seqs]
         if not any(marks):
             return None

@@ -17,6 +17,7 @@ import math
 import torch
 
 from ..csrc import ops, ops_kv8
+from . import attention_dispatch as ad
 from .linear import chain_flags, matmul_nt
 from .registry import MIXERS, Part
 from .spec import TensorDecl, attention_cache_need, mask_span, visible_keys, visible_pairs
@@ -94,6 +95,10 @@ class GQAAttention(Part):
     takes_scaled = True            # its input goes to one product (Runtime.leave_normed)
     quantised_cache = True
 
+    @property
+    def reads_common_pages(self):
+        return ad.takes_common_pages(self.rt, self.H, self.KVH, self.hd, self.span)
+
     def forward(self, h, residual, ctx, cache, state, owns_cache=True, projected=None):
         """projected: Wqkv h (Wq h first), computed by the caller; the rotation works in it."""
         if self.reads_cache and owns_cache:
@@ -108,7 +113,6 @@ class GQAAttention(Part):
             # how the products are chained to their neighbours in the stream: parts/linear.py
             matmul_nt(self.rt, qkv, h, self.w_qkv[:width], early=chain_flags("mixer_in", T))
         cos, sin = self.position.tables() if self.position is not None else (None, None)
-        from . import attention_dispatch as ad
         o = self.rt.empty(T, q_width)
         ad.mixer_core(self.rt, o, qkv, cos, sin, cache, ctx, self.H, self.KVH, self.hd, self.span, self.scale,
                       owns_cache)

@@ -97,6 +97,10 @@ class DecoderModel:
                 out[e.cache_from] = out[e.cache_from].joined(mine)
         return out
 
+    def reads_common_pages(self) -> bool:
+        """Whether a step of sequences that begin with the same pages is another step for some mixer."""
+        return any(self.layers[e.layer].mixer.reads_common_pages for e in self.schedule)
+
     def state_needs(self):
         """Per schedule entry: dict name -> StateNeed of its mixer."""
         return [dict(self.layers[e.layer].mixer.state_need()) for e in self.schedule]

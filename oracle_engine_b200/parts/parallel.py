@@ -102,6 +102,10 @@ class ParallelMixers(Part):
     def quantised_cache(self):
         return all(m.quantised_cache for _, m, _ in self.branches if m.cache_need() is not None)
 
+    @property
+    def reads_common_pages(self):
+        return any(m.reads_common_pages for _, m, _ in self.branches)
+
     def cache_need(self):
         for _, m, _ in self.branches:
             if m.cache_need() is not None:

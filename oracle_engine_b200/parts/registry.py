@@ -38,7 +38,7 @@ Mixer  (MIXERS; e.g. attention)
     step_choice(step) (Part.step_choice); one that is a mixture of experts has `mixture = True`
 
     optional: a mixer whose forward also takes an 8-bit cache (cache.kv is then a pair, CacheView.kv) has `quantised_cache = True`
-    and declares that form where runtime.cache_codes asks for it
+    and declares that form where runtime.cache_codes asks for it; one that looks at ctx.prefix has `reads_common_pages = True`
 
     optional: a mixer made of mixers with output norms may hand those outputs over unnormed, with the norms' weights
     (`normed_outputs`, `eps`); an arrangement that norms the sum then does all of it in one kernel
@@ -123,6 +123,8 @@ class Part:
 
     mixture = False                # a mixture of experts
     quantised_cache = False        # a mixer that can keep its cache in 8 bits (Runtime.cache_codes)
+    # a mixer whose steps of single tokens read pages that several sequences begin with once for all of them (StepContext.prefix)
+    reads_common_pages = False
 
     def __init__(self, params: dict, prefix: str, runtime):
         self.params = dict(params)

@@ -195,3 +195,22 @@ def test_captured_steps_of_groups_that_come_and_go_are_bounded():
     assert len(made) > step.MAX_PREFIX_GRAPHS and st._decode_graph(64, 0, None) is plain
     last = st._decode_graph(128, 3, shared_prefixes([(1, 1000)] * 60, 128))
     assert st._decode_graph(128, 3, shared_prefixes([(7, 400)] * 60, 128)) is last       # (no form distinguishes the two)
+
+
+def test_which_models_read_common_pages_apart():
+    import conftest
+    import fuvipel_models as fm
+    import torch
+
+    from oracle_engine_b200.config.base import get_architecture
+    from oracle_engine_b200.engine.runtime import Runtime
+    from oracle_engine_b200.parts.model import DecoderModel
+
+    def reads(raw, dtype=torch.bfloat16, tensor_cores=True):
+        arch = get_architecture(raw.get("architecture") or raw["architectures"][0])
+        rt = Runtime(dtype, torch.device("cpu"), tensor_cores)
+        return DecoderModel(arch.build_spec(arch.config_cls.from_dict(raw), 256), rt).reads_common_pages()
+    assert reads(conftest.TINY_E)
+    assert not reads(conftest.TINY_E, torch.float32) and not reads(conftest.TINY_E, tensor_cores=False)
+    assert not reads(conftest.TINY_B)                    # heads of another size
+    assert not reads(fm.F1)

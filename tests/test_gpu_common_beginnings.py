@@ -84,3 +84,21 @@ def test_captured_steps_of_many_shapes(model_dirs, monkeypatch):
             for s in sl:
                 e.free(s)
     eng.check_device_errors()
+
+
+def test_steps_that_read_no_page_apart_are_captured_once(model_dirs, monkeypatch):
+    """A float32 engine's kernels do not look at the groups: their shapes are no part of what is captured."""
+    from oracle_engine_b200 import SequenceStep
+    from oracle_engine_b200.csrc import ops_kv8
+    from oracle_engine_b200.engine.engine import Engine
+    monkeypatch.setattr(ops_kv8, "sharing_pays", lambda *a: True)
+    eng = Engine.from_pretrained(model_dirs["E"], dtype="float32", max_tokens=4096)
+    for n in (5, 6, 7):
+        base = eng.alloc()
+        eng.step([SequenceStep(base, helpers.random_tokens(128, 389, 1), [])])
+        slots = [eng.fork(base) for _ in range(n)] + [base]
+        for _ in range(2):
+            eng.step([SequenceStep(s, [7], [0]) for s in slots])
+        for s in slots:
+            eng.free(s)
+    assert list(eng.stepper._graphs) == [(8, 0)] and not eng.stepper._prefix_graphs

@@ -20,7 +20,8 @@
 //                           dimensions of each of 4 keys, whose bytes are paired by permutes.  P^T comes from S^T by movmatrix.
 // Masks: key <= the row's position; window > 0 the last `window` keys, window < 0 the keys of the row's chunk.  A masked key's weight is
 // set to zero whatever its score and scale are, so rows behind the last token of a page may hold anything.
-// A page number outside the cache counts as a page without keys.
+// A page number outside the cache counts as a page without keys; a row at a position without an angle comes out undefined, and its token's key and
+// value are not written.
 // Measured (us; B200, 8 KV heads; with the write of the new tokens' rows):  64 sequences of 144 to 4,019 keys, 24 heads of 128, int8, 290 MB:
 // 68, 4.3 TB/s, 65 % of the measured copy; one of 32,000, 32 heads of 128, e4m3: 22 with the kernel that joins 36 parts, 3.0 TB/s; 16 with a
 // window of 1,024, 32 heads of 64: 9.3, 1.9 TB/s; one of 137 keys: 6.4.  Bound where there are many keys by the codes' conversion (logic
@@ -119,6 +120,7 @@ struct Args {
     const int* seq_start;      // [B] cache length before the step
     const int* seq_qlen;       // [B]
     int H, KVH, window;
+    int n_positions;           // that the angles are there for
     float scale_log2;
     int cluster;               // CTAs that share a tile of rows
     int ahead;                 // rows of earlier tokens may be read before the wait
@@ -371,7 +373,7 @@ attn_kv8_kernel(const Args a) {
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) qw[nt][ks] = r < rows ? __ldcg((const uint2*)(src + ks * 16)) : make_uint2(0u, 0u);
             if (a.cos_tab != nullptr) {
-                const size_t at = (size_t)(start + rr / G) * (HD / 2) + tig * 4;
+                const size_t at = (size_t)min((unsigned)(start + rr / G), (unsigned)a.n_positions - 1u) * (HD / 2) + tig * 4;
 #pragma unroll
                 for (int ks = 0; ks < KS / 2; ks++) {
                     qc[nt][ks] = *(const float4*)(a.cos_tab + at + ks * 16);
@@ -432,6 +434,8 @@ attn_kv8_kernel(const Args a) {
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
             down = kv8_row_factor(most, &up[nt]);
         }
+        const int at = start + (row0 + (nt * 8 + gid < rows ? nt * 8 + gid : 0)) / G;
+        if ((unsigned)at >= (unsigned)a.n_positions) up[nt] = __uint_as_float(0x7fc00000u);
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
 #pragma unroll
@@ -463,7 +467,8 @@ attn_kv8_kernel(const Args a) {
         }
     }
     // the warp that meets the new token's tile makes that token's rows and stores them in the cache
-    const bool owner = own_kv && n_my > 0 && (t_hi - t_lo - gw) % stride == 0;
+    // (without an angle it is not made, and the row's result, the only one that its key is for, is undefined)
+    const bool owner = own_kv && n_my > 0 && (t_hi - t_lo - gw) % stride == 0 && (unsigned)start < (unsigned)a.n_positions;
     NewToken<KIND> fresh;
     if (owner) {
         fresh.make(a, a.q + packed0 * a.q_stride, start, kvh, lane);
@@ -849,6 +854,7 @@ int oe_attn_kv8(const Kv8Call* call) {
     if (c.n_seqs <= 0 || c.max_qlen <= 0) return 0;
     if (c.KVH <= 0 || c.H % c.KVH || c.stride % 8 || ((uintptr_t)c.qkv & 15) || ((uintptr_t)c.cache & 15) || ((uintptr_t)c.scales & 15) ||
         ((uintptr_t)c.cos_tab & 15) || ((uintptr_t)c.sin_tab & 15) || ((uintptr_t)c.out & 15)) return OE_ERR_UNSUPPORTED;
+    if (c.n_positions < 1) return OE_ERR_UNSUPPORTED;
     if (c.cluster < 1 || c.cluster > 8 || (c.cluster & (c.cluster - 1)) || (c.write && c.max_qlen != 1)) return OE_ERR_UNSUPPORTED;
     const bool no_parts = c.part_o == nullptr || c.part_ml == nullptr;
     if (c.seq_pages != nullptr && (c.window != 0 || c.max_qlen != 1 || c.splits < 1 || c.splits + c.cluster > MAX_JOINED || no_parts)) return OE_ERR_UNSUPPORTED;
@@ -858,7 +864,7 @@ int oe_attn_kv8(const Kv8Call* call) {
     a.cache = c.cache; a.scales = c.scales;
     if (c.write) { a.cache_w = c.cache; a.scales_w = c.scales; }
     a.n_pages = c.n_pages; a.tables = c.tables; a.max_pages = c.max_pages; a.cu_q = c.cu_q; a.seq_start = c.seq_start; a.seq_qlen = c.seq_qlen;
-    a.H = c.H; a.KVH = c.KVH; a.window = c.window; a.scale_log2 = c.scale * LOG2E; a.cluster = c.cluster;
+    a.H = c.H; a.KVH = c.KVH; a.window = c.window; a.n_positions = c.n_positions; a.scale_log2 = c.scale * LOG2E; a.cluster = c.cluster;
     a.seq_pages = c.seq_pages; a.splits = c.splits; a.ahead = c.ahead; a.shares = c.shares;
     a.late = c.seq_pages != nullptr && c.n_groups > 0 && c.n_members > 0;
     if (c.seq_pages != nullptr) { a.part_o = c.part_o; a.part_ml = c.part_ml; }

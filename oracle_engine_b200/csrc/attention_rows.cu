@@ -18,6 +18,8 @@
 // bfloat16: K and V as they are (TMA); queries and weights are sums of two bfloat16, a second product each.
 // Roles (warps): 0 asks for the pages, 1 issues the products, 2 prepares the scales, 4-11 turn codes into float16 (8-bit forms),
 // the last 8 load and turn the queries, then do the softmax and store.
+// A page number outside the cache counts as a page without keys; a row at a position without an angle comes out undefined; a member that is no
+// sequence of the step reads and writes nothing, and what its group gets is undefined then.
 // Few tiles: the pages are cut into `splits` runs, whose parts (O, m, l) are joined by the kernel that runs next.
 // Measured (us; 8 KV heads of 128, int8):  a page takes a CTA 0.98 with one tile and 1.38 with two, besides 10 to 13 to start and end.  No
 // unit is full then (two tiles: issue slots 56 %, exponentials and tensor cores 39 % each); the time is the chain that a page's
@@ -105,11 +107,13 @@ struct Args {
     const int* seq_start;
     const int* seq_qlen;
     int H, KVH, window;
+    int n_positions;           // that the angles are there for
     float scale_log2;
     int ahead;
     const int* members;        // prefixes, as in attention_kv8.cu
     const int* first;
     const int* pages;
+    int n_members, n_seqs;     // that `members` holds, and that its numbers are below
     int splits;
     float* part_o;             // [rows, splits, HD]: row = (sequence or packed token) * H + head
     float* part_ml;            // [rows, splits, 2]
@@ -365,13 +369,18 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.H / a.KVH, tpt = BM / G;               // tokens, or members, of a tile
     const int kvh = blockIdx.x % a.KVH, split = blockIdx.x / a.KVH;
+    auto member = [&](int i) {                             // the sequence of the group's i-th member, -1: none
+        const int at = a.first[blockIdx.y] + i, sq = (unsigned)at < (unsigned)a.n_members ? a.members[at] : -1;
+        return (unsigned)sq < (unsigned)a.n_seqs ? sq : -1;
+    };
     // the tiles' rows and the CTA's pages (the step's integers were written before its first kernel)
     int b, count, t0, start = 0, key_lo = 0, j_lo, n_blocks[MT];
     if (PREFIX) {
         const int g = blockIdx.y;
         count = a.first[g + 1] - a.first[g];
         t0 = blockIdx.z * MT * tpt;
-        b = t0 < count ? a.members[a.first[g]] : 0;
+        b = t0 < count ? member(0) : 0;
+        if (b < 0) count = 0;
     } else {
         b = blockIdx.y;
         count = a.seq_qlen[b];
@@ -456,14 +465,17 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
             pos_of[k] = 0;
             if (g < GROUPS && r < tpt * G && tok < count) {
                 long long at;
+                int pos;
                 if (PREFIX) {
-                    const int sq = a.members[a.first[blockIdx.y] + tok];
+                    const int sq = member(tok);
+                    if (sq < 0) continue;
                     at = a.cu_q[sq];
-                    pos_of[k] = a.seq_start[sq];
+                    pos = a.seq_start[sq];
                 } else {
                     at = a.cu_q[b] + tok;
-                    pos_of[k] = start + tok;
+                    pos = start + tok;
                 }
+                pos_of[k] = (unsigned)pos < (unsigned)a.n_positions ? pos : -1;
                 src[k] = a.q + at * a.q_stride + (long long)(kvh * G + r % G) * HD + d;
             }
         }
@@ -488,8 +500,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                 for (int k = 0; k < ROUND; k++) {
 #pragma unroll
                     for (int j = 0; j < 8; j += 4) {
-                        *(float4*)&cs[k][j] = *(const float4*)(a.cos_tab + (long long)pos[k] * (HD / 2) + d + j);
-                        *(float4*)&sn[k][j] = *(const float4*)(a.sin_tab + (long long)pos[k] * (HD / 2) + d + j);
+                        *(float4*)&cs[k][j] = *(const float4*)(a.cos_tab + (long long)max(pos[k], 0) * (HD / 2) + d + j);
+                        *(float4*)&sn[k][j] = *(const float4*)(a.sin_tab + (long long)max(pos[k], 0) * (HD / 2) + d + j);
                     }
                 }
             }
@@ -521,7 +533,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
                     for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                     down = kv8_row_factor(most, &up);
                 }
-                if (d == 0) ctl->up[rr] = up;
+                if (d == 0) ctl->up[rr] = pos[k] < 0 ? __uint_as_float(0x7fc00000u) : up;      // (no angle: an undefined row)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     const int dim = d + half * (HD / 2);
@@ -718,16 +730,19 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a) {
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
         const uint32_t s_addr = lane_addr + (uint32_t)(tile * 2 * BN), o_addr = lane_addr + Z::S_COLS + (uint32_t)(tile * HD + half * (HD / SPLIT));
         const int tok = t0 + tile * tpt + r / G, head = kvh * G + r % G;
-        const bool valid = r < tpt * G && tok < count;
+        bool valid = r < tpt * G && tok < count;
         int pos = 0, low = 0;
         long long row = 0;                                 // the packed row of q and out
         long long part = 0;
         if (valid) {
             if (PREFIX) {
-                const int sq = a.members[a.first[blockIdx.y] + tok];
-                row = a.cu_q[sq];
-                pos = a.seq_start[sq];
-                part = (long long)sq * a.H + head;
+                const int sq = member(tok);
+                valid = sq >= 0;
+                if (valid) {
+                    row = a.cu_q[sq];
+                    pos = a.seq_start[sq];
+                    part = (long long)sq * a.H + head;
+                }
             } else {
                 row = a.cu_q[b] + tok;
                 pos = start + tok;
@@ -999,13 +1014,14 @@ Args arguments(const Kv8Call& c) {
     Args a = {};
     a.out = c.out; a.q = c.qkv; a.q_stride = c.stride; a.cos_tab = c.cos_tab; a.sin_tab = c.sin_tab; a.codes = (const uint8_t*)c.cache;
     a.scales = c.scales; a.n_pages = c.n_pages; a.tables = c.tables; a.max_pages = c.max_pages; a.cu_q = c.cu_q; a.seq_start = c.seq_start;
-    a.seq_qlen = c.seq_qlen; a.H = c.H; a.KVH = c.KVH; a.window = c.window; a.scale_log2 = c.scale * LOG2E; a.ahead = c.ahead;
+    a.seq_qlen = c.seq_qlen; a.H = c.H; a.KVH = c.KVH; a.window = c.window; a.n_positions = c.n_positions; a.n_members = c.n_members; a.n_seqs = c.n_seqs;
+    a.scale_log2 = c.scale * LOG2E; a.ahead = c.ahead;
     a.members = c.members; a.first = c.first; a.pages = c.pages; a.splits = c.splits; a.part_o = c.part_o; a.part_ml = c.part_ml;
     return a;
 }
 bool operands_ok(const Args& a, const void* cache) {
     return a.KVH > 0 && a.H % a.KVH == 0 && a.H / a.KVH <= BM && a.q_stride % 8 == 0 && !((uintptr_t)a.q & 15) && !((uintptr_t)cache & 15) &&
-           !((uintptr_t)a.scales & 15) && !((uintptr_t)a.cos_tab & 15) && !((uintptr_t)a.sin_tab & 15) && a.splits >= 1 && a.n_pages >= 1;
+           !((uintptr_t)a.scales & 15) && !((uintptr_t)a.cos_tab & 15) && !((uintptr_t)a.sin_tab & 15) && a.splits >= 1 && a.n_pages >= 1 && a.n_positions >= 1;
 }
 
 }  // namespace

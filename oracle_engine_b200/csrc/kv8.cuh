@@ -46,7 +46,7 @@ struct Kv8Call {
     cudaStream_t stream;
     int bytes;                     // of this struct
     int kind, write, max_pages, n_seqs, n_tokens, max_qlen, H, KVH, window, warps, cluster, ordered, shares, mt, splits, n_groups, n_members, ahead;
-    int n_positions, n_tables;     // that the angles and the page tables are there for (the write's bounds)
+    int n_positions, n_tables;     // that the angles and (for the write) the page tables are there for
     float scale;
 };
 static_assert(sizeof(Kv8Call) == 21 * 8 + 22 * 4, "as the host packs it");

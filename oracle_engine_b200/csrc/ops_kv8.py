@@ -75,7 +75,7 @@ def _packed(out, qkv, cos, sin, rows, scales, tables, ctx, part, part_rows: int,
         ctx.seq_qlen.data_ptr(), 0, 0, *lists,
         part_o, part_o + 4 * part_rows * parts * head_dim if part_o else 0, _stream(dev),
         _CALL.size, kind, write, max_pages, ctx.n_seqs, T, max_qlen, n_heads, n_kv_heads, window, warps, cluster, ordered, shares, mt, splits,
-        n_groups, n_members, ahead, 0, 0, scale)
+        n_groups, n_members, ahead, 2 ** 31 - 1 if cos is None else cos.shape[0], tables.shape[0], scale)
 
 
 def _stream(dev: int) -> int:
@@ -161,7 +161,7 @@ def _check_step(what: str, out, qkv, cos, tables, ctx, n_heads: int, head_dim: i
     table = tables.shape
     if len(table) != 2 or table[0] < n or cu_q.numel() <= n or start.numel() < n or qlen.numel() < n:
         raise KernelError(f"{what}: the step's tables are shorter than its {n} sequences")
-    if longest > table[1] * PAGE or cos is not None and longest > cos.shape[0]:
+    if longest > table[1] * PAGE or cos is not None and max(longest, 1) > cos.shape[0]:
         raise KernelError(f"{what}: a sequence of {longest} tokens is longer than its page table or the position tables")
 
 
@@ -233,7 +233,8 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
 
     qkv bfloat16 [T, (H + 2 KVH) hd] (or [T, H hd] when has_kv is false: the rows are in the cache) before rotation, left as it
     is; out bfloat16 [T, H hd]; ctx: the step (StepContext: cu_q, seq_start, seq_qlen, tok_seq, tok_pos, n_seqs, max_qlen,
-    all_decode).  A step of one token a sequence is one launch, any other a write and an attention.  form: the kernel's
+    all_decode; max_kvlen, where it is there, is checked against the tables).  A token at a position without an angle comes out
+    undefined and is not written; pages that are not in the cache, or behind the page table, have no keys.  A step of one token a sequence is one launch, any other a write and an attention.  form: the kernel's
     form (decode_form where a sequence has few rows, prompt_form else); None: by those rules."""
     what = "attention_kv8"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
@@ -340,6 +341,7 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     groups without members), max_pages (the most pages a group has in common), and int32 tensors members (sequences in the order of
     their groups), first [n_groups + 1] (where each group's members begin), pages [n_groups] (full pages that the group's
     tables begin with, whose tokens are all earlier than the step's), seq_pages [n_seqs] (those of the sequence's group, 0 for a sequence in none).
+    A group with a member that is no sequence of the step has undefined results.
     form: the kernels' form; None: by shared_form."""
     what = "attention_shared"
     _check_heads(what, n_heads, n_kv_heads, head_dim)

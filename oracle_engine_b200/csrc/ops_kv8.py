@@ -121,6 +121,12 @@ def _check_heads(what: str, n_heads: int, n_kv_heads: int, head_dim: int) -> Non
                           f"(head sizes {HEAD_DIMS}, heads a multiple of the KV heads)")
 
 
+def _check_scale(what: str, scale: float) -> None:
+    """The kernels take a row's largest score times the scale for its largest weight's exponent."""
+    if not 0.0 < scale < float("inf"):
+        raise KernelError(f"{what}: the scores' scale must be a positive number, not {scale}")
+
+
 def _check_rows(what: str, qkv, cos, sin, width: int, head_dim: int) -> None:
     shape, stride = qkv.shape, qkv.stride()
     if qkv.dtype is not _BF16 or len(shape) != 2 or shape[1] != width or stride[1] != 1 or stride[0] % 8 or qkv.data_ptr() % 16:
@@ -238,6 +244,7 @@ def attention_kv8(out, qkv, cos, sin, cache, tables, ctx, n_heads: int, n_kv_hea
     form (decode_form where a sequence has few rows, prompt_form else); None: by those rules."""
     what = "attention_kv8"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
+    _check_scale(what, scale)
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)
     dev = _here(what, out, qkv, cos, sin, codes, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen)
     _check_rows(what, qkv, cos, sin, (n_heads + (2 * n_kv_heads if has_kv else 0)) * head_dim, head_dim)
@@ -345,6 +352,7 @@ def attention_shared(out, qkv, cos, sin, cache, tables, ctx, prefix, n_heads: in
     form: the kernels' form; None: by shared_form."""
     what = "attention_shared"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
+    _check_scale(what, scale)
     kind, rows, scales = _cache_args(what, cache, n_kv_heads, head_dim, True)
     lists = (prefix.members, prefix.first, prefix.pages, prefix.seq_pages)
     dev = _here(what, out, qkv, cos, sin, rows, scales, tables, ctx.cu_q, ctx.seq_start, ctx.seq_qlen, *lists)

@@ -97,7 +97,7 @@ class GQAAttention(Part):
 
     @property
     def reads_common_pages(self):
-        return ad.takes_common_pages(self.rt, self.H, self.KVH, self.hd, self.span)
+        return ad.takes_common_pages(self.rt, self.H, self.KVH, self.hd, self.span, self.scale)
 
     def forward(self, h, residual, ctx, cache, state, owns_cache=True, projected=None):
         """projected: Wqkv h (Wq h first), computed by the caller; the rotation works in it."""

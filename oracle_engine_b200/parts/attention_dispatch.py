@@ -14,15 +14,15 @@ import torch
 from ..csrc import ops, ops_kv8
 
 
-def takes_common_pages(rt, H, KVH, hd, window) -> bool:
+def takes_common_pages(rt, H, KVH, hd, window, scale) -> bool:
     """Whether single tokens of sequences that begin with the same pages go to the kernels that read those once."""
-    return not window and rt.dtype == torch.bfloat16 and rt.tensor_cores and ops_kv8.supported(hd, H, KVH)
+    return not window and scale > 0 and rt.dtype == torch.bfloat16 and rt.tensor_cores and ops_kv8.supported(hd, H, KVH)
 
 
 def mixer_core(rt, out, qkv, cos, sin, cache, ctx, H, KVH, hd, window, scale, owns_cache) -> None:
     """Rotation, cache write and attention of one attention mixer for the step's tokens.  (`ahead`: in a model's step the
     projections lie between whatever wrote the cache and its attention.)"""
-    if getattr(ctx, "prefix", None) is not None and takes_common_pages(rt, H, KVH, hd, window):
+    if getattr(ctx, "prefix", None) is not None and takes_common_pages(rt, H, KVH, hd, window, scale):
         ops_kv8.attention_shared(out, qkv, cos, sin, cache.kv, cache.tables, ctx, ctx.prefix, H, KVH, hd, scale, owns_cache, ahead=True)
         return
     if rt.cache_codes is not None:

@@ -214,3 +214,9 @@ def test_which_models_read_common_pages_apart():
     assert not reads(conftest.TINY_E, torch.float32) and not reads(conftest.TINY_E, tensor_cores=False)
     assert not reads(conftest.TINY_B)                    # heads of another size
     assert not reads(fm.F1)
+    odd = dict(conftest.TINY_E)
+    arch = get_architecture(odd["architectures"][0])
+    model = DecoderModel(arch.build_spec(arch.config_cls.from_dict(odd), 256), Runtime(torch.bfloat16, torch.device("cpu"), True))
+    for e in model.schedule:
+        model.layers[e.layer].mixer.scale = -0.125       # the kernels of common beginnings take positive scales
+    assert not model.reads_common_pages()

@@ -7,8 +7,10 @@ head) reads as code * scale: with a the row's largest magnitude and c = 127 or 4
 even) and scale = a / c.  Keys are turned by their position and rounded to bfloat16 before that.  A row with an infinite or
 undefined value reads as undefined.
 
-`ahead`: the caller knows that another kernel lies between whatever wrote the cache's earlier rows and this call, as in a model's
-step, where the projections do; the kernel then asks for those rows while the kernel before it still runs.
+`ahead`: the caller knows that whatever wrote the cache's earlier rows has ended when the kernel before this call starts; the call's kernel
+then asks for those rows while the kernel before it still runs.  A copy between the two is enough, or a kernel that is launched without
+programmatic serialization, as torch's are; one of this package's is not, since most of them let their successor start before they
+have waited for their predecessor.  A model's steps have such a copy: that of their integers.
 """
 from __future__ import annotations
 

@@ -20,8 +20,8 @@ def takes_common_pages(rt, H, KVH, hd, window, scale) -> bool:
 
 
 def mixer_core(rt, out, qkv, cos, sin, cache, ctx, H, KVH, hd, window, scale, owns_cache) -> None:
-    """Rotation, cache write and attention of one attention mixer for the step's tokens.  (`ahead`: in a model's step the
-    projections lie between whatever wrote the cache and its attention.)"""
+    """Rotation, cache write and attention of one attention mixer for the step's tokens.  (`ahead`: the rows of earlier
+    tokens are those of earlier steps, which ended before the copy of this step's integers, and other kernels lie before the attention.)"""
     if getattr(ctx, "prefix", None) is not None and takes_common_pages(rt, H, KVH, hd, window, scale):
         ops_kv8.attention_shared(out, qkv, cos, sin, cache.kv, cache.tables, ctx, ctx.prefix, H, KVH, hd, scale, owns_cache, ahead=True)
         return

@@ -124,9 +124,10 @@ def _check_heads(what: str, n_heads: int, n_kv_heads: int, head_dim: int) -> Non
 
 
 def _check_scale(what: str, scale: float) -> None:
-    """The kernels take a row's largest score times the scale for its largest weight's exponent."""
-    if not 0.0 < scale < float("inf"):
-        raise KernelError(f"{what}: the scores' scale must be a positive number, not {scale}")
+    """The kernels take a row's largest score times the scale for its largest weight's exponent; with the factor of a row of queries of
+    zeros, 2^-126, the scale has to stay a number that is not 0."""
+    if not 1e-6 <= scale < float("inf"):
+        raise KernelError(f"{what}: the scores' scale must be a positive number, 1e-6 at least, not {scale}")
 
 
 def _check_rows(what: str, qkv, cos, sin, width: int, head_dim: int) -> None:
@@ -176,7 +177,7 @@ def _check_step(what: str, out, qkv, cos, tables, ctx, n_heads: int, head_dim: i
 def kv8_write(qkv, cos, sin, cache, tables, tok_seq, tok_pos, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
     """Keys (turned at each token's position; cos/sin float32 [max_pos, hd/2] or None) and values of the step's tokens into the
     8-bit cache.  qkv [T, (H + 2 KVH) hd] is left as it is; tok_seq < 0: a padding row; a sequence without a table, a
-    position without an angle or a page outside the cache: nothing is written."""
+    position without an angle or a page outside the cache: nothing is written.  No two tokens of a call have the same place."""
     what = "kv8_write"
     _check_heads(what, n_heads, n_kv_heads, head_dim)
     kind, codes, scales = _cache_args(what, cache, n_kv_heads, head_dim, False)

@@ -9,7 +9,7 @@ from oracle_engine_b200.csrc.ops import KernelError
 from test_kv8_cpu import entry
 
 
-@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("scale", [0.0, 1e-9, -0.125, float("nan"), float("inf"), -float("inf")])
 def test_scales_that_are_not_positive(scale):
     cache, i = entry(), torch.zeros(2, dtype=torch.int32)
     qkv, out = torch.zeros(1, 8 * 64, dtype=torch.bfloat16), torch.zeros(1, 4 * 64, dtype=torch.bfloat16)

@@ -102,3 +102,45 @@ def test_steps_that_read_no_page_apart_are_captured_once(model_dirs, monkeypatch
         for s in slots:
             eng.free(s)
     assert list(eng.stepper._graphs) == [(8, 0)] and not eng.stepper._prefix_graphs
+
+
+@pytest.mark.parametrize("dtype,kind", [("float32", None), ("bfloat16", None), ("bfloat16", "int8")])
+def test_forks_over_chunks_and_another_entry_s_cache(tmp_path, monkeypatch, dtype, kind):
+    """Layers of chunks give their part of the common pages back one sequence at a time, beside a layer that keeps all of them."""
+    import numpy as np
+
+    import goridra_models as gm
+    from oracle_engine_b200 import SequenceStep
+    from oracle_engine_b200.csrc import ops_kv8
+    from oracle_engine_b200.engine.engine import Engine
+    monkeypatch.setattr(ops_kv8, "sharing_pays", lambda *a: True)
+    raw = gm.config(150, 128, 1e-5, [gm.layer(gm.attention(4, 2, 64, 64, 0.125, 70, (24, 50000.0)), gm.dense(64)),
+                                     gm.layer(gm.attention(4, 2, 64, 64, 0.2, 100, (24, 50000.0), 0), gm.dense(64)),
+                                     gm.layer(gm.attention(2, 1, 64, 64, 0.125), gm.dense(64))])
+    eng = Engine.from_pretrained(gm.write(tmp_path, raw, 3), dtype=dtype, max_tokens=4096, cache_dtype=kind)
+    common = helpers.random_tokens(128, 150, 4)
+    tails = [helpers.random_tokens(90, 150, 5 + i) for i in range(3)]
+
+    def run(shared):
+        if shared:
+            base = eng.alloc()
+            eng.step([SequenceStep(base, common, [])])
+            slots = [eng.fork(base) for _ in tails]
+            eng.free(base)
+        else:
+            slots = [eng.alloc() for _ in tails]
+            for s in slots:
+                eng.step([SequenceStep(s, common, [])])
+        out = []
+        for at, n in ((0, 40), (40, 1), (41, 1), (42, 40)) + tuple((82 + i, 1) for i in range(8)):
+            got = eng.step([SequenceStep(s, t[at:at + n], [n - 1]) for s, t in zip(slots, tails)])
+            out.append(got.float().cpu().numpy().copy())
+            eng.cache.check()
+        for s in slots:
+            eng.free(s)
+        return np.stack(out)
+    alone, forked = run(False), run(True)
+    if dtype == "float32":
+        assert np.array_equal(alone, forked)
+    assert np.sqrt(((alone - forked) ** 2).mean() / (alone ** 2).mean()) < helpers.TOL[dtype]
+    eng.check_device_errors()

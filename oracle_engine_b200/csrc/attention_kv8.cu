@@ -23,10 +23,11 @@
 // A page number outside the cache counts as a page without keys; a row at a position without an angle comes out undefined, and its token's key and
 // value are not written.
 // Measured (us; B200, 8 KV heads; with the write of the new tokens' rows):  64 sequences of 144 to 4,019 keys, 24 heads of 128, int8, 290 MB:
-// 68, 4.3 TB/s, 65 % of the measured copy; one of 32,000, 32 heads of 128, e4m3: 22 with the kernel that joins 36 parts, 3.0 TB/s; 16 with a
-// window of 1,024, 32 heads of 64: 9.3, 1.9 TB/s; one of 137 keys: 6.4.  Bound where there are many keys by the codes' conversion (logic
-// and permutes of 12 warps an SM beside their products) more than by the reads, where there are few by the chain of loads: the
-// sequence's numbers, its pages, queries and rows, then the join.
+// 69, 4.2 TB/s, 65 % of the measured copy; one of 32,000, 32 heads of 128, e4m3: 23 with the kernel that joins 37 parts, 2.9 TB/s; 16 with a
+// window of 1,024, 32 heads of 64: 9.3, 1.9 TB/s; one of 137 keys: 6.4.  Where there are few keys the chain of loads bounds it: the sequence's
+// numbers, its pages, queries and rows, then the join.  Where there are many, no unit is full (64 sequences in int8 / e4m3: issue slots
+// 48 / 46 %, logic pipe 46 / 53 %, DRAM 47 / 55 %): the codes' conversion and the products are chains of dependent instructions, and an SM has
+// eight warps for them.  A third CTA of four warps does not help (see `len`).
 #include "kv8.cuh"
 
 #ifndef OE_HD
@@ -327,6 +328,9 @@ attn_kv8_kernel(const Args a) {
     int b = blockIdx.z;
     if (a.ordered) {
         // more CTAs than there is room for: the long sequences' start first, so that the short ones' fill the end
+        // With heads of 128 the list leaves an SM room for two CTAs of four warps.  Kept where the rings are, which makes room for three (us):
+        // 64 sequences of 144 to 4,019 keys 88 instead of 69, one of 32,000 in 37 parts 27 instead of 23, 32 behind 4,096 common tokens 27.8
+        // instead of 25.4; only many short ones gain, 200 of 100 to 900 keys 43 instead of 52.
         __shared__ int len[MAX_ORDERED], which;
         for (int t = threadIdx.x; t < a.ordered; t += NW * 32)
             len[t] = a.seq_qlen[t] > 0 ? a.seq_start[t] + 1 - (a.seq_pages != nullptr ? a.seq_pages[t] * OE_PAGE : 0) : 0;
@@ -802,6 +806,7 @@ template <int KIND, int NT, int NW, int ST>
 int launch(const Args& a, long long rows, int n_seqs, cudaStream_t st) {
     auto kernel = attn_kv8_kernel<KIND, NT, NW, ST>;
     constexpr size_t smem = (size_t)NW * ST * Tile<KIND>::BYTES;
+    static_assert(NW != 4 || HD != 128 || 3 * (smem + (MAX_ORDERED + 1) * 4 + 1024) > 228 * 1024, "two CTAs of four warps an SM, as measured");
     const long long x = (rows + 8 * NT - 1) / (8 * NT) * a.cluster * a.shares;
     if (x > 0x7fffffffLL || a.KVH > 65535 || n_seqs > 65535) return OE_ERR_UNSUPPORTED;
     static Kv8Devices set;
@@ -814,7 +819,8 @@ int launch(const Args& a, long long rows, int n_seqs, cudaStream_t st) {
     if (a.cluster > 1) return oe_launch_cluster(kernel, (unsigned)a.cluster, grid, dim3(NW * 32), smem, st, a);
     return oe_launch(kernel, grid, dim3(NW * 32), smem, st, a);
 }
-// warps: 12 (a CTA has an SM to itself) or 4 (three an SM); of a 16-bit cache, whose tiles are twice as large, 6 or 3.
+// warps: 12 (a CTA has an SM to itself) or 4 (two an SM with heads of 128, five with 64); of a 16-bit cache, whose tiles are twice as
+// large, 6 or 3 (two, three).
 template <int KIND, int NT>
 int launch_form(int warps, const Args& a, long long rows, int n_seqs, cudaStream_t st) {
     constexpr int MANY = KIND == OE_KV_BF16 ? 6 : 12, FEW = KIND == OE_KV_BF16 ? 3 : 4;

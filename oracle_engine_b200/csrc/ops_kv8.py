@@ -202,7 +202,7 @@ def _write(what: str, dev: int, kind: int, qkv, cos, sin, codes, scales, tables,
 
 
 def many_pairs(n_seqs: int, n_kv_heads: int, sm_count: int | None = None) -> bool:
-    """More (sequence, KV head) pairs than CTAs of four warps that are resident at once: the longest sequences go first."""
+    """More than three (sequence, KV head) pairs for each SM, of which two to five are resident at once: the longest sequences go first."""
     return n_seqs * n_kv_heads > 3 * (sm_count or ops.sm_count())
 
 
@@ -214,7 +214,7 @@ def decode_form(n_seqs: int, n_kv_heads: int, context_class: int, window: int = 
     Longer ones: CTAs of four warps, which leave room on their SMs for the products that overlap them; up to 8 of a cluster, and
     for very long ones as many as fill the SMs twice and leave parts for another kernel.  ms a decode step of the 28-layer model with 24
     heads over 8 KV heads of 128, int8:  1 sequence of 2,000 keys 12x1 1.83, 12x4 1.63, 12x8 1.58, 4x8 1.64; of 8,000 12x8 1.78,
-    12x1x18 2.39, 4x1x18 1.74; of 32,000 12x8 2.46, 12x1x18 2.74, 4x1x18 2.29, 4x1x36 2.05;  4 of 2,000 12x2 1.79, 12x4 2.47, 4x4
+    12x1x18 2.39, 4x1x18 1.74; of 32,000 12x8 2.46, 12x1x18 2.74, 4x1x18 2.30, 4x1x37 2.05;  4 of 2,000 12x2 1.79, 12x4 2.47, 4x4
     1.79, of 8,000 12x2 2.43, 4x4 2.40;  8 of 512 12x1 1.66, 4x1 1.77, of 2,000 12x1 2.10, 12x2 2.46, 4x2 2.03, 4x4 1.90, of 8,000 12x1
     3.40, 12x2 3.15, 4x4 2.52;  16 of 2,000 12x1 2.39, 4x1 2.64, 4x2 2.32;  32 of 1,000 12x1 2.94, 4x1 2.78."""
     sms = sm_count or ops.sm_count()
@@ -316,7 +316,14 @@ def sharing_pays(groups: list, eight: bool) -> bool:
     2.28/1.61, 2.42/1.74, 2.65/1.96; 4 2.22/1.63, 2.30/1.74, 2.44/1.97, 2.64/2.41; 8 2.03/1.77, 2.13/2.00, 2.27/2.46, 2.47/3.29; 16 2.00/2.04,
     2.06/2.27, 2.17/2.71, 2.37/3.56; 32 2.73/2.62, 2.78/3.01, 2.83/3.79.  int8: 2 1.73/1.62, 1.79/1.68, 1.92/1.73, 2.12/1.85; 4 1.77/1.67,
     1.83/1.78, 1.93/2.01, 2.14/2.45; 8 1.86/1.78, 1.91/1.89, 2.02/2.12, 2.22/2.56; 16 2.00/2.08, 2.06/2.32, 2.17/2.76, 2.37/3.61; 32
-    2.69/2.75, 2.72/3.19, 2.77/4.05."""
+    2.69/2.75, 2.72/3.19, 2.77/4.05.
+    The rule does not look at heads.  Other shapes (16 layers, us a layer of a step, shared / apart; S: the rule shares).  16-bit cache, 32
+    heads over 8 of 64, 4 members behind 1,024, 2,048, 8,192 tokens 44/44, 46/48, 55/70; 8 46/49, 48/56, 57/97 S; 64 behind 1,024 83/80 S;
+    32 over 8 of 128, 8 103/103, 105/111, 116/157 S; 64 behind 1,024 165/152 S; 16 over 16 of 128, 4 59/50, 63/58, 88/104; 8 55/60,
+    59/67, 87/115 S; 64 behind 1,024 119/132 S; 32 over 2 of 64, 8 48/48, 51/49, 55/62 S; 64 behind 1,024 76/74 S; 16 over 2 of 128, 8 50/48,
+    53/50, 59/63 S.  int8, 32 over 8 of 64, 4 45/52, 47/57, 57/91 S; 8 46/56, 49/60 S, 59/94 S; 16 over 16 of 128, 4 52/50, 56/54, 81/77 S;
+    8 52/62, 56/62 S, 81/109 S; 32 over 2 of 64, 4 46/45, 48/46, 50/51 S; 16 over 2 of 128, 4 46/45, 48/46, 52/51 S.  Near its border it costs
+    up to 9 % of a layer where it shares, and where it does not it leaves up to a fifth with heads of 64."""
     less, base = (1, 256) if eight else (3, 768)
     return sum((members - less) * (pages * PAGE - base) for members, pages in groups if members > less and pages * PAGE > base) >= 11500
 
@@ -326,8 +333,8 @@ def shared_form(n_seqs: int, n_members: int, n_groups: int, group: int, n_kv_hea
     """(tiles of 128 rows a CTA has, runs that a prefix's pages are cut into; warps of a CTA and CTAs of a cluster for the keys behind
     the prefixes).  One tile, so that there are fewer parts to join, unless the tiles alone outnumber the SMs (us, 64 members of 32
     heads behind 8,192 tokens in 8 bits: two tiles and 18 runs 54.0, one tile and 9 runs 53.1; behind 2,048 44.0 / 39.8).  The two kernels
-    run beside each other: as many runs as give half of the SMs a CTA while the own keys' CTAs fit the other half, else as many as
-    give every SM one (us, 24 heads, runs of half / of all SMs: 8 members behind 2,048 tokens 14.8 / 21.4, in 8 bits 14.2 / 21.3; 16 behind
+    run beside each other: as many runs as give half of the SMs a CTA while there are at most three of the own keys' CTAs for each SM of the
+    other half, else as many as give every SM one (us, 24 heads, runs of half / of all SMs: 8 members behind 2,048 tokens 14.8 / 21.4, in 8 bits 14.2 / 21.3; 16 behind
     4,096 21.7 / 25.6, 18.1 / 23.7; 32 in 8 bits 30.9 / 28.1).  Own keys: CTAs of all an SM has room for while they have an SM each, no clusters
     (8 members, 9 runs, 6 / 3 warps 14.8 / 15.9; 16 24.9 / 21.7)."""
     sms = sm_count or ops.sm_count()

@@ -49,7 +49,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Keys and values of a step's tokens into the 8-bit cache.  HD / 16 lanes have a token's key and value of one KV head: 8 dimensions of
 // the lower half and the 8 that they are turned with, so that a row's lanes read 16 bytes each of both halves and only its maximum
 // crosses lanes.  Both rows are asked for at once and share the look-ups of the token's place.
-// Measured (B200): 10,235 tokens of 24 heads over 8 KV heads of 128 in int8, 46 MB, 16 us: 2.8 TB/s (a lane group a row: 21 us), bound by the
+// Measured (B200): 7,440 tokens of 24 heads over 8 KV heads of 128 in int8, 46 MB, 16 us: 2.8 TB/s (a lane group a row: 21 us), bound by the
 // loads' latency, at 32 warps an SM, and by the instructions of the exact roundings; one token 1.9 us, 64 tokens 3.8: the start of a
 // kernel and two rounds of loads.
 template <int KIND>

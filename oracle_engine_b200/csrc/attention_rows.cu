@@ -29,6 +29,7 @@
 // warp for each tile's products: 1.44 instead of 1.38.  A prompt of 2,048 tokens with 24 heads takes 66 (390 TFLOP/s of causal
 // work), 192 tokens with 32 heads behind 12,005 of e4m3 73 (518 TFLOP/s), joined from 6 runs, both with the cache write; 64 members with 32 heads behind
 // 8,192 common tokens 50 with the kernel of their own keys (177 TFLOP/s).
+// The 16-bit cache's kernel takes that prompt in 46 with its rotation and write: it turns no codes, so that two of its CTAs fit an SM.
 // Every wait on an mbarrier is bounded in time; one that runs out raises an error flag, every role leaves its loop, copies in
 // flight get a fixed time, and tensor memory is freed.
 #include <cuda.h>

@@ -216,13 +216,18 @@ def decode_form(n_seqs: int, n_kv_heads: int, context_class: int, window: int = 
     heads over 8 KV heads of 128, int8:  1 sequence of 2,000 keys 12x1 1.83, 12x4 1.63, 12x8 1.58, 4x8 1.64; of 8,000 12x8 1.78,
     12x1x18 2.39, 4x1x18 1.74; of 32,000 12x8 2.46, 12x1x18 2.74, 4x1x18 2.30, 4x1x37 2.05;  4 of 2,000 12x2 1.79, 12x4 2.47, 4x4
     1.79, of 8,000 12x2 2.43, 4x4 2.40;  8 of 512 12x1 1.66, 4x1 1.77, of 2,000 12x1 2.10, 12x2 2.46, 4x2 2.03, 4x4 1.90, of 8,000 12x1
-    3.40, 12x2 3.15, 4x4 2.52;  16 of 2,000 12x1 2.39, 4x1 2.64, 4x2 2.32;  32 of 1,000 12x1 2.94, 4x1 2.78."""
+    3.40, 12x2 3.15, 4x4 2.52;  16 of 2,000 12x1 2.39, 4x1 2.64, 4x2 2.32;  32 of 1,000 12x1 2.94, 4x1 2.78.
+    A pair's parts are joined by one warp a row, and a CTA of 8,000 keys split over 296 has no tile for most warps: no more than half as many
+    as there are SMs (us a call, one sequence of 8,000, 32,000, 120,000 keys: 16 heads over 1 of 128 with 37 CTAs 15.5, 24.2, 56.1, 74 18.0,
+    23.5, 39.7, 296 39.7, 41.8, 47.4; 16 over 2 with 37 12.6, 19.6, 45.1, 74 15.8, 19.9, 32.4, 148 23.7, 26.5, 37.3).  Heads do not enter
+    otherwise: with heads of 64, calls alone are faster with twelve warps than by this rule (32 over 8 heads, 8 of 8,000 keys 27 instead
+    of 38, 16 of 2,000 15 instead of 21), with heads of 128 it is within 20 % of the fastest form for 8 and 16 KV heads."""
     sms = sm_count or ops.sm_count()
     pairs = n_seqs * n_kv_heads
     if window and abs(window) <= 1536:             # no more than the second class of contexts is seen
         context_class = min(context_class, 1 if abs(window) > 768 else 0)
     if context_class >= 3 and pairs * 8 <= sms:
-        return 4, 1, 2 * sms // pairs
+        return 4, 1, min(2 * sms // pairs, sms // 2)
     if context_class >= 1:
         if pairs * 16 <= sms:
             return 12, 8, 1
